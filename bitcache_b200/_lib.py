@@ -22,6 +22,8 @@ BC_RES_NONE, BC_RES_FP16_SCALE, BC_RES_FP32_SCALE = 0, 1, 2
 BC_MODE_BINARY, BC_MODE_COMPENSATED = 0, 1
 BC_DEVERR_TIMEOUT = 1
 BC_DEVERR_PAGE = 2
+BC_DEVERR_INDEX = 4
+BC_DTYPE_F16, BC_DTYPE_BF16, BC_DTYPE_F32 = 0, 1, 2
 
 c_void_p = ctypes.c_void_p
 c_int = ctypes.c_int
@@ -41,6 +43,20 @@ class PageTable(ctypes.Structure):
 
     _fields_ = [("pages", c_void_p), ("max_pages", ctypes.c_int32), ("page_size", ctypes.c_int32),
                 ("n_pages", ctypes.c_int32)]
+
+
+class Heads(ctypes.Structure):
+    """bc_heads: head rows of a strided tensor (strides in elements)."""
+
+    _fields_ = [("data", c_void_p), ("token_stride", c_int64), ("head_stride", c_int64)]
+
+
+class Rope(ctypes.Structure):
+    """bc_rope: rotation tables and norm weights."""
+
+    _fields_ = [("cos", c_void_p), ("sin", c_void_p), ("q_weight", c_void_p), ("k_weight", c_void_p),
+                ("n_positions", c_int64), ("rotary_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("eps", c_float)]
 
 
 class CopySeg(ctypes.Structure):
@@ -104,6 +120,11 @@ _SIGS = {
                                      c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "bc_append_kv_paged": (c_int, [c_void_p, c_void_p, KVPlanes, KVPlanes, PageTable, c_int, c_int, c_int64, c_int,
                                    c_void_p]),
+    "bc_qk_norm_rope": (c_int, [Heads, Heads, c_void_p, Rope, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int,
+                                c_int, c_void_p]),
+    "bc_append_qkv_paged": (c_int, [Heads, Heads, Heads, c_void_p, c_void_p, Rope, c_void_p, KVPlanes, KVPlanes,
+                                    PageTable, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,
+                                    c_void_p]),
     "bc_decode_noalloc_max_scratch_bytes": (c_size_t, []),
     "bc_decode_attention_noalloc": (c_int, [c_void_p, KVPlanes, KVPlanes, c_void_p, c_void_p, c_int, c_int, c_int,
                                             c_int64, c_int, c_int, c_void_p]),

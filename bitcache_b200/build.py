@@ -4,7 +4,8 @@ Each CUDA source under csrc/ is compiled with nvcc for sm_100a only and linked
 into ``bitcache_b200/libbitcache_b200.so`` next to this file.  The flags match
 the reference build (``-O3 --use_fast_math``): the encoders rely on the same
 fast-math division as the reference kernels to produce bit-identical INT4
-codes and scales.
+codes and scales.  Sources in IEEE_SOURCES are compiled without fast-math:
+their results are defined by correctly rounded operations.
 
 Usage: ``python -m bitcache_b200.build`` (rebuilds what changed).
 """
@@ -24,8 +25,8 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libbitcache_b200.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-NVCC_FLAGS = ["-O3", "--use_fast_math", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
-              "-I", INCLUDE, "-I", CSRC]
+NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-I", INCLUDE, "-I", CSRC]
+IEEE_SOURCES = ("rope.cu",)
 
 
 def nvcc() -> str:
@@ -47,7 +48,8 @@ def _stale(target: str, deps: list[str]) -> bool:
 def _compile(src: str, extra: list[str]) -> str:
     obj = os.path.join(BUILD, os.path.basename(src) + ".o")
     if _stale(obj, [src] + _deps()):
-        cmd = [nvcc(), *ARCH, *NVCC_FLAGS, *extra, "-c", src, "-o", obj]
+        fast = [] if os.path.basename(src) in IEEE_SOURCES else ["--use_fast_math"]
+        cmd = [nvcc(), *ARCH, *NVCC_FLAGS, *fast, *extra, "-c", src, "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"nvcc failed for {src}:\n{r.stderr}")

@@ -363,6 +363,131 @@ def append_kv_paged(k: torch.Tensor, v: torch.Tensor, K: Planes, V: Planes, pt: 
                                       residual_mode, _stream(k)), "append_kv_paged")
 
 
+_DTYPES = {torch.float16: _lib.BC_DTYPE_F16, torch.bfloat16: _lib.BC_DTYPE_BF16, torch.float32: _lib.BC_DTYPE_F32}
+
+
+class Rope:
+    """Rotation tables and per-head norm weights (bc_rope), made once per layer.
+
+    cos, sin  fp32 CUDA [n_positions, rotary_dim / 2]; both None: no rotation
+    q_weight, k_weight  RMS-norm weights, any float type, CUDA [head_dim]; None: no norm
+    interleaved  pairs of adjacent elements instead of elements rotary_dim / 2 apart"""
+
+    def __init__(self, cos: torch.Tensor | None, sin: torch.Tensor | None, interleaved: bool = False,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None,
+                 eps: float = 1e-6) -> None:
+        if (cos is None) != (sin is None):
+            raise RuntimeError("cos and sin must both be given, or neither")
+        if cos is not None:
+            for t, name in ((cos, "cos"), (sin, "sin")):
+                if not (t.is_cuda and t.is_contiguous() and t.dtype == torch.float32 and t.dim() == 2):
+                    raise RuntimeError(f"{name} must be a contiguous float32 CUDA tensor [n_positions, rotary_dim / 2]")
+            if cos.shape != sin.shape:
+                raise RuntimeError("cos and sin must have the same shape")
+        self.cos, self.sin, self.interleaved, self.eps = cos, sin, bool(interleaved), float(eps)
+        self.q_weight, self.k_weight = (None if w is None else w.float().contiguous() for w in (q_weight, k_weight))
+        n, half = (0, 0) if cos is None else cos.shape
+        self._c = _lib.Rope(_lib.ptr(cos), _lib.ptr(sin), _lib.ptr(self.q_weight), _lib.ptr(self.k_weight), n,
+                            2 * half, 1 if interleaved else 0, self.eps)
+
+    def c(self, head_dim: int) -> _lib.Rope:
+        if self._c.rotary_dim > head_dim:
+            raise RuntimeError(f"rotary_dim {self._c.rotary_dim} exceeds head_dim {head_dim}")
+        for w in (self.q_weight, self.k_weight):
+            if w is not None and not (w.is_cuda and w.numel() == head_dim):
+                raise RuntimeError(f"norm weights must be CUDA tensors of {head_dim} elements")
+        return self._c
+
+
+def _heads(x: torch.Tensor, name: str, n_tokens: int, head_dim: int, dtype: torch.dtype) -> _lib.Heads:
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+    if x.dim() != 3 or x.shape[0] != n_tokens or x.shape[2] != head_dim:
+        raise RuntimeError(f"{name} must be [n_tokens, heads, head_dim]")
+    if x.dtype != dtype:
+        raise RuntimeError(f"{name} must be {dtype} like the others")
+    if head_dim > 1 and x.stride(2) != 1:
+        raise RuntimeError(f"{name}: the elements of a head must be contiguous")
+    return _lib.Heads(x.data_ptr(), x.stride(0), x.stride(1))
+
+
+def _index(x: torch.Tensor, name: str, n: int) -> int:
+    if not (x.is_cuda and x.dtype == torch.int32 and x.is_contiguous() and x.numel() == n):
+        raise RuntimeError(f"{name} must be a contiguous int32 CUDA tensor of {n} elements")
+    return x.data_ptr()
+
+
+def _like(x: torch.Tensor | None, name: str, shape: tuple, dtypes, device: torch.device) -> torch.Tensor:
+    if x is None:
+        return torch.empty(shape, dtype=dtypes[0], device=device)
+    if not (x.is_cuda and x.is_contiguous() and tuple(x.shape) == shape and x.dtype in dtypes):
+        raise RuntimeError(f"{name} must be a contiguous CUDA tensor {shape} of {' or '.join(map(str, dtypes))}")
+    return x
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rope: Rope,
+                 q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Per-head RMS norm and position rotation of queries and keys in one pass (bc_qk_norm_rope).
+
+    q [n_tokens, n_heads, head_dim], k [n_tokens, n_kv_heads, head_dim], fp16, bf16 or fp32;
+    token and head strides are free (slices of a packed projection).  positions int32
+    [n_tokens]; a negative one marks a padding token, whose rows come back zero.  Outputs are
+    contiguous, of the inputs' type unless q_out and k_out (of one type) are given."""
+    n, _, d = q.shape
+    cq, ck = _heads(q, "q", n, d, q.dtype), _heads(k, "k", n, d, q.dtype)
+    if q.dtype not in _DTYPES:
+        raise RuntimeError("q and k must be float16, bfloat16 or float32")
+    types = tuple(_DTYPES) if q_out is not None else (q.dtype,)
+    q_out = _like(q_out, "q_out", tuple(q.shape), types, q.device)
+    k_out = _like(k_out, "k_out", tuple(k.shape), (q_out.dtype,), q.device)
+    _lib.check(_lib.load().bc_qk_norm_rope(cq, ck, _index(positions, "positions", n), rope.c(d), q_out.data_ptr(),
+                                           k_out.data_ptr(), n, q.shape[1], k.shape[1], d, _DTYPES[q.dtype],
+                                           _DTYPES[q_out.dtype], _stream(q)), "qk_norm_rope")
+    return q_out, k_out
+
+
+def append_qkv_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, K: Planes, V: Planes, pt: PageTable,
+                     seq_ids: torch.Tensor, positions: torch.Tensor, rope: Rope,
+                     residual_mode: int = RES_FP32_SCALE, q_out: torch.Tensor | None = None,
+                     want_hat: bool = False) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Norm and rotation of queries and keys as qk_norm_rope, and the append of the keys and of
+    the values to a paged cache, in one launch (bc_append_qkv_paged).
+
+    Token t (q [n_tokens, n_heads, d], k and v [n_tokens, n_kv_heads, d]) is position
+    positions[t] of sequence seq_ids[t]; pt has n_seqs * n_kv_heads rows.  Tokens of any mix of
+    sequences, prompts or single steps.  Returns the rotated queries, fp16 [n_tokens, n_heads,
+    d], and with want_hat also k_hat and v_hat, fp16 [n_tokens, n_kv_heads, d]: the rows as the
+    cache now holds them, for a prompt's own attention."""
+    n, hq, d = q.shape
+    hkv = k.shape[1] if k.dim() == 3 else 0
+    cq, ck, cv = (_heads(x, name, n, d, q.dtype) for x, name in ((q, "q"), (k, "k"), (v, "v")))
+    if q.dtype not in _DTYPES:
+        raise RuntimeError("q, k and v must be float16, bfloat16 or float32")
+    if v.shape[1] != hkv or hkv == 0 or pt.n_slots % hkv:
+        raise RuntimeError("k and v must have the same heads, and the block table a row for each of a sequence's")
+    if K.head_dim != d or V.head_dim != d:
+        raise RuntimeError(f"the cache holds vectors of {K.head_dim} elements, not {d}")
+    if residual_mode != RES_NONE and not (K.compensated and V.compensated):
+        raise RuntimeError("a residual mode needs compensated (residual) caches")
+    _check_pool(K, V, pt)
+    q_out = _like(q_out, "q_out", (n, hq, d), (torch.float16,), q.device)
+    hats = [torch.empty((n, hkv, d), dtype=torch.float16, device=q.device) for _ in range(2 * want_hat)]
+    kh, vh = (h.data_ptr() for h in hats) if want_hat else (None, None)
+    _lib.check(_lib.load().bc_append_qkv_paged(cq, ck, cv, _index(seq_ids, "seq_ids", n),
+                                               _index(positions, "positions", n), rope.c(d), q_out.data_ptr(), K.c(),
+                                               V.c(), pt.c(), kh, vh, n, pt.n_slots // hkv, hq, hkv, d,
+                                               _DTYPES[q.dtype], residual_mode, _stream(q)), "append_qkv_paged")
+    return (q_out, *hats) if want_hat else q_out
+
+
+def _check_pool(K: Planes, V: Planes, pt: PageTable) -> None:
+    for P in (K, V):
+        if P.n_slots != pt.n_pages or P.kv_stride != pt.page_size:
+            raise RuntimeError(f"the pool holds {P.n_slots} pages of {P.kv_stride} positions, "
+                               f"the block table names {pt.n_pages} of {pt.page_size}")
+
+
 def decode_attention_entropy(q: torch.Tensor, K: Planes, V: Planes, seq_len: int, mode: int = MODE_COMPENSATED,
                              out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Decode attention and, from the same pass, the per-head entropy of the softmax

@@ -64,11 +64,18 @@ extern "C" {
 #define BC_DEVERR_TIMEOUT 1u /* a bounded wait in a kernel gave up; outputs are invalid */
 #define BC_DEVERR_PAGE 2u    /* a block-table entry named a page outside the pool; that tile
                                 was not read or written and the outputs are invalid */
+#define BC_DEVERR_INDEX 4u   /* a token position, sequence id or length lay outside its table;
+                                see the operation for what became of it */
 
 /* residual modes for the encoders */
 #define BC_RES_NONE 0       /* binary only: sign + bscale */
 #define BC_RES_FP16_SCALE 1 /* residual against the fp16-rounded scale (reference residual.cu:28) */
 #define BC_RES_FP32_SCALE 2 /* residual against the fp32 scale (reference online_encode.cu:74) */
+
+/* element types of the operations that take activations in a model's own type */
+#define BC_DTYPE_F16 0
+#define BC_DTYPE_BF16 1
+#define BC_DTYPE_F32 2
 
 /* attention modes */
 #define BC_MODE_BINARY 0      /* xnor-popcount scores, sign*scale values (binary_attention.cu) */
@@ -224,6 +231,60 @@ int bc_decode_step_paged(const void* q, const void* new_k, const void* new_v, bc
 /* bc_append_kv into a paged cache at logical position pos of every slot. */
 int bc_append_kv_paged(const void* k, const void* v, bc_kv_planes K, bc_kv_planes V, bc_page_table pt, int n_slots,
                        int head_dim, int64_t pos, int residual_mode, void* stream);
+
+/* ---- norms and rotation of queries and keys, alone and on append -------
+ * No counterpart in the reference, whose callers rotate before append.
+ * A head row x (head_dim elements) of a token at position p:
+ *   norm      y_i = (x_i * r) * w_i, r = 1 / sqrt(sum(x^2) / head_dim + eps); q_weight /
+ *             k_weight NULL: no norm (of queries / of keys).  Values are never normed.
+ *   rotation  of the first rotary_dim elements, in pairs (i, j): j = i + rotary_dim / 2,
+ *             or adjacent elements (2n, 2n + 1) when interleaved != 0;
+ *             z_i = y_i cos - y_j sin, z_j = y_j cos + y_i sin with the tables' row p;
+ *             cos and sin NULL: no rotation.  Values are never rotated.
+ * All in fp32, each operation rounded on its own, sums in the encoders' tree
+ * order (stride 128, 64, ..., 1), divisions and the root correctly rounded.
+ * Inputs are strided: element (token t, head h, i) at data[t * token_stride +
+ * h * head_stride + i], strides in elements, so q, k and v may be slices of one
+ * packed projection.  Positions are int32 device memory.  A negative position
+ * marks a padding token: its output rows are zero and nothing is cached.  So
+ * does a position at or past n_positions, which also raises BC_DEVERR_INDEX. */
+typedef struct bc_heads {
+    const void* data;
+    int64_t token_stride;
+    int64_t head_stride;
+} bc_heads;
+typedef struct bc_rope {
+    const float* cos; /* device fp32 [n_positions][rotary_dim / 2], or NULL */
+    const float* sin;
+    const float* q_weight; /* device fp32 [head_dim], or NULL */
+    const float* k_weight;
+    int64_t n_positions;
+    int32_t rotary_dim;  /* even, 2 .. head_dim */
+    int32_t interleaved;
+    float eps;
+} bc_rope;
+
+/* q_out [n_tokens][n_heads][head_dim] and k_out [n_tokens][n_kv_heads][head_dim] of out_dtype;
+ * dtype and out_dtype are BC_DTYPE_*.  q_out may be q and k_out may be k where an input is
+ * itself laid out like its output and of the same type.  n_heads or n_kv_heads may be 0. */
+int bc_qk_norm_rope(bc_heads q, bc_heads k, const int32_t* positions, bc_rope rope, void* q_out, void* k_out,
+                    int64_t n_tokens, int n_heads, int n_kv_heads, int head_dim, int dtype, int out_dtype,
+                    void* stream);
+
+/* The same for the queries (q_out fp16), and in the same launch the normed, rotated keys and
+ * the values of the tokens are encoded (not rounded to fp16 first) into the paged caches K
+ * and V: token t is position positions[t] of sequence seq_ids[t], whose kv head h owns row
+ * seq * n_kv_heads + h of the block table (n_seqs * n_kv_heads rows).  Any mix of sequences
+ * and positions, prompts and single tokens; a position given twice in one call holds either
+ * token.  The arithmetic is bc_append_kv's with correctly rounded divisions.  A sequence id
+ * outside [0, n_seqs) or a position past the table raises BC_DEVERR_INDEX, a page outside
+ * the pool BC_DEVERR_PAGE; that token (or its rows of that head) is treated as padding.
+ * k_hat, v_hat: both NULL, or fp16 [n_tokens][n_kv_heads][head_dim] receiving the rows as the
+ * cache now holds them (sign * bscale + code / 7 * rscale), for a prompt's own attention. */
+int bc_append_qkv_paged(bc_heads q, bc_heads k, bc_heads v, const int32_t* seq_ids, const int32_t* positions,
+                        bc_rope rope, void* q_out, bc_kv_planes K, bc_kv_planes V, bc_page_table pt, void* k_hat,
+                        void* v_hat, int64_t n_tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
+                        int dtype, int residual_mode, void* stream);
 
 /* ---- compact adaptive caches (per-position adaptive precision) ----------
  * bc_select_positions_topk: like bc_select_residual_topk, but one choice per
