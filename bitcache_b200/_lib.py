@@ -125,6 +125,9 @@ _SIGS = {
     "bc_append_qkv_paged": (c_int, [Heads, Heads, Heads, c_void_p, c_void_p, Rope, c_void_p, KVPlanes, KVPlanes,
                                     PageTable, c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,
                                     c_void_p]),
+    "bc_decode_shared_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "bc_decode_attention_shared": (c_int, [c_void_p, KVPlanes, KVPlanes, PageTable, c_void_p, c_void_p, c_void_p,
+                                           c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_size_t, c_void_p]),
     "bc_decode_noalloc_max_scratch_bytes": (c_size_t, []),
     "bc_decode_attention_noalloc": (c_int, [c_void_p, KVPlanes, KVPlanes, c_void_p, c_void_p, c_int, c_int, c_int,
                                             c_int64, c_int, c_int, c_void_p]),

@@ -481,6 +481,48 @@ def append_qkv_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, K: Plane
     return (q_out, *hats) if want_hat else q_out
 
 
+def decode_attention_shared(q: torch.Tensor, K: Planes, V: Planes, pt: PageTable, seq_lens: torch.Tensor,
+                            prefix_lens: torch.Tensor | None = None, mode: int = MODE_COMPENSATED,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention of a ragged batch over a paged cache, shared prefixes read once
+    (bc_decode_attention_shared).
+
+    q fp16 [n_seqs, n_heads, head_dim]; pt has n_seqs * n_kv_heads rows (n_heads a multiple of
+    n_kv_heads); seq_lens int32 CUDA [n_seqs].  prefix_lens int32 CUDA [n_groups] splits the
+    sequences into n_groups equal runs that hold the same rows at positions below their
+    group's prefix length (the same pages, or copies of them).  Returns fp16 like q."""
+    _check_half(q, "Q")
+    if q.dim() != 3:
+        raise RuntimeError("Q must be [n_seqs, n_heads, head_dim]")
+    n, heads, d = q.shape
+    if n and pt.n_slots % n:
+        raise RuntimeError("the block table must have a row for each kv head of each sequence")
+    hkv = pt.n_slots // n if n else 1
+    if hkv == 0 or heads % hkv:
+        raise RuntimeError("n_heads must be a multiple of the block table's kv heads")
+    if K.head_dim != d or V.head_dim != d:
+        raise RuntimeError(f"the cache holds vectors of {K.head_dim} elements, not {d}")
+    if mode == MODE_COMPENSATED and not (K.compensated and V.compensated):
+        raise RuntimeError("compensated attention needs compensated (residual) caches")
+    _check_pool(K, V, pt)
+    groups = n if prefix_lens is None else prefix_lens.numel()
+    if n and (groups == 0 or n % groups):
+        raise RuntimeError("prefix_lens must split the sequences into equal groups")
+    out = _like(out, "out", (n, heads, d), (torch.float16,), q.device)
+    lens = _index(seq_lens, "seq_lens", n)
+    pre = None if prefix_lens is None else _index(prefix_lens, "prefix_lens", groups)
+    if n == 0:
+        return out
+    lib = _lib.load()
+    st = _stream(q)
+    group = heads // hkv
+    ws = _lib.workspace(q.device, st, lib.bc_decode_shared_workspace_bytes(n, groups, hkv, group, d), ("shared",))
+    _lib.check(lib.bc_decode_attention_shared(q.data_ptr(), K.c(), V.c(), pt.c(), lens, pre, out.data_ptr(), n, groups,
+                                              hkv, group, d, mode, _lib.ptr(ws), ws.numel() if ws is not None else 0,
+                                              st), "decode_attention_shared")
+    return out
+
+
 def _check_pool(K: Planes, V: Planes, pt: PageTable) -> None:
     for P in (K, V):
         if P.n_slots != pt.n_pages or P.kv_stride != pt.page_size:

@@ -286,6 +286,26 @@ int bc_append_qkv_paged(bc_heads q, bc_heads k, bc_heads v, const int32_t* seq_i
                         void* v_hat, int64_t n_tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
                         int dtype, int residual_mode, void* stream);
 
+/* ---- batches that share prefixes, and ragged lengths ---------------------
+ * Decode attention (bc_decode_attention's scores and values) of n_seqs sequences over a
+ * paged cache, one query token each: q, out fp16 [n_seqs][n_kv_heads * group][head_dim];
+ * query head h of sequence b reads row b * n_kv_heads + h / group of the block table,
+ * keys [0, seq_lens[b]).  Lengths are int32 device memory, so a captured graph follows
+ * them.  The sequences form n_groups equal runs; positions below prefix_lens[g] hold the
+ * same rows in every sequence of group g (a common prompt: the same pages, or copies; not
+ * checked) and are read once for the whole group, through the block table of its first
+ * sequence.  prefix_lens NULL: nothing is shared.  A prefix may end anywhere in a page.
+ * A length of 0 gives zeros; a sequence shorter than its group's prefix attends its own
+ * length of it.  Lengths outside [0, max_pages * page_size] are cut to it and raise
+ * BC_DEVERR_INDEX; a page id outside the pool raises BC_DEVERR_PAGE and its keys are left
+ * out.  head_dim 32, 64, 128 or 256, any group.  The workspace needs no clearing; calls
+ * that overlap on the GPU must not share one.  No counterpart in the reference. */
+size_t bc_decode_shared_workspace_bytes(int n_seqs, int n_groups, int n_kv_heads, int group, int head_dim);
+int bc_decode_attention_shared(const void* q, bc_kv_planes K, bc_kv_planes V, bc_page_table pt,
+                               const int32_t* seq_lens, const int32_t* prefix_lens, void* out, int n_seqs,
+                               int n_groups, int n_kv_heads, int group, int head_dim, int mode, void* workspace,
+                               size_t workspace_bytes, void* stream);
+
 /* ---- compact adaptive caches (per-position adaptive precision) ----------
  * bc_select_positions_topk: like bc_select_residual_topk, but one choice per
  * position for K and V together, keyed by the fp32 sum of the K and V keys;
