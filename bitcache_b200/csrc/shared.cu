@@ -7,22 +7,31 @@
 // n and scales bs, rs, value likewise:
 //   s   = (bs mean|q| (sgn q . sgn k) + rs / 7 (q . n)) / sqrt(d)
 //   out = sum_s softmax(s) (bs_v sgn v + rs_v / 7 n_v)
-// Work is a flat list of units, one unit being one 128-key tile for one block of
-// up to 8 query rows of one kv head ("item": a prefix of a group, or the rest of
-// a sequence).  The grid divides the list evenly, so ragged lengths need no plan
-// on the host; a CTA's stretch of an item is a piece, whose record (U, l, o)
-// k_shared_merge joins with the row's other pieces.
+// Work is a flat list: an item is one block of up to 8 query rows of one kv head
+// against a prefix of a group or the rest of a sequence, in tiles of 32 keys.
+// The warps of the grid divide the list evenly, each item weighing its tiles and
+// a constant for its start and end, so ragged lengths need no plan on the host.
+// A warp's stretch of an item is a piece, whose record (U, l, o) k_shared_merge
+// joins with the row's other pieces.  A warp works alone: its own ring of tiles
+// (cp.async), its own softmax state, no barrier but the one after the list's
+// sums.  (With the four warps of a CTA on the 32-key quarters of one tile, the
+// merge and the barriers at every piece cost more than the products of a short
+// sequence: 51 of 84 us busy at 16 sequences of 8192 shared and 64 own keys.)
 //
 // Rows are the narrow side of every product (mma.sync m16n8k16, fp16 in, fp32
 // accumulators): the 16 rows of A are keys in the scores and dims in the values,
 // the 8 columns of B are query rows.  A is built in registers from the packed
-// bytes, two instructions per pair of elements and no scale: sign bits become
-// +-1, codes n become the fp16 numbers 24 + n (the nibble n + 8 in the mantissa
-// of 16), whose constant part 24 sum(b) is subtracted at the end.  A key's
-// scales multiply its few scores, and its probabilities before they become the
-// value product's B operand: P1 = e bs, P2 = e rs / 7, rounded to fp16.  They
-// keep at least 11 significant bits down to 2^-22 of a row's largest one: e is
-// 2^(s - U) with U such that the largest P lies between 2^8 and 2^15.
+// bytes: masked in place, a sign bit or nibble is an fp16 subnormal, 2^(p - 24)
+// times its value at bit position p.  For the scores that is A already (the
+// powers of two go into the query's side, the offset 8 of the codes and the 0/1
+// of the sign bits into a constant per row); for the values one fma makes it the
+// signed number times 2^-10, so that the long sums stay centred: the tensor
+// cores cut what they add to, and with the offset left in, a sum over 200000
+// keys lost 3%.  A key's scales multiply its few scores, and its probabilities
+// before they become the value product's B operand: P1 = e bs, P2 = e rs / 7,
+// rounded to fp16.  They keep at least 11 significant bits down to 2^-22 of a
+// row's largest one: e is 2^(s - U) with U such that the largest P lies between
+// 2^8 and 2^15.
 #include "common.cuh"
 
 namespace bc {
@@ -30,10 +39,12 @@ namespace {
 
 constexpr int kShThreads = 128;
 constexpr int kShWarps = kShThreads / 32;
-constexpr int kShTile = 128;   // keys per unit: 32 per warp
-constexpr int kShRows = 8;     // query rows per unit
+constexpr int kShTile = 32;        // keys per tile
+constexpr int kShRows = 8;         // query rows per item
 constexpr int kShStages = 2;
-constexpr int kShMaxCtas = 148 * 8;  // bound of the grid, for the workspace's size
+constexpr int kShItemCost = 2;     // an item's start and end, in tiles
+constexpr int kShMinTiles = 1;     // least weight a worker is given
+constexpr int kShMaxWorkers = 148 * 16;  // bound of the workers, for the workspace's size
 constexpr float kShLog2e = 1.4426950408889634f;
 constexpr float kShNone = -1e30f;  // U of a row without keys
 
@@ -49,7 +60,8 @@ struct SharedArgs {
     int n_seqs, n_groups, per;  // per: sequences of a group
     int n_kv, group;
     int prefix_blocks, own_blocks;  // blocks of 8 query rows of a prefix item / of a sequence's own item
-    int n_ctas;
+    int n_workers;
+    bool q_aligned;  // q on a 16-byte boundary
 };
 
 template <int D, bool COMP>
@@ -62,15 +74,12 @@ struct ShCfg {
     static constexpr int NIB_OFF = SIGN_B;
     static constexpr int BS_OFF = SIGN_B + NIB_B;
     static constexpr int RS_OFF = BS_OFF + SC_B;
-    static constexpr int STAGE_B = 2 * HALF_B;
-    static constexpr int MG_B = 2 * kShRows * (D + 4) * 4;  // two warps' records
-    static constexpr int Q_OFF = kShStages * STAGE_B;
-    static constexpr int Q_B = kShRows * (D + 8) * 2;
-    static constexpr int MG_OFF = Q_OFF + Q_B;
-    static constexpr int SCAN_OFF = MG_OFF + MG_B;
-    static constexpr int SCAN_B = (kShThreads + 1) * 8 + 32;
-    static constexpr int BAR_OFF = (SCAN_OFF + SCAN_B + 15) / 16 * 16;
-    static constexpr int SMEM_B = BAR_OFF + 2 * kShStages * 8 + kShStages * 4 + 16 + 128;
+    static constexpr int Q_ROW = 2 * D + 16;  // padded: the rows' 2-byte reads spread over the banks
+    static constexpr int Q_OFF = 2 * HALF_B;  // the query rows, with the first tile of an item
+    static constexpr int STAGE_B = Q_OFF + kShRows * Q_ROW;
+    static constexpr int WARP_B = kShStages * STAGE_B;
+    static constexpr int SCAN_OFF = kShWarps * WARP_B;
+    static constexpr int SMEM_B = SCAN_OFF + (kShThreads + 1) * 8 + 8;
 };
 
 __host__ __device__ constexpr int sh_record_floats(int d) { return kShRows * (d + 4); }
@@ -94,6 +103,7 @@ struct ShEntry {
     int lo, hi;  // key positions
     int tile0, tiles;
     int blocks;
+    __device__ __forceinline__ int weight() const { return tiles ? tiles + kShItemCost : 0; }  // of one item
 };
 __device__ __forceinline__ ShEntry sh_entry(const SharedArgs& a, int e) {
     ShEntry x;
@@ -111,8 +121,8 @@ __device__ __forceinline__ ShEntry sh_entry(const SharedArgs& a, int e) {
     x.tiles = x.hi > x.lo ? (x.hi + kShTile - 1) / kShTile - x.tile0 : 0;
     return x;
 }
-__device__ __forceinline__ int64_t sh_units(const SharedArgs& a, const ShEntry& x) {
-    return (int64_t)x.tiles * x.blocks * a.n_kv;
+__device__ __forceinline__ int64_t sh_weight(const SharedArgs& a, const ShEntry& x) {
+    return (int64_t)x.weight() * x.blocks * a.n_kv;
 }
 __device__ __forceinline__ int64_t sh_first_item(const SharedArgs& a, int e) {
     return e < a.n_groups ? (int64_t)e * a.n_kv * a.prefix_blocks
@@ -120,13 +130,14 @@ __device__ __forceinline__ int64_t sh_first_item(const SharedArgs& a, int e) {
                                 (int64_t)(e - a.n_groups) * a.n_kv * a.own_blocks;
 }
 
-// Exclusive sums of the entries' units over the CTA's threads (each thread a
+// Exclusive sums of the entries' weights over the CTA's threads (each thread a
 // run of consecutive entries) in scan[0 .. kShThreads]; scan[kShThreads] is the total.
 __device__ __forceinline__ int64_t sh_scan(const SharedArgs& a, int64_t* scan) {
     const int n = a.n_groups + a.n_seqs, chunk = (n + kShThreads - 1) / kShThreads;
     const int lane = threadIdx.x & 31;
     int64_t sum = 0;
-    for (int e = threadIdx.x * chunk; e < min(n, ((int)threadIdx.x + 1) * chunk); ++e) sum += sh_units(a, sh_entry(a, e));
+    for (int e = threadIdx.x * chunk; e < min(n, ((int)threadIdx.x + 1) * chunk); ++e)
+        sum += sh_weight(a, sh_entry(a, e));
     scan[threadIdx.x] = sum;
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -153,38 +164,40 @@ __device__ __forceinline__ int64_t sh_scan(const SharedArgs& a, int64_t* scan) {
 }
 static_assert(kShThreads == 128, "sh_scan: four sums per lane");
 
-// CTA c's units: [sh_begin(c), sh_begin(c + 1)), n = min(CTAs, units) so that
-// none of the n is empty.  A piece's record is number item + CTA: along the list
-// every new piece raises one of the two.
-__device__ __forceinline__ int64_t sh_begin(int64_t units, int n, int64_t c) { return units * c / n; }
-__device__ __forceinline__ int sh_cta_of(int64_t units, int n, int64_t u) {
-    return (int)(((u + 1) * n + units - 1) / units) - 1;
+// Worker w's stretch of the list: weights [sh_begin(w), sh_begin(w + 1)).  Within
+// an item the first kShItemCost units stand for its start and end, the others
+// for its tiles.  A piece's record is number item + worker: along the list every
+// new piece raises one of the two.
+__device__ __forceinline__ int sh_workers(const SharedArgs& a, int64_t total) {
+    return (int)min((int64_t)a.n_workers, (total + kShMinTiles - 1) / kShMinTiles);
+}
+__device__ __forceinline__ int64_t sh_begin(int64_t total, int n, int64_t w) { return total * w / n; }
+__device__ __forceinline__ int sh_worker_of(int64_t total, int n, int64_t at) {
+    return (int)(((at + 1) * n + total - 1) / total) - 1;
+}
+__device__ __forceinline__ int sh_tile_at(int64_t at_in_item, int tiles) {
+    return (int)max((int64_t)0, min((int64_t)tiles, at_in_item - kShItemCost));
 }
 
-// Position in the list; every thread keeps its own copy.
+// Position in the list; every lane keeps its own copy.
 struct ShCursor {
     int e;
     ShEntry x;
     int h, blk, tile;  // tile: index within the item
 };
-__device__ __forceinline__ void sh_seek(const SharedArgs& a, ShCursor& c, int e, int64_t at) {
-    c.e = e;
-    c.x = sh_entry(a, e);
-    c.tile = (int)(at % c.x.tiles);
-    const int64_t it = at / c.x.tiles;
-    c.blk = (int)(it % c.x.blocks);
-    c.h = (int)(it / c.x.blocks);
-}
-// Next unit; true when it begins another item.  Never called on the last unit.
-__device__ __forceinline__ bool sh_next(const SharedArgs& a, ShCursor& c) {
-    if (++c.tile < c.x.tiles) return false;
+__device__ __forceinline__ void sh_next_item(const SharedArgs& a, ShCursor& c) {
     c.tile = 0;
-    if (++c.blk < c.x.blocks) return true;
+    if (++c.blk < c.x.blocks) return;
     c.blk = 0;
-    if (++c.h < a.n_kv) return true;
+    if (++c.h < a.n_kv) return;
     c.h = 0;
     do c.x = sh_entry(a, ++c.e);
     while (c.x.tiles == 0);
+}
+// Next tile; true when it begins another item.  Never called on the list's last tile.
+__device__ __forceinline__ bool sh_next(const SharedArgs& a, ShCursor& c) {
+    if (++c.tile < c.x.tiles) return false;
+    sh_next_item(a, c);
     return true;
 }
 
@@ -203,39 +216,56 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
 __device__ __forceinline__ void sh_ldsm4(const uint8_t* row, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(smem_u32(row)));
+                 : "r"(smem_u32(row)) : "memory");
 }
 // Two 16x16 byte matrices, transposed: lanes 0-15 / 16-31 give the rows of the
 // first / second; lane (g, q) gets bytes g and g + 8 of rows 4q .. 4q + 3.
 __device__ __forceinline__ void sh_ldsm_t2(const uint8_t* row, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(smem_u32(row)));
+                 : "r"(smem_u32(row)) : "memory");
 }
 __device__ __forceinline__ void sh_ldsm_t1(const uint8_t* row, uint32_t& r0, uint32_t& r1) {
     asm volatile("ldmatrix.sync.aligned.m16n16.x1.trans.shared.b8 {%0,%1}, [%2];"
                  : "=r"(r0), "=r"(r1)
-                 : "r"(smem_u32(row)));
+                 : "r"(smem_u32(row)) : "memory");
 }
-// Bits i and i + 16 of w as +-1 (1 for a set bit).
-__device__ __forceinline__ uint32_t pm1(uint32_t w, int left) { return ((w << left) & 0x80008000u) ^ 0xBC00BC00u; }
-// Nibbles at bits 0-3 and 16-19 of (w shifted) as 16 + u = 24 + code.
-__device__ __forceinline__ uint32_t code24_l(uint32_t w, int left) { return ((w << left) & 0x03C003C0u) | 0x4C004C00u; }
-__device__ __forceinline__ uint32_t code24_r(uint32_t w, int right) { return ((w >> right) & 0x03C003C0u) | 0x4C004C00u; }
-// Nibbles t and t + 4 (t < 4).
-__device__ __forceinline__ uint32_t code24(uint32_t w, int t) { return t < 2 ? code24_l(w, 6 - 4 * t) : code24_r(w, 4 * t - 6); }
+__device__ __forceinline__ void sh_cp16(uint8_t* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
 
+// fp16 pairs.  2^e, e in [-14, 15], in both halves:
+__device__ constexpr uint32_t pow2_h2(int e) { return (uint32_t)(e + 15) * 0x04000400u; }
+__device__ __forceinline__ uint32_t fma_h2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+// Value operands carry the factor 2^-10 (kShValue undoes it).
+constexpr float kShValue = 1024.0f;
+// Bits t and t + 16 of w (t <= 9) as +-2^-10: b 2^(t - 24) -> b 2^-9 - 2^-10.
+__device__ __forceinline__ uint32_t sign_h2(uint32_t w, int t) {
+    return fma_h2(w & (0x00010001u << t), pow2_h2(15 - t), 0x8000'8000u | pow2_h2(-10));
+}
+// Nibbles at bits 0-3 and 16-19 (hi: 4-7 and 20-23) of w, code + 8, as code 2^-10.
+__device__ __forceinline__ uint32_t code_h2(uint32_t w, int hi) {
+    return fma_h2(w & (hi ? 0x00F000F0u : 0x000F000Fu), pow2_h2(hi ? 10 : 14), 0x8000'8000u | pow2_h2(-7));
+}
 
 // The query rows as B operands, and what the scores need of each row.
+// A pair of sign bits at position p is worth 2^(p - 24): its +-1 is +-2^(9 - p)
+// here, the product's unit 2^-15.  A nibble at bits 0-3 / 4-7 is worth 2^-24 /
+// 2^-20: its q is 16 q / q times a power of two u that puts the row's largest
+// element at 2^10 .. 2^11, the product's unit 2^-20 / u.
 template <int D, bool COMP>
 struct ShQuery {
     uint32_t sign[D / 16][2];
     uint32_t code[COMP ? D / 16 : 1][2];
-    float bco[2], rco[2], off[2];  // rows 2q, 2q + 1: score = bs bco D1 + rs rco (D2 - off)
+    float bco[2], boff[2], rco[2], roff[2];  // rows 2q, 2q + 1: score = bs (bco D1 - boff) + rs (rco D2 - roff)
 };
 
 // Dim of element `half` (0, 1) of register r of k step s in the sign part / code part, lane column q.
@@ -246,64 +276,78 @@ __device__ __forceinline__ int sign_dim(int s, int r, int half, int q) {
     if constexpr (D == 64) return 32 * (q / 2) + 8 * (q % 2) + p + 16 * half;
     return 4 * q + p + 16 * half;  // D == 32
 }
+// Where pair p (of 16 in a word) is masked: in place, or 6 lower in the word shifted by 6.
+__device__ constexpr int sign_pos(int p) { return p % 16 < 10 ? p % 16 : p % 16 - 6; }
 template <int D>
 __device__ __forceinline__ int code_dim(int s, int r, int half, int q) {
     const int c = s / 2, n = 2 * (s % 2) + r + 4 * half;  // chunk, nibble of its word q
     return nib_dim(D, c, 4 * q + n / 2, n % 2);
 }
 
+// Query rows of the cursor's item: count, and the first one's sequence.
+__device__ __forceinline__ void sh_rows(const SharedArgs& a, const ShCursor& c, int& rows, int& b0) {
+    const bool prefix = c.e < a.n_groups;
+    rows = prefix ? a.per * a.group : a.group;
+    b0 = prefix ? c.e * a.per : c.e - a.n_groups;
+}
+
 template <int D, bool COMP>
-__device__ __forceinline__ void sh_load_query(const SharedArgs& a, const ShCursor& c, uint8_t* smem,
+__device__ __forceinline__ void sh_load_query(const SharedArgs& a, const ShCursor& c, const uint8_t* qrows,
                                               ShQuery<D, COMP>& Q, int (&hi)[2], int& hi_min) {
     using C = ShCfg<D, COMP>;
-    constexpr int ROW = D + 8;
-    __half* qs = reinterpret_cast<__half*>(smem + C::Q_OFF);
     const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3;
-    const bool prefix = c.e < a.n_groups;
-    const int rows = prefix ? a.per * a.group : a.group;
-    const int b0 = prefix ? c.e * a.per : c.e - a.n_groups;
-    __syncthreads();  // the previous item's rows are read
-    for (int i = threadIdx.x; i < kShRows * D; i += kShThreads) {
-        const int r = c.blk * kShRows + i / D;
-        __half v = __float2half(0.0f);
-        if (r < rows)
-            v = a.q[((int64_t)(b0 + r / a.group) * a.n_kv * a.group + (int64_t)c.h * a.group + r % a.group) * D + i % D];
-        qs[(i / D) * ROW + i % D] = v;
-    }
-    __syncthreads();
-    const __half* row = qs + g8 * ROW;
-    float sum = 0.0f, mag = 0.0f;
+    int rows, b0;
+    sh_rows(a, c, rows, b0);
+    const bool live = c.blk * kShRows + g8 < rows;
+    const __half* row = reinterpret_cast<const __half*>(qrows + g8 * C::Q_ROW);
+    float sum = 0.0f, mag = 0.0f, top = 0.0f, sgn = 0.0f;
 #pragma unroll
     for (int s = 0; s < D / 16; ++s)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            const __half x0 = row[sign_dim<D>(s, r, 0, q)], x1 = row[sign_dim<D>(s, r, 1, q)];
-            const float f0 = __half2float(x0), f1 = __half2float(x1);
-            Q.sign[s][r] = (f0 >= 0.0f ? 0x3C00u : 0xBC00u) | (f1 >= 0.0f ? 0x3C000000u : 0xBC000000u);
+            const float f0 = live ? __half2float(row[sign_dim<D>(s, r, 0, q)]) : 0.0f;
+            const float f1 = live ? __half2float(row[sign_dim<D>(s, r, 1, q)]) : 0.0f;
+            Q.sign[s][r] = pow2_h2(9 - sign_pos(2 * s + r)) | (f0 >= 0.0f ? 0u : 0x8000u) | (f1 >= 0.0f ? 0u : 0x80000000u);
             mag += fabsf(f0) + fabsf(f1);
             sum += f0 + f1;
-            if constexpr (COMP) {
-                const uint32_t y0 = __half_as_ushort(row[code_dim<D>(s, r, 0, q)]);
-                const uint32_t y1 = __half_as_ushort(row[code_dim<D>(s, r, 1, q)]);
-                Q.code[s][r] = y0 | (y1 << 16);
-            }
+            sgn += (f0 >= 0.0f ? 1.0f : -1.0f) + (f1 >= 0.0f ? 1.0f : -1.0f);
+            top = fmaxf(top, fmaxf(fabsf(f0), fabsf(f1)));
         }
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
         mag += __shfl_xor_sync(0xffffffffu, mag, o);
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        sgn += __shfl_xor_sync(0xffffffffu, sgn, o);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    }
+    // u: the largest element to 2^10 .. 2^11 (a row of zeros, or with an infinity: 1)
+    const int ex = (__float_as_int(top) >> 23) - 127;
+    const float u = top > 0.0f && ex < 16 ? exp2i(10 - ex) : 1.0f;
+    if constexpr (COMP) {
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float w = r == 0 ? 16.0f * u : u;  // r = 0: nibbles 0-3 and 16-19 of the word, or of it shifted by 8
+                const float f0 = live ? __half2float(row[code_dim<D>(s, r, 0, q)]) : 0.0f;
+                const float f1 = live ? __half2float(row[code_dim<D>(s, r, 1, q)]) : 0.0f;
+                Q.code[s][r] = pack_h2(f0 * w, f1 * w);
+            }
     }
     const float scale = kShLog2e * rsqrtf((float)D);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const float m = __shfl_sync(0xffffffffu, mag, 4 * (2 * q + j));
-        const float t = __shfl_sync(0xffffffffu, sum, 4 * (2 * q + j));
-        Q.bco[j] = m * (1.0f / D) * scale;
-        Q.rco[j] = scale * (1.0f / 7.0f);
-        Q.off[j] = 24.0f * t;
+        const int from = 4 * (2 * q + j);
+        const float m = __shfl_sync(0xffffffffu, mag, from) * (1.0f / D) * scale;
+        const float t = __shfl_sync(0xffffffffu, sum, from) * scale * (8.0f / 7.0f);
+        const float w = __shfl_sync(0xffffffffu, u, from);
+        Q.bco[j] = m * 65536.0f;  // sgn q . sgn k = 2 sum(sgn q bit) - sum(sgn q), in units of 2^-15
+        Q.boff[j] = m * __shfl_sync(0xffffffffu, sgn, from);
+        Q.rco[j] = scale * (1.0f / 7.0f) * 1048576.0f / w;
+        Q.roff[j] = t;
         const int r = c.blk * kShRows + 2 * q + j;
         // a sequence shorter than its group's prefix sees its own length of it
-        hi[j] = prefix && r < rows ? min(c.x.hi, sh_len(a, b0 + r / a.group)) : c.x.hi;
+        hi[j] = c.e < a.n_groups && r < rows ? min(c.x.hi, sh_len(a, b0 + r / a.group)) : c.x.hi;
     }
     hi_min = (int)__reduce_min_sync(0xffffffffu, (unsigned)min(hi[0], hi[1]));
 }
@@ -313,7 +357,7 @@ __device__ __forceinline__ void sh_load_query(const SharedArgs& a, const ShCurso
 template <int D>
 struct ShState {
     float o[D / 16][4];
-    float U[2], l[2], t[2];  // per row 2q, 2q + 1: unit, partial sums of e and of P2 over this lane's keys
+    float U[2], l[2];  // per row 2q, 2q + 1: unit, and the sum of e over this lane's keys
 };
 template <int D>
 __device__ __forceinline__ void sh_clear(ShState<D>& st) {
@@ -321,11 +365,8 @@ __device__ __forceinline__ void sh_clear(ShState<D>& st) {
     for (int m = 0; m < D / 16; ++m)
 #pragma unroll
         for (int i = 0; i < 4; ++i) st.o[m][i] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-        st.U[j] = kShNone;
-        st.l[j] = st.t[j] = 0.0f;
-    }
+    st.U[0] = st.U[1] = kShNone;
+    st.l[0] = st.l[1] = 0.0f;
 }
 
 // Position of matrix row r (0 .. 15) of a transposing load among its 16 keys:
@@ -333,10 +374,10 @@ __device__ __forceinline__ void sh_clear(ShState<D>& st) {
 // the elements 2q + 8, 2q + 9.
 __device__ __forceinline__ int sh_key_of_row(int r) { return 2 * (r >> 2) + ((r >> 1) & 1) + 8 * (r & 1); }
 
-// One warp's 32 keys (k0 .. k0 + 31 of the tile at key position kpos) of a stage.
+// The 32 keys of a tile at key position kpos.
 template <int D, bool COMP>
-__device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>& st, const uint8_t* sb, int k0,
-                                           int kpos, int lo, const int (&hi)[2], bool masked) {
+__device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>& st, const uint8_t* sb, int kpos,
+                                           int lo, const int (&hi)[2], bool masked) {
     using C = ShCfg<D, COMP>;
     constexpr int NW = C::NW;
     const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3;
@@ -345,7 +386,7 @@ __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>
     // ---- scores of two blocks of 16 keys
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-        const int kb = k0 + 16 * b;
+        const int kb = 16 * b;
         float d1[4] = {0.f, 0.f, 0.f, 0.f}, d2[4] = {0.f, 0.f, 0.f, 0.f};
         {
             constexpr int PAIRS = D / 8;  // pairs of dims per lane
@@ -363,16 +404,16 @@ __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>
                 }
             }
 #pragma unroll
-            for (int st2 = 0; st2 < PAIRS / 2; ++st2) {
-                const int p = 2 * st2;
-                mma_f16(d1, pm1(w[0][p / 16], 15 - p % 16), pm1(w[1][p / 16], 15 - p % 16),
-                        pm1(w[0][p / 16], 14 - p % 16), pm1(w[1][p / 16], 14 - p % 16), Q.sign[st2][0],
-                        Q.sign[st2][1]);
+            for (int k = 0; k < PAIRS / 2; ++k) {
+                const int i = 2 * k / 16, p = 2 * k % 16;  // pairs p, p + 1 of word i
+                const uint32_t w0 = p < 10 ? w[0][i] : w[0][i] >> 6, w1 = p < 10 ? w[1][i] : w[1][i] >> 6;
+                const uint32_t m0 = 0x00010001u << sign_pos(p), m1 = m0 << 1;
+                mma_f16(d1, w0 & m0, w1 & m0, w0 & m1, w1 & m1, Q.sign[k][0], Q.sign[k][1]);
             }
         }
         if constexpr (COMP) {
             const uint8_t* nib = ks + C::NIB_OFF + (kb >> 3) * 4 * D;
-            // word q of chunk c of key g8 (blk 0) and g8 + 8 (blk 1)
+            // word q of chunk c of key g8 (x = 0) and g8 + 8 (x = 1)
             uint32_t n[NW][2];
             if constexpr (NW >= 4) {
 #pragma unroll
@@ -393,11 +434,13 @@ __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>
                     for (int c = 0; c < NW; ++c) n[c][x] = r[x * NW + c];
             }
 #pragma unroll
-            for (int c = 0; c < NW; ++c)
-#pragma unroll
-                for (int t = 0; t < 4; t += 2)
-                    mma_f16(d2, code24(n[c][0], t), code24(n[c][1], t), code24(n[c][0], t + 1), code24(n[c][1], t + 1),
-                            Q.code[2 * c + t / 2][0], Q.code[2 * c + t / 2][1]);
+            for (int c = 0; c < NW; ++c) {
+                mma_f16(d2, n[c][0] & 0x000F000Fu, n[c][1] & 0x000F000Fu, n[c][0] & 0x00F000F0u, n[c][1] & 0x00F000F0u,
+                        Q.code[2 * c][0], Q.code[2 * c][1]);
+                const uint32_t y0 = n[c][0] >> 8, y1 = n[c][1] >> 8;
+                mma_f16(d2, y0 & 0x000F000Fu, y1 & 0x000F000Fu, y0 & 0x00F000F0u, y1 & 0x00F000F0u,
+                        Q.code[2 * c + 1][0], Q.code[2 * c + 1][1]);
+            }
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -406,8 +449,8 @@ __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>
             const float rs = COMP ? __half2float(reinterpret_cast<const __half*>(ks + C::RS_OFF)[key]) : 0.0f;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float v = bs * (Q.bco[j] * d1[2 * x + j]);
-                if constexpr (COMP) v += rs * (Q.rco[j] * (d2[2 * x + j] - Q.off[j]));
+                float v = bs * (Q.bco[j] * d1[2 * x + j] - Q.boff[j]);
+                if constexpr (COMP) v += rs * (Q.rco[j] * d2[2 * x + j] - Q.roff[j]);
                 s[b][2 * x + j] = v;
             }
         }
@@ -418,7 +461,7 @@ __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>
     for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const int key = k0 + 16 * b + g8 + 8 * x;
+            const int key = 16 * b + g8 + 8 * x;
             vb[b][x] = __half2float(reinterpret_cast<const __half*>(vs + C::BS_OFF)[key]);
             vr[b][x] = COMP ? __half2float(reinterpret_cast<const __half*>(vs + C::RS_OFF)[key]) * (1.0f / 7.0f) : 0.0f;
             // 2^grow bounds the larger scale; a key whose scales are next to 0 does not pull U down by more than 2^40
@@ -440,7 +483,6 @@ __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>
             const float f = exp2f(st.U[j] - U);
             st.U[j] = U;
             st.l[j] *= f;
-            st.t[j] *= f;
 #pragma unroll
             for (int mt = 0; mt < D / 16; ++mt) {
                 st.o[mt][j] *= f;
@@ -454,27 +496,20 @@ __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>
         uint32_t p1[2], p2[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            float e[2], c1[2], c2[2];
+            float c1[2], c2[2];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const float v = s[b][2 * x + j];
-                e[j] = exp2f(v - st.U[j]);
-                st.l[j] += e[j];
+                const float e = exp2f(v - st.U[j]);
+                st.l[j] += e;
                 const bool out = masked && v == -INFINITY;  // a masked row's scales may be anything
-                c1[j] = out ? 0.0f : e[j] * vb[b][x];
-                c2[j] = out ? 0.0f : e[j] * vr[b][x];
+                c1[j] = out ? 0.0f : e * vb[b][x];
+                c2[j] = out ? 0.0f : e * vr[b][x];
             }
-            p1[x] = pack_h2(c1[0], c1[1]);
-            if constexpr (COMP) {
-                p2[x] = pack_h2(c2[0], c2[1]);
-                const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&p2[x]));
-                st.t[0] += r.x;
-                st.t[1] += r.y;
-                p2[x] = movmatrix(p2[x]);
-            }
-            p1[x] = movmatrix(p1[x]);
+            p1[x] = movmatrix(pack_h2(c1[0], c1[1]));
+            if constexpr (COMP) p2[x] = movmatrix(pack_h2(c2[0], c2[1]));
         }
-        const int kb = k0 + 16 * b;
+        const int kb = 16 * b;
         const int key = kb + sh_key_of_row(lane & 15);
         uint32_t sg[D >= 256 ? 4 : 2], wd[4];
         if constexpr (D == 128) {
@@ -491,7 +526,7 @@ __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                wd[i] = reinterpret_cast<const uint32_t*>(vs)[kb + sh_key_of_row(4 * q + i)];
+                wd[i] = reinterpret_cast<const uint32_t*>(vs)[kb + sh_key_of_row(4 * q + i)] >> (2 * g8);
         }
 #pragma unroll
         for (int c = 0; c < NW; c += 2) {
@@ -509,125 +544,59 @@ __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>
                     uint32_t a0, a1, a2, a3;
                     if constexpr (D >= 128) {
                         const int w = (c + cx) / 4, t = (c + cx) % 4 + 4 * h;
-                        a0 = pm1(sg[2 * w], 15 - t);
-                        a1 = pm1(sg[2 * w + 1], 15 - t);
-                        a2 = pm1(sg[2 * w], 7 - t);
-                        a3 = pm1(sg[2 * w + 1], 7 - t);
+                        a0 = sign_h2(sg[2 * w], t);
+                        a1 = sign_h2(sg[2 * w + 1], t);
+                        a2 = sign_h2(sg[2 * w] >> 8, t);
+                        a3 = sign_h2(sg[2 * w + 1] >> 8, t);
                     } else if constexpr (D == 64) {
                         const int t = 2 * (c + cx) + 4 * h;
-                        a0 = pm1(sg[0], 15 - t);
-                        a1 = pm1(sg[0], 14 - t);
-                        a2 = pm1(sg[0], 7 - t);
-                        a3 = pm1(sg[0], 6 - t);
+                        a0 = sign_h2(sg[0], t);
+                        a1 = sign_h2(sg[0], t + 1);
+                        a2 = sign_h2(sg[0] >> 8, t);
+                        a3 = sign_h2(sg[0] >> 8, t + 1);
                     } else {
-                        const int left = 15 - 2 * g8 - h;
-                        a0 = pm1(__byte_perm(wd[0], wd[2], 0x5410), left);
-                        a1 = pm1(__byte_perm(wd[0], wd[2], 0x7632), left);
-                        a2 = pm1(__byte_perm(wd[1], wd[3], 0x5410), left);
-                        a3 = pm1(__byte_perm(wd[1], wd[3], 0x7632), left);
+                        a0 = sign_h2(__byte_perm(wd[0], wd[2], 0x5410), h);
+                        a1 = sign_h2(__byte_perm(wd[0], wd[2], 0x7632), h);
+                        a2 = sign_h2(__byte_perm(wd[1], wd[3], 0x5410), h);
+                        a3 = sign_h2(__byte_perm(wd[1], wd[3], 0x7632), h);
                     }
                     mma_f16(o, a0, a1, a2, a3, p1[0], p1[1]);
                     if constexpr (COMP) {
                         const uint32_t x0 = r[2 * cx], x1 = r[2 * cx + 1];
-                        if (h == 0)
-                            mma_f16(o, code24_l(x0, 6), code24_l(x1, 6), code24_r(x0, 2), code24_r(x1, 2), p2[0], p2[1]);
-                        else
-                            mma_f16(o, code24_l(x0, 2), code24_l(x1, 2), code24_r(x0, 6), code24_r(x1, 6), p2[0], p2[1]);
+                        mma_f16(o, code_h2(x0, h), code_h2(x1, h), code_h2(x0 >> 8, h), code_h2(x1 >> 8, h), p2[0], p2[1]);
                     }
                 }
         }
     }
 }
 
-// Join the four warps' sums and write the piece's record:
-// floats [8 rows][D] o, then [8 rows][2] (U, l).
-template <int D, bool COMP>
-__device__ __forceinline__ void sh_flush(const SharedArgs& a, ShState<D>& st, uint8_t* smem, int64_t record) {
-    using C = ShCfg<D, COMP>;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g8 = lane >> 2, q = lane & 3;
+// The piece's record: rows of D + 4 floats, o then (U, l).
+template <int D>
+__device__ __forceinline__ void sh_flush(const SharedArgs& a, ShState<D>& st, int64_t record) {
+    const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3;
+    float* m = a.ws + record * sh_record_floats(D);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
+        float l = st.l[j];
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-            st.l[j] += __shfl_xor_sync(0xffffffffu, st.l[j], o);
-            st.t[j] += __shfl_xor_sync(0xffffffffu, st.t[j], o);
-        }
-        if constexpr (COMP) {
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        float* row = m + (2 * q + j) * (D + 4);
 #pragma unroll
-            for (int mt = 0; mt < D / 16; ++mt) {
-                st.o[mt][j] -= 24.0f * st.t[j];
-                st.o[mt][2 + j] -= 24.0f * st.t[j];
-            }
+        for (int mt = 0; mt < D / 16; ++mt) {
+            row[nib_dim(D, mt / 2, g8, mt % 2)] = st.o[mt][j] * kShValue;
+            row[nib_dim(D, mt / 2, g8 + 8, mt % 2)] = st.o[mt][2 + j] * kShValue;
         }
+        if (g8 == 0) *reinterpret_cast<float2*>(row + D) = make_float2(st.U[j], l);
     }
-    constexpr int REC = kShRows * (D + 4);
-    auto put = [&](float* m) {  // [2q + j][dim], rows D + 4 floats apart; (U, l) behind each row
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            float* row = m + (2 * q + j) * (D + 4);
-#pragma unroll
-            for (int mt = 0; mt < D / 16; ++mt) {
-                row[nib_dim(D, mt / 2, g8, mt % 2)] = st.o[mt][j];
-                row[nib_dim(D, mt / 2, g8 + 8, mt % 2)] = st.o[mt][2 + j];
-            }
-            if (g8 == 0) {
-                row[D] = st.U[j];
-                row[D + 1] = st.l[j];
-            }
-        }
-    };
-    auto add = [&](const float* m) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float* row = m + (2 * q + j) * (D + 4);
-            const float U = fmaxf(st.U[j], row[D]), f = exp2f(st.U[j] - U), g = exp2f(row[D] - U);
-            st.U[j] = U;
-            st.l[j] = st.l[j] * f + row[D + 1] * g;
-#pragma unroll
-            for (int mt = 0; mt < D / 16; ++mt) {
-                st.o[mt][j] = st.o[mt][j] * f + row[nib_dim(D, mt / 2, g8, mt % 2)] * g;
-                st.o[mt][2 + j] = st.o[mt][2 + j] * f + row[nib_dim(D, mt / 2, g8 + 8, mt % 2)] * g;
-            }
-        }
-    };
-    float* mg = reinterpret_cast<float*>(smem + C::MG_OFF);
-    if (warp >= 2) put(mg + (warp - 2) * REC);
-    __syncthreads();
-    if (warp < 2) add(mg + warp * REC);
-    __syncthreads();
-    if (warp == 1) put(mg);
-    __syncthreads();
-    if (warp == 0) {
-        add(mg);
-        put(a.ws + record * REC);
-    }
-}
-
-__device__ __forceinline__ void sh_arrive(uint64_t* bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 template <int D, bool COMP>
 __global__ void __launch_bounds__(kShThreads) k_shared_rows(const SharedArgs a) {
     using C = ShCfg<D, COMP>;
-    extern __shared__ __align__(128) uint8_t sh_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sh_raw) + 127) & ~uintptr_t(127));
+    extern __shared__ __align__(128) uint8_t smem[];
     int64_t* scan = reinterpret_cast<int64_t*>(smem + C::SCAN_OFF);
-    int64_t* found = scan + kShThreads + 1;  // entry and unit within it of the CTA's first unit
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);
-    uint64_t* empty = full + kShStages;
-    int* present = reinterpret_cast<int*>(empty + kShStages);  // per stage: its page is in the pool
-    const int tid = threadIdx.x, warp = tid >> 5;
-
-    if (tid == 0) {
-        for (int s = 0; s < kShStages; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], kShWarps);
-        }
-        fence_mbar_init();
-    }
-    const int64_t units = sh_scan(a, scan);
-    const int n_ctas = (int)min((int64_t)a.n_ctas, units);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int64_t total = sh_scan(a, scan);
     if (blockIdx.x == 0) {  // lengths outside the block table are cut, and said so
         const int64_t cap = (int64_t)a.pt.max_pages * a.pt.page_size;
         for (int b = tid; b < a.n_seqs; b += kShThreads)
@@ -636,117 +605,147 @@ __global__ void __launch_bounds__(kShThreads) k_shared_rows(const SharedArgs a) 
             for (int g = tid; g < a.n_groups; g += kShThreads)
                 if (a.prefix_lens[g] < 0 || a.prefix_lens[g] > cap) raise_device_error(a.err, BC_DEVERR_INDEX);
     }
-    if ((int)blockIdx.x >= n_ctas) return;
-    const int64_t u0 = sh_begin(units, n_ctas, blockIdx.x), u1 = sh_begin(units, n_ctas, blockIdx.x + 1);
-    if (scan[tid] <= u0 && u0 < scan[tid + 1]) {
+    const int n_workers = sh_workers(a, total);
+    const int worker = blockIdx.x * kShWarps + warp;
+    if (worker >= n_workers) return;
+    const int64_t w0 = sh_begin(total, n_workers, worker), w1 = sh_begin(total, n_workers, worker + 1);
+
+    // the entry that holds w0: the thread's run by bisection, then along it
+    ShCursor cur;
+    int64_t left = w1 - w0;  // weight of the stretch from the cursor's tile on
+    {
+        int run = 0;
+#pragma unroll
+        for (int step = kShThreads / 2; step; step >>= 1)
+            if (scan[run + step] <= w0) run += step;
         const int n = a.n_groups + a.n_seqs, chunk = (n + kShThreads - 1) / kShThreads;
-        int64_t at = u0 - scan[tid];
-        int e = tid * chunk;
-        for (;; ++e) {
-            const int64_t w = sh_units(a, sh_entry(a, e));
+        int64_t at = w0 - scan[run];
+        cur.e = run * chunk;
+        for (;; ++cur.e) {
+            cur.x = sh_entry(a, cur.e);
+            const int64_t w = sh_weight(a, cur.x);
             if (at < w) break;
             at -= w;
         }
-        found[0] = e;
-        found[1] = at;
+        const int64_t it = at / cur.x.weight();
+        cur.blk = (int)(it % cur.x.blocks);
+        cur.h = (int)(it / cur.x.blocks);
+        const int in = (int)(at - it * cur.x.weight());
+        cur.tile = sh_tile_at(in, cur.x.tiles);
+        left -= max(0, kShItemCost - in);
     }
-    __syncthreads();
-    ShCursor cur, ahead;
-    sh_seek(a, cur, (int)found[0], found[1]);
-    ahead = cur;
-
-    const int n_units = (int)(u1 - u0);
-    auto issue = [&](int it) {  // thread 0: the tile `ahead` points at, into stage it % kShStages
-        const int s = it % kShStages;
-        uint8_t* dst = smem + s * C::STAGE_B;
+    if (left <= 0) return;  // the stretch ends within its first item's start
+    // Number of tiles of the stretch, item by item (later items cost kShItemCost before their first tile).
+    uint8_t* ring = smem + warp * C::WARP_B;
+    ShCursor ahead = cur;
+    int64_t ahead_left = left;  // weight left at `ahead`, > 0 while it points at a tile of the stretch
+    bool ahead_new = true;      // the query rows travel with the first tile of each piece
+    unsigned present = 0;       // bit s: the page of stage s is in the pool
+    auto issue = [&](int s) {
+        uint8_t* dst = ring + s * C::STAGE_B;
         const int seq = ahead.e < a.n_groups ? ahead.e * a.per : ahead.e - a.n_groups;
-        const int64_t pos = (int64_t)(ahead.x.tile0 + ahead.tile) * kShTile;
+        const int pos = (ahead.x.tile0 + ahead.tile) * kShTile;
         const int pg = __ldg(a.pt.pages + ((int64_t)seq * a.n_kv + ahead.h) * a.pt.max_pages + pos / a.pt.page_size);
-        const bool ok = pg >= 0 && pg < a.pt.n_pages;
-        present[s] = ok;
-        if (!ok) {
-            raise_device_error(a.err, BC_DEVERR_PAGE);
-            sh_arrive(&full[s]);
-            return;
+        if (pg >= 0 && pg < a.pt.n_pages) {
+            present |= 1u << s;
+            const int64_t row = (int64_t)pg * a.pt.page_size + pos % a.pt.page_size;
+            auto part = [&](const bc_kv_planes& P, uint8_t* d) {
+#pragma unroll
+                for (int i = lane * 16; i < C::SIGN_B; i += 512) sh_cp16(d + i, (const uint8_t*)P.sign + row * (D / 8) + i);
+                if constexpr (COMP) {
+#pragma unroll
+                    for (int i = lane * 16; i < C::NIB_B; i += 512)
+                        sh_cp16(d + C::NIB_OFF + i, (const uint8_t*)P.nib + row * (D / 2) + i);
+                }
+                constexpr int SC = C::SC_B / 16;
+                if (lane < SC * (COMP ? 2 : 1)) {
+                    const uint8_t* src = (const uint8_t*)(lane < SC ? P.bscale : P.rscale) + row * 2 + (lane % SC) * 16;
+                    sh_cp16(d + C::BS_OFF + lane * 16, src);
+                }
+            };
+            part(a.K, dst);
+            part(a.V, dst + C::HALF_B);
+        } else {
+            present &= ~(1u << s);
+            if (lane == 0) raise_device_error(a.err, BC_DEVERR_PAGE);
         }
-        const int64_t row = (int64_t)pg * a.pt.page_size + pos % a.pt.page_size;
-        mbar_arrive_expect_tx(&full[s], C::STAGE_B);
-        auto part = [&](const bc_kv_planes& P, uint8_t* d) {
-            bulk_g2s(d, (const uint8_t*)P.sign + row * (D / 8), C::SIGN_B, &full[s]);
-            bulk_g2s(d + C::BS_OFF, (const uint8_t*)P.bscale + row * 2, C::SC_B, &full[s]);
-            if constexpr (COMP) {
-                bulk_g2s(d + C::NIB_OFF, (const uint8_t*)P.nib + row * (D / 2), C::NIB_B, &full[s]);
-                bulk_g2s(d + C::RS_OFF, (const uint8_t*)P.rscale + row * 2, C::SC_B, &full[s]);
+        if (ahead_new) {
+            int rows, b0;
+            sh_rows(a, ahead, rows, b0);
+            for (int i = lane; i < kShRows * (D / 8); i += 32) {
+                const int r = ahead.blk * kShRows + i / (D / 8), at = i % (D / 8) * 8;
+                if (r >= rows) break;
+                const __half* src =
+                    a.q + (((int64_t)(b0 + r / a.group) * a.n_kv + ahead.h) * a.group + r % a.group) * D + at;
+                uint8_t* to = dst + C::Q_OFF + i / (D / 8) * C::Q_ROW + 2 * at;
+                if (a.q_aligned)
+                    sh_cp16(to, src);
+                else
+                    for (int k = 0; k < 8; ++k) reinterpret_cast<__half*>(to)[k] = src[k];
             }
-        };
-        part(a.K, dst);
-        part(a.V, dst + C::HALF_B);
-    };
-    int issued = 0;
-    if (tid == 0)
-        for (; issued < min(kShStages, n_units); ++issued) {
-            if (issued) sh_next(a, ahead);
-            issue(issued);
         }
+    };
+    auto advance = [&]() {  // `ahead` to the next tile of the stretch, or ahead_left <= 0
+        ahead_left -= 1;
+        ahead_new = false;
+        if (ahead_left > 0 && ++ahead.tile == ahead.x.tiles) {
+            ahead_left -= kShItemCost;
+            if (ahead_left > 0) {
+                sh_next_item(a, ahead);
+                ahead_new = true;
+            }
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < kShStages; ++s) {
+        if (ahead_left > 0) {
+            issue(s);
+            advance();
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
 
     ShQuery<D, COMP> Q;
     ShState<D> st;
     int hi[2], hi_min;
-    sh_load_query<D, COMP>(a, cur, smem, Q, hi, hi_min);
-    sh_clear(st);
-    bool alive = true;
-    for (int it = 0; it < n_units; ++it) {
-        const int s = it % kShStages;
-        const uint32_t phase = (uint32_t)(it / kShStages) & 1u;
-        if (it > 0 && sh_next(a, cur)) {
-            sh_load_query<D, COMP>(a, cur, smem, Q, hi, hi_min);
+    bool begin = true;
+    for (int s = 0;; s = s + 1 == kShStages ? 0 : s + 1) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kShStages - 1) : "memory");
+        __syncwarp();
+        const uint8_t* sb = ring + s * C::STAGE_B;
+        if (begin) {
+            sh_load_query<D, COMP>(a, cur, sb + C::Q_OFF, Q, hi, hi_min);
             sh_clear(st);
         }
-        // refill the stage that the previous unit left, once all warps have
-        if (tid == 0 && it > 0 && issued < n_units) {
-            const int ps = (it - 1) % kShStages;
-            if (alive && mbar_wait_bounded(&empty[ps], (uint32_t)((it - 1) / kShStages) & 1u)) {
-                fence_proxy_async_smem();
-                sh_next(a, ahead);
-                issue(issued++);
-            } else if (alive) {
-                raise_device_error(a.err, BC_DEVERR_TIMEOUT);
-                alive = false;
-            }
-        }
-        alive = __all_sync(0xffffffffu, alive);
-        alive = __all_sync(0xffffffffu, alive && mbar_wait_bounded(&full[s], phase));
-        if (alive) {
-            const int kpos = (cur.x.tile0 + cur.tile) * kShTile;
-            const bool here = present[s] != 0;
-            if (here)
-                sh_consume<D, COMP>(Q, st, smem + s * C::STAGE_B, 32 * warp, kpos, cur.x.lo, hi,
-                                    kpos < cur.x.lo || kpos + kShTile > hi_min);
-        } else if ((tid & 31) == 0) {
-            raise_device_error(a.err, BC_DEVERR_TIMEOUT);
-        }
+        const int kpos = (cur.x.tile0 + cur.tile) * kShTile;
+        if (present >> s & 1) sh_consume<D, COMP>(Q, st, sb, kpos, cur.x.lo, hi, kpos < cur.x.lo || kpos + kShTile > hi_min);
         __syncwarp();
-        if ((tid & 31) == 0) sh_arrive(&empty[s]);
-        const bool last = it + 1 == n_units || cur.tile + 1 == cur.x.tiles;
-        if (last) {
-            const int64_t item = sh_first_item(a, cur.e) + (int64_t)cur.h * cur.x.blocks + cur.blk;
-            sh_flush<D, COMP>(a, st, smem, item + blockIdx.x);
+        if (ahead_left > 0) {
+            issue(s);
+            advance();
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        left -= 1;
+        begin = cur.tile + 1 == cur.x.tiles;
+        if (begin || left <= 0) {
+            const int64_t item = sh_first_item(a, cur.e) + (int64_t)cur.h * cur.x.blocks + cur.blk;
+            sh_flush<D>(a, st, item + worker);
+            if (begin) left -= kShItemCost;
+            if (left <= 0) break;
+        }
+        sh_next(a, cur);
     }
-    if (!alive && tid == 0)  // gave up: let the copies in flight land (bounded) before the memory is reused
-        for (int i = max(0, issued - kShStages); i < issued; ++i)
-            mbar_wait_bounded(&full[i % kShStages], (uint32_t)(i / kShStages) & 1u);
 }
 
 // One CTA per (sequence, kv head): joins the pieces of each query row.
 template <int D>
 __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a) {
-    constexpr int REC = kShRows * (D + 4), PER = D / 32;
+    constexpr int REC = sh_record_floats(D), PER = D / 32;
     __shared__ int64_t scan[kShThreads + 1], at[2];
     const int b = blockIdx.x / a.n_kv, h = blockIdx.x % a.n_kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t units = sh_scan(a, scan);
-    const int n_ctas = (int)min((int64_t)a.n_ctas, units);
+    const int64_t total = sh_scan(a, scan);
+    const int n_workers = sh_workers(a, total);
     const int n = a.n_groups + a.n_seqs, chunk = (n + kShThreads - 1) / kShThreads;
     const int want[2] = {b / a.per, a.n_groups + b};
     ShEntry x[2];
@@ -754,7 +753,7 @@ __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a)
     for (int i = 0; i < 2; ++i) {
         if ((int)threadIdx.x == want[i] / chunk) {
             int64_t sum = scan[threadIdx.x];
-            for (int e = threadIdx.x * chunk; e < want[i]; ++e) sum += sh_units(a, sh_entry(a, e));
+            for (int e = threadIdx.x * chunk; e < want[i]; ++e) sum += sh_weight(a, sh_entry(a, e));
             at[i] = sum;
         }
         x[i] = sh_entry(a, want[i]);
@@ -770,16 +769,49 @@ __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a)
             if (x[i].tiles == 0) continue;
             const int r = i == 0 ? (b % a.per) * a.group + g : g;
             const int64_t it = (int64_t)h * x[i].blocks + r / kShRows;
-            const int64_t first = at[i] + it * x[i].tiles;
-            const int c0 = sh_cta_of(units, n_ctas, first), c1 = sh_cta_of(units, n_ctas, first + x[i].tiles - 1);
+            const int64_t first = at[i] + it * x[i].weight();
+            const int c0 = sh_worker_of(total, n_workers, first);
+            const int c1 = sh_worker_of(total, n_workers, first + x[i].weight() - 1);
             const float* rec = a.ws + (sh_first_item(a, want[i]) + it) * REC + (r % kShRows) * (D + 4);
-            for (int c = c0; c <= c1; ++c) {
-                const float* p = rec + (int64_t)c * REC;
-                const float U = fmaxf(M, p[D]), f = exp2f(M - U), w = exp2f(p[D] - U);
-                M = U;
-                L = L * f + p[D + 1] * w;
+            // 32 workers at a time: units and sums lane by lane, then the sums over dims
+            for (int base = c0; base <= c1; base += 32) {
+                const int c = base + lane;
+                bool has = c <= c1;
+                if (has)
+                    has = sh_tile_at(sh_begin(total, n_workers, c) - first, x[i].tiles) <
+                          sh_tile_at(sh_begin(total, n_workers, c + 1) - first, x[i].tiles);
+                const float2 ul = has ? *reinterpret_cast<const float2*>(rec + (int64_t)c * REC + D) : make_float2(kShNone, 0.0f);
+                float top = ul.x;
 #pragma unroll
-                for (int k = 0; k < PER; ++k) o[k] = o[k] * f + p[32 * k + lane] * w;
+                for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+                const float U = fmaxf(M, top), f = exp2f(M - U);
+                const float w = has ? exp2f(ul.x - U) : 0.0f;
+                float l = ul.y * w;
+#pragma unroll
+                for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+                M = U;
+                L = L * f + l;
+#pragma unroll
+                for (int k = 0; k < PER; ++k) o[k] *= f;
+                unsigned todo = __ballot_sync(0xffffffffu, has);
+                while (todo) {
+                    constexpr int AT_ONCE = 4;
+                    float v[AT_ONCE][PER], wt[AT_ONCE];
+#pragma unroll
+                    for (int u = 0; u < AT_ONCE; ++u) {
+                        const int src = todo ? __ffs(todo) - 1 : 0;
+                        const bool on = todo != 0;
+                        todo &= todo - 1;
+                        wt[u] = __shfl_sync(0xffffffffu, w, src);
+#pragma unroll
+                        for (int k = 0; k < PER; ++k) v[u][k] = on ? rec[(int64_t)(base + src) * REC + 32 * k + lane] : 0.0f;
+                        if (!on) wt[u] = 0.0f;
+                    }
+#pragma unroll
+                    for (int u = 0; u < AT_ONCE; ++u)
+#pragma unroll
+                        for (int k = 0; k < PER; ++k) o[k] += v[u][k] * wt[u];
+                }
             }
         }
         const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;  // no keys: zeros
@@ -789,7 +821,7 @@ __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a)
 }
 
 template <int D, bool COMP>
-int sh_ctas(int* n_ctas) {
+int sh_workers_on_device(int* n_workers) {
     constexpr int smem = ShCfg<D, COMP>::SMEM_B;
     static int cached[64] = {};
     int dev = 0;
@@ -804,17 +836,17 @@ int sh_ctas(int* n_ctas) {
             e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&occ, k_shared_rows<D, COMP>, kShThreads, smem);
         if (e != cudaSuccess) return BC_ERR_CUDA_BASE + (int)e;
         if (occ <= 0) return BC_ERR_UNSUPPORTED;
-        cached[dev] = min(sms * occ, kShMaxCtas);
+        cached[dev] = min(sms * occ * kShWarps, kShMaxWorkers);
     }
-    *n_ctas = cached[dev];
+    *n_workers = cached[dev];
     return BC_OK;
 }
 
 template <int D, bool COMP>
 int sh_run(SharedArgs& a, cudaStream_t st) {
-    const int rc = sh_ctas<D, COMP>(&a.n_ctas);
+    const int rc = sh_workers_on_device<D, COMP>(&a.n_workers);
     if (rc) return rc;
-    k_shared_rows<D, COMP><<<a.n_ctas, kShThreads, ShCfg<D, COMP>::SMEM_B, st>>>(a);
+    k_shared_rows<D, COMP><<<(a.n_workers + kShWarps - 1) / kShWarps, kShThreads, ShCfg<D, COMP>::SMEM_B, st>>>(a);
     BC_LAUNCH_CHECK();
     k_shared_merge<D><<<a.n_seqs * a.n_kv, kShThreads, 0, st>>>(a);
     BC_LAUNCH_CHECK();
@@ -826,7 +858,7 @@ bool sh_head_dim(int d) { return d == 32 || d == 64 || d == 128 || d == 256; }
 int64_t sh_records(int n_seqs, int n_groups, int n_kv, int group) {
     const int per = n_seqs / n_groups;
     const int64_t prefix = ((int64_t)per * group + kShRows - 1) / kShRows, own = (group + kShRows - 1) / kShRows;
-    return (int64_t)n_groups * n_kv * prefix + (int64_t)n_seqs * n_kv * own + kShMaxCtas;
+    return (int64_t)n_groups * n_kv * prefix + (int64_t)n_seqs * n_kv * own + kShMaxWorkers;
 }
 
 }  // namespace
@@ -870,6 +902,7 @@ int bc_decode_attention_shared(const void* q, bc_kv_planes K, bc_kv_planes V, bc
         return BC_ERR_WORKSPACE;
     SharedArgs a{};
     a.q = (const __half*)q;
+    a.q_aligned = bc_aligned(q, 16);
     a.K = K;
     a.V = V;
     a.pt = pt;

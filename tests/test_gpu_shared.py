@@ -287,6 +287,15 @@ def test_same_results_again_on_another_stream_and_in_a_graph(cuda):
     b.check(out)
 
 
+def test_queries_off_a_16_byte_boundary(cuda):
+    b = Batch(cuda, [300, 20, 150], [], 2, 4, 128, True, 128, seed=15)
+    first = b.run()
+    store = torch.empty(b.q.numel() + 1, dtype=torch.float16, device=cuda)
+    store[1:] = b.q.flatten()
+    b.q = store[1:].view(b.q.shape)
+    assert b.q.data_ptr() % 16 and torch.equal(b.run(), first)
+
+
 def test_no_prefix_equals_the_paged_step(cuda):
     b = Batch(cuda, [1000] * 4, [], 2, 4, 128, True, 128, seed=12)
     want = planes.decode_step_paged(b.q.view(-1, 128), None, None, b.K, b.V, b.pt, 1000)
