@@ -43,7 +43,6 @@ constexpr int kShTile = 32;        // keys per tile
 constexpr int kShRows = 8;         // query rows per item
 constexpr int kShStages = 2;
 constexpr int kShItemCost = 2;     // an item's start and end, in tiles
-constexpr int kShMinTiles = 1;     // least weight a worker is given
 constexpr int kShMaxWorkers = 148 * 16;  // bound of the workers, for the workspace's size
 constexpr float kShLog2e = 1.4426950408889634f;
 constexpr float kShNone = -1e30f;  // U of a row without keys
@@ -55,13 +54,22 @@ struct SharedArgs {
     const int32_t* seq_lens;
     const int32_t* prefix_lens;  // null: no prefixes
     __half* out;
-    float* ws;
     unsigned int* err;
     int n_seqs, n_groups, per;  // per: sequences of a group
     int n_kv, group;
-    int prefix_blocks, own_blocks;  // blocks of 8 query rows of a prefix item / of a sequence's own item
-    int n_workers;
     bool q_aligned;  // q on a 16-byte boundary
+};
+
+// One kernel's list of work: entries [0, n_pre) are the groups' prefixes, the
+// following n_own the sequences' own keys.  An item is one block of query rows of
+// one kv head of an entry.
+struct ShList {
+    int n_pre, n_own;
+    int pre_blocks, own_blocks;  // blocks of `rows` query rows of a prefix / of a sequence
+    int tile, rows;              // keys of a tile; query rows of a block, and of a record
+    int cost;                    // an item's start and end, in tiles
+    int n_workers;
+    float* records;
 };
 
 template <int D, bool COMP>
@@ -82,8 +90,6 @@ struct ShCfg {
     static constexpr int SMEM_B = SCAN_OFF + (kShThreads + 1) * 8 + 8;
 };
 
-__host__ __device__ constexpr int sh_record_floats(int d) { return kShRows * (d + 4); }
-
 // ---- the list of work ------------------------------------------------------
 __device__ __forceinline__ int sh_capacity(const SharedArgs& a) {
     const int64_t c = (int64_t)a.pt.max_pages * a.pt.page_size;
@@ -98,47 +104,50 @@ __device__ __forceinline__ int sh_prefix(const SharedArgs& a, int g) {
     return max(0, min(__ldg(a.prefix_lens + g), sh_capacity(a)));
 }
 
-// Entry e of the list: group e's prefix (e < n_groups), else sequence e - n_groups's own keys.
+// Entry e of a list.  A sequence shorter than its group's prefix takes no part in
+// it (its rows there are not read) and attends all of its keys on its own.
 struct ShEntry {
     int lo, hi;  // key positions
     int tile0, tiles;
     int blocks;
-    __device__ __forceinline__ int weight() const { return tiles ? tiles + kShItemCost : 0; }  // of one item
 };
-__device__ __forceinline__ ShEntry sh_entry(const SharedArgs& a, int e) {
+__device__ __forceinline__ ShEntry sh_entry(const SharedArgs& a, const ShList& L, int e) {
     ShEntry x;
-    if (e < a.n_groups) {
+    if (e < L.n_pre) {
         x.lo = 0;
         x.hi = sh_prefix(a, e);
-        x.blocks = a.prefix_blocks;
+        x.blocks = L.pre_blocks;
     } else {
-        const int b = e - a.n_groups;
-        x.lo = sh_prefix(a, b / a.per);
+        const int b = e - L.n_pre, prefix = sh_prefix(a, b / a.per);
         x.hi = sh_len(a, b);
-        x.blocks = a.own_blocks;
+        x.lo = x.hi < prefix ? 0 : prefix;
+        x.blocks = L.own_blocks;
     }
-    x.tile0 = x.lo / kShTile;
-    x.tiles = x.hi > x.lo ? (x.hi + kShTile - 1) / kShTile - x.tile0 : 0;
+    x.tile0 = x.lo / L.tile;
+    x.tiles = x.hi > x.lo ? (x.hi + L.tile - 1) / L.tile - x.tile0 : 0;
     return x;
 }
-__device__ __forceinline__ int64_t sh_weight(const SharedArgs& a, const ShEntry& x) {
-    return (int64_t)x.weight() * x.blocks * a.n_kv;
+__device__ __forceinline__ int sh_item_weight(const ShList& L, const ShEntry& x) { return x.tiles ? x.tiles + L.cost : 0; }
+__device__ __forceinline__ int64_t sh_weight(const SharedArgs& a, const ShList& L, const ShEntry& x) {
+    return (int64_t)sh_item_weight(L, x) * x.blocks * a.n_kv;
 }
-__device__ __forceinline__ int64_t sh_first_item(const SharedArgs& a, int e) {
-    return e < a.n_groups ? (int64_t)e * a.n_kv * a.prefix_blocks
-                          : (int64_t)a.n_groups * a.n_kv * a.prefix_blocks +
-                                (int64_t)(e - a.n_groups) * a.n_kv * a.own_blocks;
+__host__ __device__ __forceinline__ int64_t sh_first_item(const ShList& L, int n_kv, int e) {
+    return e < L.n_pre ? (int64_t)e * n_kv * L.pre_blocks
+                       : ((int64_t)L.n_pre * L.pre_blocks + (int64_t)(e - L.n_pre) * L.own_blocks) * n_kv;
 }
 
-// Exclusive sums of the entries' weights over the CTA's threads (each thread a
-// run of consecutive entries) in scan[0 .. kShThreads]; scan[kShThreads] is the total.
-__device__ __forceinline__ int64_t sh_scan(const SharedArgs& a, int64_t* scan) {
-    const int n = a.n_groups + a.n_seqs, chunk = (n + kShThreads - 1) / kShThreads;
+// Exclusive sums of the entries' weights over the CTA's first kShThreads threads
+// (each a run of consecutive entries) in scan[0 .. kShThreads - 1]; the total
+// behind them.
+__device__ __forceinline__ int64_t sh_scan(const SharedArgs& a, const ShList& L, int64_t* scan) {
+    const int n = L.n_pre + L.n_own, chunk = (n + kShThreads - 1) / kShThreads;
     const int lane = threadIdx.x & 31;
-    int64_t sum = 0;
-    for (int e = threadIdx.x * chunk; e < min(n, ((int)threadIdx.x + 1) * chunk); ++e)
-        sum += sh_weight(a, sh_entry(a, e));
-    scan[threadIdx.x] = sum;
+    if (threadIdx.x < kShThreads) {
+        int64_t sum = 0;
+        for (int e = threadIdx.x * chunk; e < min(n, ((int)threadIdx.x + 1) * chunk); ++e)
+            sum += sh_weight(a, L, sh_entry(a, L, e));
+        scan[threadIdx.x] = sum;
+    }
     __syncthreads();
     if (threadIdx.x < 32) {
         int64_t v[4], run = 0;
@@ -165,41 +174,89 @@ __device__ __forceinline__ int64_t sh_scan(const SharedArgs& a, int64_t* scan) {
 static_assert(kShThreads == 128, "sh_scan: four sums per lane");
 
 // Worker w's stretch of the list: weights [sh_begin(w), sh_begin(w + 1)).  Within
-// an item the first kShItemCost units stand for its start and end, the others
-// for its tiles.  A piece's record is number item + worker: along the list every
-// new piece raises one of the two.
-__device__ __forceinline__ int sh_workers(const SharedArgs& a, int64_t total) {
-    return (int)min((int64_t)a.n_workers, (total + kShMinTiles - 1) / kShMinTiles);
-}
+// an item the first L.cost units stand for its start and end, the others for its
+// tiles.  A piece's record is number item + worker: along the list every new
+// piece raises one of the two.
+__device__ __forceinline__ int sh_workers(const ShList& L, int64_t total) { return (int)min((int64_t)L.n_workers, total); }
 __device__ __forceinline__ int64_t sh_begin(int64_t total, int n, int64_t w) { return total * w / n; }
 __device__ __forceinline__ int sh_worker_of(int64_t total, int n, int64_t at) {
     return (int)(((at + 1) * n + total - 1) / total) - 1;
 }
-__device__ __forceinline__ int sh_tile_at(int64_t at_in_item, int tiles) {
-    return (int)max((int64_t)0, min((int64_t)tiles, at_in_item - kShItemCost));
+__device__ __forceinline__ int sh_tile_at(const ShList& L, int64_t at_in_item, int tiles) {
+    return (int)max((int64_t)0, min((int64_t)tiles, at_in_item - L.cost));
 }
 
-// Position in the list; every lane keeps its own copy.
+// Position in a list; every thread keeps its own copy.
 struct ShCursor {
     int e;
     ShEntry x;
     int h, blk, tile;  // tile: index within the item
+    int64_t left;      // weight of the stretch from this tile on; <= 0 behind the last one
 };
-__device__ __forceinline__ void sh_next_item(const SharedArgs& a, ShCursor& c) {
-    c.tile = 0;
-    if (++c.blk < c.x.blocks) return;
-    c.blk = 0;
-    if (++c.h < a.n_kv) return;
-    c.h = 0;
-    do c.x = sh_entry(a, ++c.e);
-    while (c.x.tiles == 0);
+// The first tile of worker w's stretch.
+__device__ __forceinline__ void sh_seek(const SharedArgs& a, const ShList& L, const int64_t* scan, int n_workers, int w,
+                                        ShCursor& c) {
+    const int64_t total = scan[kShThreads], w0 = sh_begin(total, n_workers, w);
+    c.left = sh_begin(total, n_workers, w + 1) - w0;
+    int run = 0;
+#pragma unroll
+    for (int step = kShThreads / 2; step; step >>= 1)
+        if (scan[run + step] <= w0) run += step;
+    const int n = L.n_pre + L.n_own, chunk = (n + kShThreads - 1) / kShThreads;
+    int64_t at = w0 - scan[run];
+    c.e = run * chunk;
+    for (;; ++c.e) {
+        c.x = sh_entry(a, L, c.e);
+        const int64_t weight = sh_weight(a, L, c.x);
+        if (at < weight) break;
+        at -= weight;
+    }
+    const int one = sh_item_weight(L, c.x);
+    const int64_t it = at / one;
+    const int in = (int)(at - it * one);
+    c.blk = (int)(it % c.x.blocks);
+    c.h = (int)(it / c.x.blocks);
+    c.tile = sh_tile_at(L, in, c.x.tiles);
+    c.left -= max(0, L.cost - in);
 }
-// Next tile; true when it begins another item.  Never called on the list's last tile.
-__device__ __forceinline__ bool sh_next(const SharedArgs& a, ShCursor& c) {
-    if (++c.tile < c.x.tiles) return false;
-    sh_next_item(a, c);
+// Next tile of the stretch; true when it begins another item.  c.left tells whether there is one.
+__device__ __forceinline__ bool sh_next(const SharedArgs& a, const ShList& L, ShCursor& c) {
+    c.left -= 1;
+    if (c.left <= 0 || ++c.tile < c.x.tiles) return false;
+    c.left -= L.cost;
+    if (c.left <= 0) return false;
+    c.tile = 0;
+    if (++c.blk < c.x.blocks) return true;
+    c.blk = 0;
+    if (++c.h < a.n_kv) return true;
+    c.h = 0;
+    do c.x = sh_entry(a, L, ++c.e);
+    while (c.x.tiles == 0);
     return true;
 }
+// The cursor's tile is the last of its piece.
+__device__ __forceinline__ bool sh_piece_ends(const ShCursor& c) { return c.left <= 1 || c.tile + 1 == c.x.tiles; }
+__device__ __forceinline__ float* sh_record(const SharedArgs& a, const ShList& L, const ShCursor& c, int worker, int d) {
+    return L.records + (sh_first_item(L, a.n_kv, c.e) + (int64_t)c.h * c.x.blocks + c.blk + worker) * L.rows * (d + 4);
+}
+__device__ __forceinline__ int sh_lead(const SharedArgs& a, const ShList& L, const ShCursor& c) {
+    return c.e < L.n_pre ? c.e * a.per : c.e - L.n_pre;  // the sequence whose block table is read
+}
+// Query row r (0 ..) of the cursor's (entry, kv head): null past the last one.
+__device__ __forceinline__ const __half* sh_query(const SharedArgs& a, const ShList& L, const ShCursor& c, int r, int d) {
+    const int rows = c.e < L.n_pre ? a.per * a.group : a.group;
+    if (r >= rows) return nullptr;
+    return a.q + (((int64_t)(sh_lead(a, L, c) + r / a.group) * a.n_kv + c.h) * a.group + r % a.group) * d;
+}
+// Records hold the dims in the order of the packed codes: position n of word wi of
+// chunk c (a pair n % 4, then n and n + 4) is element 8 (4 c + wi) + 2 (n % 4) + n / 4.
+__host__ __device__ constexpr int sh_code_dim(int d, int at) {
+    const int n = (at % 8) / 2 + 4 * (at % 2), u = at / 8;
+    return nib_dim(d, u / 4, 4 * (u % 4) + n / 2, n % 2);
+}
+// Programmatic dependent launch: wait for the launch before this one / let the next one in.
+__device__ __forceinline__ void sh_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void sh_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---- fragments -------------------------------------------------------------
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -284,21 +341,12 @@ __device__ __forceinline__ int code_dim(int s, int r, int half, int q) {
     return nib_dim(D, c, 4 * q + n / 2, n % 2);
 }
 
-// Query rows of the cursor's item: count, and the first one's sequence.
-__device__ __forceinline__ void sh_rows(const SharedArgs& a, const ShCursor& c, int& rows, int& b0) {
-    const bool prefix = c.e < a.n_groups;
-    rows = prefix ? a.per * a.group : a.group;
-    b0 = prefix ? c.e * a.per : c.e - a.n_groups;
-}
-
 template <int D, bool COMP>
-__device__ __forceinline__ void sh_load_query(const SharedArgs& a, const ShCursor& c, const uint8_t* qrows,
-                                              ShQuery<D, COMP>& Q, int (&hi)[2], int& hi_min) {
+__device__ __forceinline__ void sh_load_query(const SharedArgs& a, const ShList& L, const ShCursor& c,
+                                              const uint8_t* qrows, ShQuery<D, COMP>& Q) {
     using C = ShCfg<D, COMP>;
     const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3;
-    int rows, b0;
-    sh_rows(a, c, rows, b0);
-    const bool live = c.blk * kShRows + g8 < rows;
+    const bool live = sh_query(a, L, c, c.blk * kShRows + g8, D) != nullptr;
     const __half* row = reinterpret_cast<const __half*>(qrows + g8 * C::Q_ROW);
     float sum = 0.0f, mag = 0.0f, top = 0.0f, sgn = 0.0f;
 #pragma unroll
@@ -345,11 +393,7 @@ __device__ __forceinline__ void sh_load_query(const SharedArgs& a, const ShCurso
         Q.boff[j] = m * __shfl_sync(0xffffffffu, sgn, from);
         Q.rco[j] = scale * (1.0f / 7.0f) * 1048576.0f / w;
         Q.roff[j] = t;
-        const int r = c.blk * kShRows + 2 * q + j;
-        // a sequence shorter than its group's prefix sees its own length of it
-        hi[j] = c.e < a.n_groups && r < rows ? min(c.x.hi, sh_len(a, b0 + r / a.group)) : c.x.hi;
     }
-    hi_min = (int)__reduce_min_sync(0xffffffffu, (unsigned)min(hi[0], hi[1]));
 }
 
 // Accumulators of one warp: o[mt][4] with rows of m-tile mt = 2c + h the dims
@@ -377,7 +421,7 @@ __device__ __forceinline__ int sh_key_of_row(int r) { return 2 * (r >> 2) + ((r 
 // The 32 keys of a tile at key position kpos.
 template <int D, bool COMP>
 __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>& st, const uint8_t* sb, int kpos,
-                                           int lo, const int (&hi)[2], bool masked) {
+                                           int lo, int hi, bool masked) {
     using C = ShCfg<D, COMP>;
     constexpr int NW = C::NW;
     const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3;
@@ -469,7 +513,7 @@ __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 float& v = s[b][2 * x + j];
-                if (masked && (kpos + key < lo || kpos + key >= hi[j])) v = -INFINITY;
+                if (masked && (kpos + key < lo || kpos + key >= hi)) v = -INFINITY;
                 top[j] = fmaxf(top[j], v + grow);
             }
         }
@@ -570,11 +614,10 @@ __device__ __forceinline__ void sh_consume(const ShQuery<D, COMP>& Q, ShState<D>
     }
 }
 
-// The piece's record: rows of D + 4 floats, o then (U, l).
+// The piece's record: rows of D + 4 floats, o (in the order of sh_code_dim) then (U, l).
 template <int D>
-__device__ __forceinline__ void sh_flush(const SharedArgs& a, ShState<D>& st, int64_t record) {
+__device__ __forceinline__ void sh_flush(const ShState<D>& st, float* m) {
     const int lane = threadIdx.x & 31, g8 = lane >> 2, q = lane & 3;
-    float* m = a.ws + record * sh_record_floats(D);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         float l = st.l[j];
@@ -582,21 +625,25 @@ __device__ __forceinline__ void sh_flush(const SharedArgs& a, ShState<D>& st, in
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
         float* row = m + (2 * q + j) * (D + 4);
 #pragma unroll
-        for (int mt = 0; mt < D / 16; ++mt) {
-            row[nib_dim(D, mt / 2, g8, mt % 2)] = st.o[mt][j] * kShValue;
-            row[nib_dim(D, mt / 2, g8 + 8, mt % 2)] = st.o[mt][2 + j] * kShValue;
-        }
+        for (int mt = 0; mt < D / 16; ++mt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {  // byte g8 + 8x of chunk mt / 2, its nibble mt % 2
+                const int n = 2 * (g8 % 4) + mt % 2;
+                row[8 * (4 * (mt / 2) + g8 / 4 + 2 * x) + 2 * (n % 4) + n / 4] = st.o[mt][2 * x + j] * kShValue;
+            }
         if (g8 == 0) *reinterpret_cast<float2*>(row + D) = make_float2(st.U[j], l);
     }
 }
 
 template <int D, bool COMP>
-__global__ void __launch_bounds__(kShThreads) k_shared_rows(const SharedArgs a) {
+__global__ void __launch_bounds__(kShThreads) k_shared_rows(const SharedArgs a, const ShList L) {
     using C = ShCfg<D, COMP>;
     extern __shared__ __align__(128) uint8_t smem[];
     int64_t* scan = reinterpret_cast<int64_t*>(smem + C::SCAN_OFF);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int64_t total = sh_scan(a, scan);
+    sh_wait_before();
+    sh_let_next();
+    const int64_t total = sh_scan(a, L, scan);
     if (blockIdx.x == 0) {  // lengths outside the block table are cut, and said so
         const int64_t cap = (int64_t)a.pt.max_pages * a.pt.page_size;
         for (int b = tid; b < a.n_seqs; b += kShThreads)
@@ -605,50 +652,39 @@ __global__ void __launch_bounds__(kShThreads) k_shared_rows(const SharedArgs a) 
             for (int g = tid; g < a.n_groups; g += kShThreads)
                 if (a.prefix_lens[g] < 0 || a.prefix_lens[g] > cap) raise_device_error(a.err, BC_DEVERR_INDEX);
     }
-    const int n_workers = sh_workers(a, total);
+    const int n_workers = sh_workers(L, total);
     const int worker = blockIdx.x * kShWarps + warp;
     if (worker >= n_workers) return;
-    const int64_t w0 = sh_begin(total, n_workers, worker), w1 = sh_begin(total, n_workers, worker + 1);
-
-    // the entry that holds w0: the thread's run by bisection, then along it
     ShCursor cur;
-    int64_t left = w1 - w0;  // weight of the stretch from the cursor's tile on
-    {
-        int run = 0;
-#pragma unroll
-        for (int step = kShThreads / 2; step; step >>= 1)
-            if (scan[run + step] <= w0) run += step;
-        const int n = a.n_groups + a.n_seqs, chunk = (n + kShThreads - 1) / kShThreads;
-        int64_t at = w0 - scan[run];
-        cur.e = run * chunk;
-        for (;; ++cur.e) {
-            cur.x = sh_entry(a, cur.e);
-            const int64_t w = sh_weight(a, cur.x);
-            if (at < w) break;
-            at -= w;
-        }
-        const int64_t it = at / cur.x.weight();
-        cur.blk = (int)(it % cur.x.blocks);
-        cur.h = (int)(it / cur.x.blocks);
-        const int in = (int)(at - it * cur.x.weight());
-        cur.tile = sh_tile_at(in, cur.x.tiles);
-        left -= max(0, kShItemCost - in);
-    }
-    if (left <= 0) return;  // the stretch ends within its first item's start
-    // Number of tiles of the stretch, item by item (later items cost kShItemCost before their first tile).
+    sh_seek(a, L, scan, n_workers, worker, cur);
+    if (cur.left <= 0) return;  // the stretch ends within its first item's start
+
     uint8_t* ring = smem + warp * C::WARP_B;
     ShCursor ahead = cur;
-    int64_t ahead_left = left;  // weight left at `ahead`, > 0 while it points at a tile of the stretch
-    bool ahead_new = true;      // the query rows travel with the first tile of each piece
-    unsigned present = 0;       // bit s: the page of stage s is in the pool
+    bool ahead_new = true;   // the query rows travel with the first tile of each piece
+    unsigned present = 0;    // bit s: the page of stage s is in the pool
+    int in_page = 0;         // position of `ahead` in its page
+    int64_t row = -1;        // plane row of `ahead`; -1: page outside the pool
+    const int32_t* page = nullptr;
     auto issue = [&](int s) {
         uint8_t* dst = ring + s * C::STAGE_B;
-        const int seq = ahead.e < a.n_groups ? ahead.e * a.per : ahead.e - a.n_groups;
-        const int pos = (ahead.x.tile0 + ahead.tile) * kShTile;
-        const int pg = __ldg(a.pt.pages + ((int64_t)seq * a.n_kv + ahead.h) * a.pt.max_pages + pos / a.pt.page_size);
-        if (pg >= 0 && pg < a.pt.n_pages) {
+        if (ahead_new) {
+            const int pos = (ahead.x.tile0 + ahead.tile) * kShTile;
+            const int j = pos / a.pt.page_size;
+            in_page = pos - j * a.pt.page_size;
+            page = a.pt.pages + ((int64_t)sh_lead(a, L, ahead) * a.n_kv + ahead.h) * a.pt.max_pages + j;
+        }
+        if (ahead_new || in_page == a.pt.page_size) {
+            if (!ahead_new) {
+                ++page;
+                in_page = 0;
+            }
+            const int pg = __ldg(page);
+            row = pg >= 0 && pg < a.pt.n_pages ? (int64_t)pg * a.pt.page_size + in_page : -1;
+            if (row < 0 && lane == 0) raise_device_error(a.err, BC_DEVERR_PAGE);
+        }
+        if (row >= 0) {
             present |= 1u << s;
-            const int64_t row = (int64_t)pg * a.pt.page_size + pos % a.pt.page_size;
             auto part = [&](const bc_kv_planes& P, uint8_t* d) {
 #pragma unroll
                 for (int i = lane * 16; i < C::SIGN_B; i += 512) sh_cp16(d + i, (const uint8_t*)P.sign + row * (D / 8) + i);
@@ -665,122 +701,109 @@ __global__ void __launch_bounds__(kShThreads) k_shared_rows(const SharedArgs a) 
             };
             part(a.K, dst);
             part(a.V, dst + C::HALF_B);
+            row += kShTile;
         } else {
             present &= ~(1u << s);
-            if (lane == 0) raise_device_error(a.err, BC_DEVERR_PAGE);
         }
-        if (ahead_new) {
-            int rows, b0;
-            sh_rows(a, ahead, rows, b0);
+        in_page += kShTile;
+        if (ahead_new)
             for (int i = lane; i < kShRows * (D / 8); i += 32) {
-                const int r = ahead.blk * kShRows + i / (D / 8), at = i % (D / 8) * 8;
-                if (r >= rows) break;
-                const __half* src =
-                    a.q + (((int64_t)(b0 + r / a.group) * a.n_kv + ahead.h) * a.group + r % a.group) * D + at;
-                uint8_t* to = dst + C::Q_OFF + i / (D / 8) * C::Q_ROW + 2 * at;
+                const int r = i / (D / 8), at = i % (D / 8) * 8;
+                const __half* src = sh_query(a, L, ahead, ahead.blk * kShRows + r, D);
+                if (!src) break;
+                uint8_t* to = dst + C::Q_OFF + r * C::Q_ROW + 2 * at;
                 if (a.q_aligned)
-                    sh_cp16(to, src);
+                    sh_cp16(to, src + at);
                 else
-                    for (int k = 0; k < 8; ++k) reinterpret_cast<__half*>(to)[k] = src[k];
+                    for (int k = 0; k < 8; ++k) reinterpret_cast<__half*>(to)[k] = src[at + k];
             }
-        }
-    };
-    auto advance = [&]() {  // `ahead` to the next tile of the stretch, or ahead_left <= 0
-        ahead_left -= 1;
-        ahead_new = false;
-        if (ahead_left > 0 && ++ahead.tile == ahead.x.tiles) {
-            ahead_left -= kShItemCost;
-            if (ahead_left > 0) {
-                sh_next_item(a, ahead);
-                ahead_new = true;
-            }
-        }
+        ahead_new = sh_next(a, L, ahead);
     };
 #pragma unroll
     for (int s = 0; s < kShStages; ++s) {
-        if (ahead_left > 0) {
-            issue(s);
-            advance();
-        }
+        if (ahead.left > 0) issue(s);
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
     ShQuery<D, COMP> Q;
     ShState<D> st;
-    int hi[2], hi_min;
     bool begin = true;
-    for (int s = 0;; s = s + 1 == kShStages ? 0 : s + 1) {
+    for (int s = 0; cur.left > 0; s = s + 1 == kShStages ? 0 : s + 1) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kShStages - 1) : "memory");
         __syncwarp();
         const uint8_t* sb = ring + s * C::STAGE_B;
         if (begin) {
-            sh_load_query<D, COMP>(a, cur, sb + C::Q_OFF, Q, hi, hi_min);
+            sh_load_query<D, COMP>(a, L, cur, sb + C::Q_OFF, Q);
             sh_clear(st);
         }
         const int kpos = (cur.x.tile0 + cur.tile) * kShTile;
-        if (present >> s & 1) sh_consume<D, COMP>(Q, st, sb, kpos, cur.x.lo, hi, kpos < cur.x.lo || kpos + kShTile > hi_min);
+        if (present >> s & 1)
+            sh_consume<D, COMP>(Q, st, sb, kpos, cur.x.lo, cur.x.hi, kpos < cur.x.lo || kpos + kShTile > cur.x.hi);
         __syncwarp();
-        if (ahead_left > 0) {
-            issue(s);
-            advance();
-        }
+        if (ahead.left > 0) issue(s);
         asm volatile("cp.async.commit_group;" ::: "memory");
-        left -= 1;
-        begin = cur.tile + 1 == cur.x.tiles;
-        if (begin || left <= 0) {
-            const int64_t item = sh_first_item(a, cur.e) + (int64_t)cur.h * cur.x.blocks + cur.blk;
-            sh_flush<D>(a, st, item + worker);
-            if (begin) left -= kShItemCost;
-            if (left <= 0) break;
-        }
-        sh_next(a, cur);
+        if (sh_piece_ends(cur)) sh_flush<D>(st, sh_record(a, L, cur, worker, D));
+        begin = sh_next(a, L, cur);
     }
 }
 
-// One CTA per (sequence, kv head): joins the pieces of each query row.
+// One CTA per (sequence, kv head): joins the pieces of each query row, of its
+// group's prefix (list P) and of its own keys (list O, which may hold both).
 template <int D>
-__global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a) {
-    constexpr int REC = sh_record_floats(D), PER = D / 32;
-    __shared__ int64_t scan[kShThreads + 1], at[2];
+__global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a, const ShList P, const ShList O, bool two) {
+    constexpr int VEC = D / 32;  // consecutive floats of a lane
+    __shared__ int64_t scan[2][kShThreads + 1], at[2];
     const int b = blockIdx.x / a.n_kv, h = blockIdx.x % a.n_kv;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t total = sh_scan(a, scan);
-    const int n_workers = sh_workers(a, total);
-    const int n = a.n_groups + a.n_seqs, chunk = (n + kShThreads - 1) / kShThreads;
-    const int want[2] = {b / a.per, a.n_groups + b};
+    sh_let_next();
+    // the lengths are older than the launches before this one, the records are theirs
+    const ShList* lists[2] = {&P, &O};
+    const int want[2] = {b / a.per, O.n_pre + b};
+    int64_t total[2];
     ShEntry x[2];
+    total[1] = sh_scan(a, O, scan[1]);
+    total[0] = two ? sh_scan(a, P, scan[0]) : total[1];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
+        const ShList& L = *lists[i];
+        const int n = L.n_pre + L.n_own, chunk = (n + kShThreads - 1) / kShThreads;
+        x[i].tiles = 0;
+        if (i == 0 && L.n_pre == 0) continue;
         if ((int)threadIdx.x == want[i] / chunk) {
-            int64_t sum = scan[threadIdx.x];
-            for (int e = threadIdx.x * chunk; e < want[i]; ++e) sum += sh_weight(a, sh_entry(a, e));
+            int64_t sum = scan[two ? i : 1][threadIdx.x];
+            for (int e = threadIdx.x * chunk; e < want[i]; ++e) sum += sh_weight(a, L, sh_entry(a, L, e));
             at[i] = sum;
         }
-        x[i] = sh_entry(a, want[i]);
+        x[i] = sh_entry(a, L, want[i]);
     }
+    if (sh_len(a, b) < x[0].hi) x[0].tiles = 0;  // takes no part in the prefix
     __syncthreads();
+    sh_wait_before();
     for (int g = warp; g < a.group; g += kShWarps) {
         const int64_t head = ((int64_t)b * a.n_kv + h) * a.group + g;
-        float M = kShNone, L = 0.0f, o[PER];
+        float M = kShNone, sum = 0.0f, o[VEC];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) o[i] = 0.0f;
+        for (int k = 0; k < VEC; ++k) o[k] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (x[i].tiles == 0) continue;
+            const ShList& L = *lists[i];
+            const int n_workers = sh_workers(L, total[i]);
             const int r = i == 0 ? (b % a.per) * a.group + g : g;
-            const int64_t it = (int64_t)h * x[i].blocks + r / kShRows;
-            const int64_t first = at[i] + it * x[i].weight();
-            const int c0 = sh_worker_of(total, n_workers, first);
-            const int c1 = sh_worker_of(total, n_workers, first + x[i].weight() - 1);
-            const float* rec = a.ws + (sh_first_item(a, want[i]) + it) * REC + (r % kShRows) * (D + 4);
+            const int64_t it = (int64_t)h * x[i].blocks + r / L.rows;
+            const int64_t first = at[i] + it * sh_item_weight(L, x[i]);
+            const int c0 = sh_worker_of(total[i], n_workers, first);
+            const int c1 = sh_worker_of(total[i], n_workers, first + sh_item_weight(L, x[i]) - 1);
+            const int64_t size = (int64_t)L.rows * (D + 4);
+            const float* rec = L.records + (sh_first_item(L, a.n_kv, want[i]) + it) * size + (r % L.rows) * (D + 4);
             // 32 workers at a time: units and sums lane by lane, then the sums over dims
             for (int base = c0; base <= c1; base += 32) {
                 const int c = base + lane;
                 bool has = c <= c1;
                 if (has)
-                    has = sh_tile_at(sh_begin(total, n_workers, c) - first, x[i].tiles) <
-                          sh_tile_at(sh_begin(total, n_workers, c + 1) - first, x[i].tiles);
-                const float2 ul = has ? *reinterpret_cast<const float2*>(rec + (int64_t)c * REC + D) : make_float2(kShNone, 0.0f);
+                    has = sh_tile_at(L, sh_begin(total[i], n_workers, c) - first, x[i].tiles) <
+                          sh_tile_at(L, sh_begin(total[i], n_workers, c + 1) - first, x[i].tiles);
+                const float2 ul = has ? __ldcg(reinterpret_cast<const float2*>(rec + c * size + D)) : make_float2(kShNone, 0.0f);
                 float top = ul.x;
 #pragma unroll
                 for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
@@ -790,33 +813,45 @@ __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a)
 #pragma unroll
                 for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
                 M = U;
-                L = L * f + l;
+                sum = sum * f + l;
 #pragma unroll
-                for (int k = 0; k < PER; ++k) o[k] *= f;
+                for (int k = 0; k < VEC; ++k) o[k] *= f;
                 unsigned todo = __ballot_sync(0xffffffffu, has);
                 while (todo) {
-                    constexpr int AT_ONCE = 4;
-                    float v[AT_ONCE][PER], wt[AT_ONCE];
+                    constexpr int AT_ONCE = 8;  // records in flight: an L2 round trip each
+                    float v[AT_ONCE][VEC], wt[AT_ONCE];
 #pragma unroll
                     for (int u = 0; u < AT_ONCE; ++u) {
                         const int src = todo ? __ffs(todo) - 1 : 0;
                         const bool on = todo != 0;
                         todo &= todo - 1;
                         wt[u] = __shfl_sync(0xffffffffu, w, src);
+                        const float* from = rec + (base + src) * size + VEC * lane;
 #pragma unroll
-                        for (int k = 0; k < PER; ++k) v[u][k] = on ? rec[(int64_t)(base + src) * REC + 32 * k + lane] : 0.0f;
-                        if (!on) wt[u] = 0.0f;
+                        for (int k = 0; k < VEC; ++k) v[u][k] = 0.0f;
+                        if (on) {
+                            if constexpr (VEC >= 4) {
+#pragma unroll
+                                for (int k = 0; k < VEC; k += 4)
+                                    *reinterpret_cast<float4*>(&v[u][k]) = __ldcg(reinterpret_cast<const float4*>(from + k));
+                            } else {
+#pragma unroll
+                                for (int k = 0; k < VEC; ++k) v[u][k] = __ldcg(from + k);
+                            }
+                        } else {
+                            wt[u] = 0.0f;
+                        }
                     }
 #pragma unroll
                     for (int u = 0; u < AT_ONCE; ++u)
 #pragma unroll
-                        for (int k = 0; k < PER; ++k) o[k] += v[u][k] * wt[u];
+                        for (int k = 0; k < VEC; ++k) o[k] += v[u][k] * wt[u];
                 }
             }
         }
-        const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;  // no keys: zeros
+        const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;  // no keys: zeros
 #pragma unroll
-        for (int k = 0; k < PER; ++k) a.out[head * D + 32 * k + lane] = __float2half_rn(o[k] * inv);
+        for (int k = 0; k < VEC; ++k) a.out[head * D + sh_code_dim(D, VEC * lane + k)] = __float2half_rn(o[k] * inv);
     }
 }
 
@@ -842,23 +877,48 @@ int sh_workers_on_device(int* n_workers) {
     return BC_OK;
 }
 
+template <typename... Args>
+cudaError_t sh_launch(void (*kernel)(Args...), int blocks, int threads, int smem, cudaStream_t st, const Args&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <int D, bool COMP>
-int sh_run(SharedArgs& a, cudaStream_t st) {
-    const int rc = sh_workers_on_device<D, COMP>(&a.n_workers);
+int sh_run(const SharedArgs& a, ShList& L, cudaStream_t st) {
+    const int rc = sh_workers_on_device<D, COMP>(&L.n_workers);
     if (rc) return rc;
-    k_shared_rows<D, COMP><<<(a.n_workers + kShWarps - 1) / kShWarps, kShThreads, ShCfg<D, COMP>::SMEM_B, st>>>(a);
-    BC_LAUNCH_CHECK();
-    k_shared_merge<D><<<a.n_seqs * a.n_kv, kShThreads, 0, st>>>(a);
-    BC_LAUNCH_CHECK();
-    return BC_OK;
+    cudaError_t e = sh_launch(k_shared_rows<D, COMP>, (L.n_workers + kShWarps - 1) / kShWarps, kShThreads,
+                              ShCfg<D, COMP>::SMEM_B, st, a, L);
+    if (e == cudaSuccess) e = sh_launch(k_shared_merge<D>, a.n_seqs * a.n_kv, kShThreads, 0, st, a, L, L, false);
+    return e == cudaSuccess ? BC_OK : BC_ERR_CUDA_BASE + (int)e;
 }
 
 bool sh_head_dim(int d) { return d == 32 || d == 64 || d == 128 || d == 256; }
 
-int64_t sh_records(int n_seqs, int n_groups, int n_kv, int group) {
-    const int per = n_seqs / n_groups;
-    const int64_t prefix = ((int64_t)per * group + kShRows - 1) / kShRows, own = (group + kShRows - 1) / kShRows;
-    return (int64_t)n_groups * n_kv * prefix + (int64_t)n_seqs * n_kv * own + kShMaxWorkers;
+ShList sh_list(int n_seqs, int n_groups, int group) {
+    ShList L{};
+    const int64_t shared = (int64_t)(n_seqs / n_groups) * group;
+    L.n_pre = n_groups;
+    L.n_own = n_seqs;
+    L.pre_blocks = (int)((shared + kShRows - 1) / kShRows);
+    L.own_blocks = (group + kShRows - 1) / kShRows;
+    L.tile = kShTile;
+    L.rows = kShRows;
+    L.cost = kShItemCost;
+    return L;
+}
+
+size_t sh_bytes(const ShList& L, int n_kv, int max_workers, int d) {
+    return (size_t)(sh_first_item(L, n_kv, L.n_pre + L.n_own) + max_workers) * L.rows * (d + 4) * sizeof(float);
 }
 
 }  // namespace
@@ -871,7 +931,7 @@ extern "C" {
 size_t bc_decode_shared_workspace_bytes(int n_seqs, int n_groups, int n_kv_heads, int group, int head_dim) {
     if (n_seqs <= 0 || n_groups <= 0 || n_seqs % n_groups || n_kv_heads <= 0 || group <= 0 || !sh_head_dim(head_dim))
         return 0;
-    return (size_t)sh_records(n_seqs, n_groups, n_kv_heads, group) * sh_record_floats(head_dim) * sizeof(float);
+    return sh_bytes(sh_list(n_seqs, n_groups, group), n_kv_heads, kShMaxWorkers, head_dim);
 }
 
 int bc_decode_attention_shared(const void* q, bc_kv_planes K, bc_kv_planes V, bc_page_table pt,
@@ -909,7 +969,6 @@ int bc_decode_attention_shared(const void* q, bc_kv_planes K, bc_kv_planes V, bc
     a.seq_lens = seq_lens;
     a.prefix_lens = prefix_lens;
     a.out = (__half*)out;
-    a.ws = (float*)workspace;
     a.err = bc_device_error_ptr();
     if (!a.err) return BC_ERR_CUDA_BASE;
     a.n_seqs = n_seqs;
@@ -917,14 +976,14 @@ int bc_decode_attention_shared(const void* q, bc_kv_planes K, bc_kv_planes V, bc
     a.per = n_seqs / n_groups;
     a.n_kv = n_kv_heads;
     a.group = group;
-    a.prefix_blocks = (int)(((int64_t)a.per * group + kShRows - 1) / kShRows);
-    a.own_blocks = (group + kShRows - 1) / kShRows;
+    ShList L = sh_list(n_seqs, n_groups, group);
+    L.records = (float*)workspace;
     cudaStream_t st = (cudaStream_t)stream;
     switch (head_dim) {
-        case 32: return comp ? sh_run<32, true>(a, st) : sh_run<32, false>(a, st);
-        case 64: return comp ? sh_run<64, true>(a, st) : sh_run<64, false>(a, st);
-        case 128: return comp ? sh_run<128, true>(a, st) : sh_run<128, false>(a, st);
-        default: return comp ? sh_run<256, true>(a, st) : sh_run<256, false>(a, st);
+        case 32: return comp ? sh_run<32, true>(a, L, st) : sh_run<32, false>(a, L, st);
+        case 64: return comp ? sh_run<64, true>(a, L, st) : sh_run<64, false>(a, L, st);
+        case 128: return comp ? sh_run<128, true>(a, L, st) : sh_run<128, false>(a, L, st);
+        default: return comp ? sh_run<256, true>(a, L, st) : sh_run<256, false>(a, L, st);
     }
 }
 
