@@ -32,45 +32,19 @@
 // rounded to fp16.  They keep at least 11 significant bits down to 2^-22 of a
 // row's largest one: e is 2^(s - U) with U such that the largest P lies between
 // 2^8 and 2^15.
-#include "common.cuh"
+#include "shared.cuh"
+#include "shared_tc.h"
 
 namespace bc {
 namespace {
 
-constexpr int kShThreads = 128;
 constexpr int kShWarps = kShThreads / 32;
 constexpr int kShTile = 32;        // keys per tile
 constexpr int kShRows = 8;         // query rows per item
 constexpr int kShStages = 2;
 constexpr int kShItemCost = 2;     // an item's start and end, in tiles
 constexpr int kShMaxWorkers = 148 * 16;  // bound of the workers, for the workspace's size
-constexpr float kShLog2e = 1.4426950408889634f;
-constexpr float kShNone = -1e30f;  // U of a row without keys
-
-struct SharedArgs {
-    const __half* q;
-    bc_kv_planes K, V;
-    bc_page_table pt;
-    const int32_t* seq_lens;
-    const int32_t* prefix_lens;  // null: no prefixes
-    __half* out;
-    unsigned int* err;
-    int n_seqs, n_groups, per;  // per: sequences of a group
-    int n_kv, group;
-    bool q_aligned;  // q on a 16-byte boundary
-};
-
-// One kernel's list of work: entries [0, n_pre) are the groups' prefixes, the
-// following n_own the sequences' own keys.  An item is one block of query rows of
-// one kv head of an entry.
-struct ShList {
-    int n_pre, n_own;
-    int pre_blocks, own_blocks;  // blocks of `rows` query rows of a prefix / of a sequence
-    int tile, rows;              // keys of a tile; query rows of a block, and of a record
-    int cost;                    // an item's start and end, in tiles
-    int n_workers;
-    float* records;
-};
+constexpr int kShTcWorkers = 148;        // CTAs of the prefix kernel, one per SM
 
 template <int D, bool COMP>
 struct ShCfg {
@@ -89,174 +63,6 @@ struct ShCfg {
     static constexpr int SCAN_OFF = kShWarps * WARP_B;
     static constexpr int SMEM_B = SCAN_OFF + (kShThreads + 1) * 8 + 8;
 };
-
-// ---- the list of work ------------------------------------------------------
-__device__ __forceinline__ int sh_capacity(const SharedArgs& a) {
-    const int64_t c = (int64_t)a.pt.max_pages * a.pt.page_size;
-    return (int)(c < 0x7fffff80 ? c : 0x7fffff80);
-}
-__device__ __forceinline__ int sh_len(const SharedArgs& a, int b) {
-    return max(0, min(__ldg(a.seq_lens + b), sh_capacity(a)));
-}
-// A group of one sequence shares with nobody: its prefix is part of its own keys.
-__device__ __forceinline__ int sh_prefix(const SharedArgs& a, int g) {
-    if (!a.prefix_lens || a.per == 1) return 0;
-    return max(0, min(__ldg(a.prefix_lens + g), sh_capacity(a)));
-}
-
-// Entry e of a list.  A sequence shorter than its group's prefix takes no part in
-// it (its rows there are not read) and attends all of its keys on its own.
-struct ShEntry {
-    int lo, hi;  // key positions
-    int tile0, tiles;
-    int blocks;
-};
-__device__ __forceinline__ ShEntry sh_entry(const SharedArgs& a, const ShList& L, int e) {
-    ShEntry x;
-    if (e < L.n_pre) {
-        x.lo = 0;
-        x.hi = sh_prefix(a, e);
-        x.blocks = L.pre_blocks;
-    } else {
-        const int b = e - L.n_pre, prefix = sh_prefix(a, b / a.per);
-        x.hi = sh_len(a, b);
-        x.lo = x.hi < prefix ? 0 : prefix;
-        x.blocks = L.own_blocks;
-    }
-    x.tile0 = x.lo / L.tile;
-    x.tiles = x.hi > x.lo ? (x.hi + L.tile - 1) / L.tile - x.tile0 : 0;
-    return x;
-}
-__device__ __forceinline__ int sh_item_weight(const ShList& L, const ShEntry& x) { return x.tiles ? x.tiles + L.cost : 0; }
-__device__ __forceinline__ int64_t sh_weight(const SharedArgs& a, const ShList& L, const ShEntry& x) {
-    return (int64_t)sh_item_weight(L, x) * x.blocks * a.n_kv;
-}
-__host__ __device__ __forceinline__ int64_t sh_first_item(const ShList& L, int n_kv, int e) {
-    return e < L.n_pre ? (int64_t)e * n_kv * L.pre_blocks
-                       : ((int64_t)L.n_pre * L.pre_blocks + (int64_t)(e - L.n_pre) * L.own_blocks) * n_kv;
-}
-
-// Exclusive sums of the entries' weights over the CTA's first kShThreads threads
-// (each a run of consecutive entries) in scan[0 .. kShThreads - 1]; the total
-// behind them.
-__device__ __forceinline__ int64_t sh_scan(const SharedArgs& a, const ShList& L, int64_t* scan) {
-    const int n = L.n_pre + L.n_own, chunk = (n + kShThreads - 1) / kShThreads;
-    const int lane = threadIdx.x & 31;
-    if (threadIdx.x < kShThreads) {
-        int64_t sum = 0;
-        for (int e = threadIdx.x * chunk; e < min(n, ((int)threadIdx.x + 1) * chunk); ++e)
-            sum += sh_weight(a, L, sh_entry(a, L, e));
-        scan[threadIdx.x] = sum;
-    }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        int64_t v[4], run = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[i] = run;
-            run += scan[4 * lane + i];
-        }
-        int64_t before = run;
-#pragma unroll
-        for (int off = 1; off < 32; off <<= 1) {
-            const int64_t up = __shfl_up_sync(0xffffffffu, before, off);
-            if (lane >= off) before += up;
-        }
-        if (lane == 31) scan[kShThreads] = before;
-        before -= run;
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) scan[4 * lane + i] = before + v[i];
-    }
-    __syncthreads();
-    return scan[kShThreads];
-}
-static_assert(kShThreads == 128, "sh_scan: four sums per lane");
-
-// Worker w's stretch of the list: weights [sh_begin(w), sh_begin(w + 1)).  Within
-// an item the first L.cost units stand for its start and end, the others for its
-// tiles.  A piece's record is number item + worker: along the list every new
-// piece raises one of the two.
-__device__ __forceinline__ int sh_workers(const ShList& L, int64_t total) { return (int)min((int64_t)L.n_workers, total); }
-__device__ __forceinline__ int64_t sh_begin(int64_t total, int n, int64_t w) { return total * w / n; }
-__device__ __forceinline__ int sh_worker_of(int64_t total, int n, int64_t at) {
-    return (int)(((at + 1) * n + total - 1) / total) - 1;
-}
-__device__ __forceinline__ int sh_tile_at(const ShList& L, int64_t at_in_item, int tiles) {
-    return (int)max((int64_t)0, min((int64_t)tiles, at_in_item - L.cost));
-}
-
-// Position in a list; every thread keeps its own copy.
-struct ShCursor {
-    int e;
-    ShEntry x;
-    int h, blk, tile;  // tile: index within the item
-    int64_t left;      // weight of the stretch from this tile on; <= 0 behind the last one
-};
-// The first tile of worker w's stretch.
-__device__ __forceinline__ void sh_seek(const SharedArgs& a, const ShList& L, const int64_t* scan, int n_workers, int w,
-                                        ShCursor& c) {
-    const int64_t total = scan[kShThreads], w0 = sh_begin(total, n_workers, w);
-    c.left = sh_begin(total, n_workers, w + 1) - w0;
-    int run = 0;
-#pragma unroll
-    for (int step = kShThreads / 2; step; step >>= 1)
-        if (scan[run + step] <= w0) run += step;
-    const int n = L.n_pre + L.n_own, chunk = (n + kShThreads - 1) / kShThreads;
-    int64_t at = w0 - scan[run];
-    c.e = run * chunk;
-    for (;; ++c.e) {
-        c.x = sh_entry(a, L, c.e);
-        const int64_t weight = sh_weight(a, L, c.x);
-        if (at < weight) break;
-        at -= weight;
-    }
-    const int one = sh_item_weight(L, c.x);
-    const int64_t it = at / one;
-    const int in = (int)(at - it * one);
-    c.blk = (int)(it % c.x.blocks);
-    c.h = (int)(it / c.x.blocks);
-    c.tile = sh_tile_at(L, in, c.x.tiles);
-    c.left -= max(0, L.cost - in);
-}
-// Next tile of the stretch; true when it begins another item.  c.left tells whether there is one.
-__device__ __forceinline__ bool sh_next(const SharedArgs& a, const ShList& L, ShCursor& c) {
-    c.left -= 1;
-    if (c.left <= 0 || ++c.tile < c.x.tiles) return false;
-    c.left -= L.cost;
-    if (c.left <= 0) return false;
-    c.tile = 0;
-    if (++c.blk < c.x.blocks) return true;
-    c.blk = 0;
-    if (++c.h < a.n_kv) return true;
-    c.h = 0;
-    do c.x = sh_entry(a, L, ++c.e);
-    while (c.x.tiles == 0);
-    return true;
-}
-// The cursor's tile is the last of its piece.
-__device__ __forceinline__ bool sh_piece_ends(const ShCursor& c) { return c.left <= 1 || c.tile + 1 == c.x.tiles; }
-__device__ __forceinline__ float* sh_record(const SharedArgs& a, const ShList& L, const ShCursor& c, int worker, int d) {
-    return L.records + (sh_first_item(L, a.n_kv, c.e) + (int64_t)c.h * c.x.blocks + c.blk + worker) * L.rows * (d + 4);
-}
-__device__ __forceinline__ int sh_lead(const SharedArgs& a, const ShList& L, const ShCursor& c) {
-    return c.e < L.n_pre ? c.e * a.per : c.e - L.n_pre;  // the sequence whose block table is read
-}
-// Query row r (0 ..) of the cursor's (entry, kv head): null past the last one.
-__device__ __forceinline__ const __half* sh_query(const SharedArgs& a, const ShList& L, const ShCursor& c, int r, int d) {
-    const int rows = c.e < L.n_pre ? a.per * a.group : a.group;
-    if (r >= rows) return nullptr;
-    return a.q + (((int64_t)(sh_lead(a, L, c) + r / a.group) * a.n_kv + c.h) * a.group + r % a.group) * d;
-}
-// Records hold the dims in the order of the packed codes: position n of word wi of
-// chunk c (a pair n % 4, then n and n + 4) is element 8 (4 c + wi) + 2 (n % 4) + n / 4.
-__host__ __device__ constexpr int sh_code_dim(int d, int at) {
-    const int n = (at % 8) / 2 + 4 * (at % 2), u = at / 8;
-    return nib_dim(d, u / 4, 4 * (u % 4) + n / 2, n % 2);
-}
-// Programmatic dependent launch: wait for the launch before this one / let the next one in.
-__device__ __forceinline__ void sh_wait_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void sh_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---- fragments -------------------------------------------------------------
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -636,12 +442,19 @@ __device__ __forceinline__ void sh_flush(const ShState<D>& st, float* m) {
 }
 
 template <int D, bool COMP>
-__global__ void __launch_bounds__(kShThreads) k_shared_rows(const SharedArgs a, const ShList L) {
+__global__ void __launch_bounds__(kShThreads) k_shared_rows(const SharedArgs a, const ShList L, bool overlap) {
     using C = ShCfg<D, COMP>;
     extern __shared__ __align__(128) uint8_t smem[];
     int64_t* scan = reinterpret_cast<int64_t*>(smem + C::SCAN_OFF);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    sh_wait_before();
+    // Behind the prefix kernel (which has waited for all that this one reads) the CTAs
+    // start as SMs fall free; one more CTA waits for it on behalf of the launches to come.
+    if (overlap && blockIdx.x == gridDim.x - 1) {
+        sh_let_next();
+        sh_wait_before();
+        return;
+    }
+    if (!overlap) sh_wait_before();
     sh_let_next();
     const int64_t total = sh_scan(a, L, scan);
     if (blockIdx.x == 0) {  // lengths outside the block table are cut, and said so
@@ -877,37 +690,31 @@ int sh_workers_on_device(int* n_workers) {
     return BC_OK;
 }
 
-template <typename... Args>
-cudaError_t sh_launch(void (*kernel)(Args...), int blocks, int threads, int smem, cudaStream_t st, const Args&... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)blocks);
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = (size_t)smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
+// The prefix kernel takes the prefixes when `tc` is given, else the rows kernel has both.
 template <int D, bool COMP>
-int sh_run(const SharedArgs& a, ShList& L, cudaStream_t st) {
-    const int rc = sh_workers_on_device<D, COMP>(&L.n_workers);
+int sh_run(const SharedArgs& a, ShList& L, const ShList* tc, cudaStream_t st) {
+    int rc = sh_workers_on_device<D, COMP>(&L.n_workers);
+    if (!rc && tc) rc = sh_tc_run(a, *tc, D, COMP, st);
     if (rc) return rc;
-    cudaError_t e = sh_launch(k_shared_rows<D, COMP>, (L.n_workers + kShWarps - 1) / kShWarps, kShThreads,
-                              ShCfg<D, COMP>::SMEM_B, st, a, L);
-    if (e == cudaSuccess) e = sh_launch(k_shared_merge<D>, a.n_seqs * a.n_kv, kShThreads, 0, st, a, L, L, false);
+    cudaError_t e = sh_launch(k_shared_rows<D, COMP>, (L.n_workers + kShWarps - 1) / kShWarps + (tc ? 1 : 0), kShThreads,
+                              ShCfg<D, COMP>::SMEM_B, st, a, L, tc != nullptr);
+    if (e == cudaSuccess)
+        e = sh_launch(k_shared_merge<D>, a.n_seqs * a.n_kv, kShThreads, 0, st, a, tc ? *tc : L, L, tc != nullptr);
     return e == cudaSuccess ? BC_OK : BC_ERR_CUDA_BASE + (int)e;
 }
 
 bool sh_head_dim(int d) { return d == 32 || d == 64 || d == 128 || d == 256; }
 
-ShList sh_list(int n_seqs, int n_groups, int group) {
+// More query rows than this behind one prefix: the prefix kernel.
+constexpr int kShTcRows = 16;
+bool sh_takes_tc(int n_seqs, int n_groups, int group, int head_dim) {
+    return (head_dim == 64 || head_dim == 128) && (int64_t)(n_seqs / n_groups) * group > kShTcRows && n_seqs > n_groups;
+}
+
+ShList sh_list(int n_seqs, int n_groups, int group, bool prefixes) {
     ShList L{};
     const int64_t shared = (int64_t)(n_seqs / n_groups) * group;
-    L.n_pre = n_groups;
+    L.n_pre = prefixes ? n_groups : 0;
     L.n_own = n_seqs;
     L.pre_blocks = (int)((shared + kShRows - 1) / kShRows);
     L.own_blocks = (group + kShRows - 1) / kShRows;
@@ -931,7 +738,9 @@ extern "C" {
 size_t bc_decode_shared_workspace_bytes(int n_seqs, int n_groups, int n_kv_heads, int group, int head_dim) {
     if (n_seqs <= 0 || n_groups <= 0 || n_seqs % n_groups || n_kv_heads <= 0 || group <= 0 || !sh_head_dim(head_dim))
         return 0;
-    return sh_bytes(sh_list(n_seqs, n_groups, group), n_kv_heads, kShMaxWorkers, head_dim);
+    const bool tc = sh_takes_tc(n_seqs, n_groups, group, head_dim);
+    return sh_bytes(sh_list(n_seqs, n_groups, group, !tc), n_kv_heads, kShMaxWorkers, head_dim) +
+           (tc ? sh_bytes(sh_tc_list(n_seqs, n_groups, group), n_kv_heads, kShTcWorkers, head_dim) : 0);
 }
 
 int bc_decode_attention_shared(const void* q, bc_kv_planes K, bc_kv_planes V, bc_page_table pt,
@@ -976,14 +785,20 @@ int bc_decode_attention_shared(const void* q, bc_kv_planes K, bc_kv_planes V, bc
     a.per = n_seqs / n_groups;
     a.n_kv = n_kv_heads;
     a.group = group;
-    ShList L = sh_list(n_seqs, n_groups, group);
+    const bool tc = sh_takes_tc(n_seqs, n_groups, group, head_dim) && prefix_lens;
+    ShList L = sh_list(n_seqs, n_groups, group, !tc), T = sh_tc_list(n_seqs, n_groups, group);
     L.records = (float*)workspace;
+    if (tc) {
+        T.n_workers = kShTcWorkers;
+        T.records = (float*)((char*)workspace + sh_bytes(L, n_kv_heads, kShMaxWorkers, head_dim));
+    }
     cudaStream_t st = (cudaStream_t)stream;
+    const ShList* t = tc ? &T : nullptr;
     switch (head_dim) {
-        case 32: return comp ? sh_run<32, true>(a, L, st) : sh_run<32, false>(a, L, st);
-        case 64: return comp ? sh_run<64, true>(a, L, st) : sh_run<64, false>(a, L, st);
-        case 128: return comp ? sh_run<128, true>(a, L, st) : sh_run<128, false>(a, L, st);
-        default: return comp ? sh_run<256, true>(a, L, st) : sh_run<256, false>(a, L, st);
+        case 32: return comp ? sh_run<32, true>(a, L, t, st) : sh_run<32, false>(a, L, t, st);
+        case 64: return comp ? sh_run<64, true>(a, L, t, st) : sh_run<64, false>(a, L, t, st);
+        case 128: return comp ? sh_run<128, true>(a, L, t, st) : sh_run<128, false>(a, L, t, st);
+        default: return comp ? sh_run<256, true>(a, L, t, st) : sh_run<256, false>(a, L, t, st);
     }
 }
 
