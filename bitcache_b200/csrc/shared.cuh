@@ -179,6 +179,15 @@ __device__ __forceinline__ bool sh_next(const SharedArgs& a, const ShList& L, Sh
     while (c.x.tiles == 0);
     return true;
 }
+// Tiles of the piece that begins at the cursor, and the step to the next one (a
+// kernel's loop over tiles then has no list code in it).
+__device__ __forceinline__ int sh_piece_tiles(const ShCursor& c) { return (int)min(c.left, (int64_t)(c.x.tiles - c.tile)); }
+__device__ __forceinline__ void sh_next_piece(const SharedArgs& a, const ShList& L, ShCursor& c) {
+    const int n = sh_piece_tiles(c) - 1;
+    c.left -= n;
+    c.tile += n;
+    sh_next(a, L, c);
+}
 // The cursor's tile is the last of its piece.
 __device__ __forceinline__ bool sh_piece_ends(const ShCursor& c) { return c.left <= 1 || c.tile + 1 == c.x.tiles; }
 __device__ __forceinline__ float* sh_record(const SharedArgs& a, const ShList& L, const ShCursor& c, int worker, int d) {

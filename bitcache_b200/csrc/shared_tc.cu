@@ -9,15 +9,20 @@
 //   f = mean|q| / h:  s = f Q . K
 // (f carries what the rounding of the row's mean would lose).  V = bs sgn v + rs/7 n.
 //
-// Roles of the 15 warps of a CTA, one CTA per SM:
-//   0-3    softmax: a thread owns a query row.  Writes the row's Q into tensor
-//          memory, then per tile reads its 128 scores, keeps U and l, writes P
-//          (fp16, over the scores) and, when U moves, rescales O.
-//   4-7    unpack K: a thread owns a key; packed bytes -> fp16 operand rows in
-//          shared memory (128-byte swizzle, K-major: 4 blocks of 64 elements).
-//   8-11   unpack V, likewise (MN-major: dims contiguous, 64 per swizzle atom).
-//   12     issues the products: Q (tensor memory) x K, P (tensor memory) x V.
-//   13, 14 bring K's / V's packed tiles with 1-D bulk copies, three ahead.
+// Roles of the 27 warps of a CTA, one CTA per SM:
+//   0-7    softmax: a thread owns a query row and half of a tile's keys (warps 0-3
+//          keys 0-63, 4-7 the others; the two warps of a row exchange maxima).
+//          Writes the row's Q into tensor memory, then per tile reads its scores,
+//          keeps U and l, writes P (fp16, over the scores) and, when U moves,
+//          rescales O.
+//   8-23   unpack: packed bytes -> fp16 operand rows in shared memory, two threads
+//          to a key.  K on the first two schedulers, K-major (128-byte swizzle,
+//          blocks of 64 elements); V on the other two, MN-major (dims contiguous).
+//          Each scheduler so has two instruction streams, not three; with fully
+//          unrolled bodies and all three on each, waiting for instructions took
+//          more than everything else (13600 clocks a tile, 4200 with rolled loops).
+//   24     issues the products: Q (tensor memory) x K, P (tensor memory) x V.
+//   25, 26 bring K's / V's packed tiles with 1-D bulk copies, three ahead.
 // Keeping Q in tensor memory spares half of the score product's shared-memory
 // reads, which with the operands' own writes are what bounds the kernel: per
 // tile 96 KB written, 96 KB read by the tensor cores and 43 KB of packed bytes in
@@ -34,7 +39,8 @@ namespace bc {
 namespace {
 
 constexpr int kTcTile = 128;
-constexpr int kTcThreads = 480;
+constexpr int kTcThreads = 27 * 32;
+constexpr int kTcUnpackWarps = 8;   // of K, and of V
 constexpr int kTcRaw = 3;        // packed tiles ahead
 constexpr int kTcItemCost = 2;   // an item's start and end, in tiles
 constexpr uint32_t kTcSpin = 1u << 22;
@@ -55,7 +61,8 @@ struct TcCfg {
     static constexpr int RAWK_OFF = V_OFF + VST * VOP_B;
     static constexpr int RAWV_OFF = RAWK_OFF + kTcRaw * RAW_B;
     static constexpr int SCAN_OFF = (RAWV_OFF + kTcRaw * RAW_B + 15) / 16 * 16;
-    static constexpr int BAR_OFF = SCAN_OFF + (kShThreads + 1) * 8 + 8;
+    static constexpr int XCH_OFF = SCAN_OFF;  // [2][2][128] maxima of the row halves, once the sums are read
+    static constexpr int BAR_OFF = SCAN_OFF + 512 * 4;
     static constexpr int FLAG_OFF = BAR_OFF + 32 * 8;
     static constexpr int SMEM_B = FLAG_OFF + 20 * 4 + 1024;  // + alignment to the swizzle atom
     // tensor memory columns
@@ -65,7 +72,7 @@ struct TcCfg {
 
 enum TcBar {
     kRawKFull = 0, kRawKEmpty = 3, kRawVFull = 6, kRawVEmpty = 9, kKFull = 12, kKEmpty = 14, kVFull = 16, kVEmpty = 18,
-    kSFull = 20, kPFull = 22, kQFull = 24, kPvDone = 25, kDrain = 26, kTcBars = 27
+    kSFull = 20, kPFull = 22, kQFull = 24, kPvDone = 25, kDrain = 26, kPair = 27, kTcBars = 31
 };
 
 // ---- tcgen05 ---------------------------------------------------------------
@@ -131,6 +138,7 @@ __host__ __device__ constexpr uint32_t tc_idesc(int n, bool b_mn) {
 // Bounded; once one has given up (dead), all do, and the CTA winds down.
 __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
     if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
     for (uint32_t it = 0; it < kTcSpin; ++it) {
         if (mbar_try_wait(bar, parity)) return true;
         if (*dead) return false;
@@ -154,6 +162,101 @@ __device__ __forceinline__ __half2 tc_code(uint32_t w, int t) {
 __device__ __forceinline__ uint32_t tc_sign(uint32_t w, int i, uint32_t flip) { return ((w << (15 - i)) & 0x80008000u) ^ flip; }
 __device__ __forceinline__ void sts128(uint8_t* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(smem_u32(p)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+__device__ __forceinline__ float2 tc_fma2(float2 x, float2 y, float2 z) {
+    unsigned long long r;
+    asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;"
+        : "=l"(r)
+        : "l"(*reinterpret_cast<unsigned long long*>(&x)), "l"(*reinterpret_cast<unsigned long long*>(&y)),
+          "l"(*reinterpret_cast<unsigned long long*>(&z)));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 tc_add2(float2 x, float2 y) {
+    unsigned long long r;
+    asm("add.rn.ftz.f32x2 %0, %1, %2;"
+        : "=l"(r)
+        : "l"(*reinterpret_cast<unsigned long long*>(&x)), "l"(*reinterpret_cast<unsigned long long*>(&y)));
+    return *reinterpret_cast<float2*>(&r);
+}
+
+// Dims 32 w .. 32 w + 31 of a query row as fp16 pairs (zeros without a row).
+__device__ __forceinline__ void tc_row_word(const __half* src, bool aligned, int w, uint32_t (&x)[16]) {
+    if (!src) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x[k] = 0;
+    } else if (aligned) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint4 v = reinterpret_cast<const uint4*>(src)[4 * w + k];
+            x[4 * k] = v.x;
+            x[4 * k + 1] = v.y;
+            x[4 * k + 2] = v.z;
+            x[4 * k + 3] = v.w;
+        }
+    } else {
+        const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src) + 32 * w;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x[k] = s16[2 * k] | ((uint32_t)s16[2 * k + 1] << 16);
+    }
+}
+__device__ __forceinline__ void tc_st4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+
+// A thread's query row into tensor memory (part 0: h sgn q, part 1: 8/7 q / f, in
+// the order of K's elements); returns the scale of its scores in log2 units.
+template <int D, bool COMP>
+__device__ __forceinline__ float tc_query(const __half* src, bool aligned, int part, uint32_t at) {
+    constexpr int NW = D / 32;
+    uint32_t x[16];
+    float mag = 0.0f;
+#pragma unroll 1
+    for (int w = 0; w < NW; ++w) {
+        tc_row_word(src, aligned, w, x);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+            const float2 f = __half22float2(bits_h2(x[k]));
+            mag += fabsf(f.x) + fabsf(f.y);
+        }
+    }
+    const float mean = mag * (1.0f / D);
+    const __half h = __float2half_rn(mean);
+    const float hf = __half2float(h);
+    const float f = hf == 0.0f ? 1.0f : mean / hf;
+    auto dim = [&](int d) { return d % 2 ? __high2float(bits_h2(x[d / 2])) : __low2float(bits_h2(x[d / 2])); };
+    if (part == 0) {
+        const uint32_t hb = __half_as_ushort(h);
+#pragma unroll 1
+        for (int w = 0; w < NW; ++w) {
+            tc_row_word(src, aligned, w, x);
+            uint32_t r[16];  // pairs (i, i + 16) of the word
+#pragma unroll
+            for (int p = 0; p < 16; ++p)
+                r[p] = (hb | (dim(p) >= 0.0f ? 0u : 0x8000u)) | ((hb | (dim(p + 16) >= 0.0f ? 0u : 0x8000u)) << 16);
+            tc_st16(at + 16 * w, r);
+        }
+    } else if constexpr (COMP) {
+        const float g = (8.0f / 7.0f) / f;
+#pragma unroll 1
+        for (int w = 0; w < NW; ++w) {
+            tc_row_word(src, aligned, w, x);
+            // the code words made of these dims: word w of every chunk (head_dim 128), words w and w + 2 (64)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int first = D == 128 ? u : 2 * (u / 2) + u % 2;  // bit of the byte that nibble 0 holds
+                const int unit = D == 128 ? 4 * u + w : 4 * (u / 2) + w + 2 * (u % 2);
+                uint32_t r[4];
+#pragma unroll
+                for (int t = 0; t < 4; ++t)  // nibbles t, t + 4: dims 4 t + first, 4 t + 16 + first of the word
+                    r[t] = h2_bits(__floats2half2_rn(dim(4 * t + first) * g, dim(4 * t + 16 + first) * g));
+                tc_st4(at + D / 2 + 4 * unit, r[0], r[1], r[2], r[3]);
+            }
+        }
+    }
+    tc_wait_st();
+    return f * kShLog2e * rsqrtf((float)D);
 }
 
 template <int D, bool COMP>
@@ -184,23 +287,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
         for (int i = 0; i < kTcRaw; ++i) {
             mbar_init(&bar[kRawKFull + i], 1);
             mbar_init(&bar[kRawVFull + i], 1);
-            mbar_init(&bar[kRawKEmpty + i], 4);
-            mbar_init(&bar[kRawVEmpty + i], 4);
+            mbar_init(&bar[kRawKEmpty + i], kTcUnpackWarps);
+            mbar_init(&bar[kRawVEmpty + i], kTcUnpackWarps);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&bar[kKFull + i], 4);
-            mbar_init(&bar[kVFull + i], 4);
+            mbar_init(&bar[kKFull + i], kTcUnpackWarps);
+            mbar_init(&bar[kVFull + i], kTcUnpackWarps);
             mbar_init(&bar[kKEmpty + i], 1);
             mbar_init(&bar[kVEmpty + i], 1);
             mbar_init(&bar[kSFull + i], 1);
-            mbar_init(&bar[kPFull + i], 4);
+            mbar_init(&bar[kPFull + i], 8);
         }
-        mbar_init(&bar[kQFull], 4);
+        mbar_init(&bar[kQFull], 8);
+        for (int i = 0; i < 4; ++i) mbar_init(&bar[kPair + i], 2);
         mbar_init(&bar[kPvDone], 1);
         mbar_init(&bar[kDrain], 1);
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == 24) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
                          smem_u32(const_cast<uint32_t*>(tmem_at)))
                      : "memory");
@@ -211,110 +315,72 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
 
-    if (warp < 4) {
-        // ---------------- softmax: row `rl` of the item's block ----------------
-        const uint32_t lane_at = tmem + ((uint32_t)(32 * warp) << 16);
-        const int rl = 32 * warp + lane;
+    if (warp < 8) {
+        // ---------------- softmax: row `rl` of the item's block, keys 64 half .. 64 half + 63 ----------------
+        const int half = warp >> 2, quad = warp & 3;
+        const uint32_t lane_at = tmem + ((uint32_t)(32 * quad) << 16);
+        const int rl = 32 * quad + lane;
+        float* xch = reinterpret_cast<float*>(smem + C::XCH_OFF) + rl;  // [2][2][128]: parity, half, row
+        uint64_t* pair = &bar[kPair + quad];
+        uint32_t met = 0;  // exchanges with the row's other warp
         float sc = 0.0f, U = kShNone, l = 0.0f;
-        bool begin = true, busy = false, valid = false, ok = true;
-        for (int i = 0; cur.left > 0; ++i) {
+        bool ok = true;
+        for (int i = 0; ok && cur.left > 0; sh_next_piece(a, L, cur)) {
+            const int end = i + sh_piece_tiles(cur);
+            const __half* src = rl < L.rows ? sh_query(a, L, cur, cur.blk * L.rows + rl, D) : nullptr;
+            const bool valid = src != nullptr, busy = __any_sync(0xffffffffu, valid);
+            if (busy) sc = tc_query<D, COMP>(src, a.q_aligned, half, lane_at + C::Q_COL);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc_arrive(&bar[kQFull]);
+            U = kShNone;
+            l = 0.0f;
+            int first = (cur.x.tile0 + cur.tile) * kTcTile + 64 * half;
+            bool begin = true;
+#pragma unroll 1
+            for (; i < end; ++i, first += kTcTile, begin = false) {
             const int b = i & 1;
-            if (begin) {
-                const __half* src = rl < L.rows ? sh_query(a, L, cur, cur.blk * L.rows + rl, D) : nullptr;
-                valid = src != nullptr;
-                busy = __any_sync(0xffffffffu, valid);
-                U = kShNone;
-                l = 0.0f;
-                if (busy) {
-                    uint32_t x[D / 2];
-                    if (!valid) {
-#pragma unroll
-                        for (int k = 0; k < D / 2; ++k) x[k] = 0;
-                    } else if (a.q_aligned) {
-#pragma unroll
-                        for (int k = 0; k < D / 8; ++k) {
-                            const uint4 v = reinterpret_cast<const uint4*>(src)[k];
-                            x[4 * k] = v.x;
-                            x[4 * k + 1] = v.y;
-                            x[4 * k + 2] = v.z;
-                            x[4 * k + 3] = v.w;
-                        }
-                    } else {
-                        const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src);
-#pragma unroll
-                        for (int k = 0; k < D / 2; ++k) x[k] = s16[2 * k] | ((uint32_t)s16[2 * k + 1] << 16);
-                    }
-                    float mag = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < D / 2; ++k) {
-                        const float2 f = __half22float2(bits_h2(x[k]));
-                        mag += fabsf(f.x) + fabsf(f.y);
-                    }
-                    const float mean = mag * (1.0f / D);
-                    const __half h = __float2half_rn(mean);
-                    const float hf = __half2float(h);
-                    const float f = hf == 0.0f ? 1.0f : mean / hf;
-                    sc = f * kShLog2e * rsqrtf((float)D);
-                    const uint32_t hb = __half_as_ushort(h);
-                    // sign part: pairs (i, i + 16) of each word
-#pragma unroll
-                    for (int w = 0; w < NW; ++w) {
-                        uint32_t r[16];
-#pragma unroll
-                        for (int p = 0; p < 16; ++p) {
-                            const int d0 = 32 * w + p, d1 = d0 + 16;
-                            const float f0 = d0 % 2 ? __high2float(bits_h2(x[d0 / 2])) : __low2float(bits_h2(x[d0 / 2]));
-                            const float f1 = d1 % 2 ? __high2float(bits_h2(x[d1 / 2])) : __low2float(bits_h2(x[d1 / 2]));
-                            r[p] = (hb | (f0 >= 0.0f ? 0u : 0x8000u)) | ((hb | (f1 >= 0.0f ? 0u : 0x8000u)) << 16);
-                        }
-                        tc_st16(lane_at + C::Q_COL + 16 * w, r);
-                    }
-                    if constexpr (COMP) {
-                        const float g = (8.0f / 7.0f) / f;
-#pragma unroll
-                        for (int w = 0; w < NW; ++w) {
-                            uint32_t r[16];
-#pragma unroll
-                            for (int p = 0; p < 16; ++p) {
-                                const int d0 = sh_code_dim(D, 32 * w + 2 * p), d1 = sh_code_dim(D, 32 * w + 2 * p + 1);
-                                const float f0 = d0 % 2 ? __high2float(bits_h2(x[d0 / 2])) : __low2float(bits_h2(x[d0 / 2]));
-                                const float f1 = d1 % 2 ? __high2float(bits_h2(x[d1 / 2])) : __low2float(bits_h2(x[d1 / 2]));
-                                r[p] = h2_bits(__floats2half2_rn(f0 * g, f1 * g));
-                            }
-                            tc_st16(lane_at + C::Q_COL + D / 2 + 16 * w, r);
-                        }
-                    }
-                    tc_wait_st();
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) tc_arrive(&bar[kQFull]);
-            }
             ok = __all_sync(0xffffffffu, tc_wait(&bar[kSFull + b], (uint32_t)(i >> 1) & 1u, dead));
             if (!ok) break;
             tc_fence_after();
             if (busy) {
-                const uint32_t s_at = lane_at + C::S_COL + 128 * b;
-                const int kpos = (cur.x.tile0 + cur.tile) * kTcTile;
+                const uint32_t s_at = lane_at + C::S_COL + 128 * b + 64 * half;
                 const bool bad = kbad[i & 7] != 0;
-                const int lo = bad ? kTcTile : max(0, cur.x.lo - kpos), hi = min(kTcTile, cur.x.hi - kpos);
-                const bool masked = lo > 0 || hi < kTcTile;
+                const int lo = bad ? 64 : cur.x.lo - first, hi = cur.x.hi - first;
                 uint32_t v[32];
-                float top = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    tc_ld32(s_at + 32 * c, v);
-                    tc_wait_ld();
-                    if (masked) {
+                if (lo > 0 || hi < 64) {  // keys outside the prefix: their scores to -inf, in place
+#pragma unroll 1
+                    for (int c = 0; c < 2; ++c) {
+                        tc_ld32(s_at + 32 * c, v);
+                        tc_wait_ld();
 #pragma unroll
                         for (int k = 0; k < 32; ++k)
-                            if (32 * c + k >= lo && 32 * c + k < hi) top = fmaxf(top, __uint_as_float(v[k]));
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(v[k]));
+                            if (32 * c + k < lo || 32 * c + k >= hi) v[k] = 0xFF800000u;
+                        tc_st32(s_at + 32 * c, v);
                     }
+                    tc_wait_st();
                 }
-                top *= sc;
+                float top = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    tc_ld32(s_at + 32 * c, v);
+                    tc_wait_ld();
+                    float m[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) m[k] = __uint_as_float(v[k]);
+#pragma unroll
+                    for (int k = 4; k < 32; k += 4)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], __uint_as_float(v[k + j]));
+                    top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+                }
+                xch[256 * (met & 1) + 128 * half] = top;
+                __syncwarp();
+                if (lane == 0) tc_arrive(pair);
+                ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead));
+                if (!ok) break;
+                top = fmaxf(top, xch[256 * (met & 1) + 128 * (half ^ 1)]) * sc;
+                ++met;
                 if (__any_sync(0xffffffffu, top - U > 15.0f)) {
                     const float U1 = top - U > 15.0f ? top - 8.0f : U, f = exp2f(U - U1);
                     U = U1;
@@ -323,232 +389,230 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                         ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead));
                         if (!ok) break;
                         tc_fence_after();
-#pragma unroll
-                        for (int c = 0; c < D / 32; ++c) {
-                            tc_ld32(lane_at + C::O_COL + 32 * c, v);
+#pragma unroll 1
+                        for (int c = 0; c < D / 64; ++c) {
+                            const uint32_t at = lane_at + C::O_COL + D / 2 * half + 32 * c;
+                            tc_ld32(at, v);
                             tc_wait_ld();
 #pragma unroll
                             for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
-                            tc_st32(lane_at + C::O_COL + 32 * c, v);
+                            tc_st32(at, v);
                         }
                         tc_wait_st();
                     }
                 }
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                float2 sum = make_float2(0.0f, 0.0f);
+                const float2 sc2 = make_float2(sc, sc), U2 = make_float2(-U, -U);
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
                     tc_ld32(s_at + 32 * c, v);
                     tc_wait_ld();
                     uint32_t p[16];
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
-                        float e0 = exp2f(__uint_as_float(v[k]) * sc - U), e1 = exp2f(__uint_as_float(v[k + 1]) * sc - U);
-                        if (masked) {
-                            if (32 * c + k < lo || 32 * c + k >= hi) e0 = 0.0f;
-                            if (32 * c + k + 1 < lo || 32 * c + k + 1 >= hi) e1 = 0.0f;
-                        }
-                        l += e0 + e1;
-                        p[k / 2] = h2_bits(__floats2half2_rn(e0, e1));
+                        float2 e = tc_fma2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), sc2, U2);
+                        e.x = exp2f(e.x);
+                        e.y = exp2f(e.y);
+                        sum = tc_add2(sum, e);
+                        p[k / 2] = h2_bits(__floats2half2_rn(e.x, e.y));
                     }
                     tc_st16(s_at + 16 * c, p);
                 }
+                l += sum.x + sum.y;
                 tc_wait_st();
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) tc_arrive(&bar[kPFull + b]);
-            if (sh_piece_ends(cur)) {
-                ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone], (uint32_t)i & 1u, dead));
+            }
+            if (ok) {
+                if (busy) {  // the row's sum: both halves'
+                    xch[256 * (met & 1) + 128 * half] = l;
+                    __syncwarp();
+                    if (lane == 0) tc_arrive(pair);
+                    ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead));
+                    if (!ok) break;
+                    l += xch[256 * (met & 1) + 128 * (half ^ 1)];
+                    ++met;
+                }
+                ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead));
                 if (!ok) break;
                 tc_fence_after();
                 if (busy) {
                     float* row = sh_record(a, L, cur, blockIdx.x, D) + rl * (D + 4);
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
+#pragma unroll 1
+                    for (int c = 0; c < D / 64; ++c) {
                         uint32_t v[32];
-                        tc_ld32(lane_at + C::O_COL + 32 * c, v);
+                        tc_ld32(lane_at + C::O_COL + D / 2 * half + 32 * c, v);
                         tc_wait_ld();
                         if (valid) {
 #pragma unroll
                             for (int k = 0; k < 32; k += 4)
-                                *reinterpret_cast<uint4*>(row + 32 * c + k) = make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                                *reinterpret_cast<uint4*>(row + D / 2 * half + 32 * c + k) =
+                                    make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
                         }
                     }
-                    if (valid) *reinterpret_cast<float2*>(row + D) = make_float2(U, l);
+                    if (valid && half == 0) *reinterpret_cast<float2*>(row + D) = make_float2(U, l);
                 }
                 tc_fence_before();
             }
-            begin = sh_next(a, L, cur);
         }
-    } else if (warp < 8) {
-        // ---------------- unpack K: key `key` of each tile ----------------
-        const int key = tid - 128;
-        for (int i = 0; cur.left > 0; ++i) {
+    } else if (warp < 24 && !(warp & 2)) {
+        // ---------------- unpack K: key `key` of each tile, words part NW / 2 .. ----------------
+        const int part = (warp - 8) >> 3, key = 32 * ((warp & 1) + ((warp >> 1) & 2)) + lane;
+        bool ok = true;
+        for (int i = 0; ok && cur.left > 0; sh_next_piece(a, L, cur))
+#pragma unroll 1
+        for (const int end = i + sh_piece_tiles(cur); i < end; ++i) {
             const int rs_ = i % kTcRaw, b = i & 1;
             const uint8_t* raw = smem + C::RAWK_OFF + rs_ * C::RAW_B;
-            bool ok = tc_wait(&bar[kRawKFull + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
-            uint32_t sg[NW];
-            uint4 nb[COMP ? NW : 1];
-#pragma unroll
-            for (int w = 0; w < NW; ++w) sg[w] = reinterpret_cast<const uint32_t*>(raw)[key * NW + w];
+            ok = tc_wait(&bar[kRawKFull + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
+            if (i >= 2) ok = ok && tc_wait(&bar[kKEmpty + b], (uint32_t)((i >> 1) - 1) & 1u, dead);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            uint8_t* op = smem + b * C::KOP_B + key * 128;
+            const int sw = key & 7;
             const uint32_t bs = *reinterpret_cast<const uint16_t*>(raw + C::BS_OFF + 2 * key);
-            uint32_t rs = 0;
-            if constexpr (COMP) {
-                rs = *reinterpret_cast<const uint16_t*>(raw + C::RS_OFF + 2 * key);
+            const uint32_t flip = (bs | (bs << 16)) ^ 0x80008000u;
+            // word w: units 4w .. 4w + 3 of the sign part, and chunk w those of the code part
+#pragma unroll 1
+            for (int w = part * (NW / 2); w < (part + 1) * (NW / 2); ++w) {
+                const uint32_t sg = reinterpret_cast<const uint32_t*>(raw)[key * NW + w];
+                uint8_t* to = op + (w >> 1) * (kTcTile * 128);
 #pragma unroll
-                for (int c = 0; c < NW; ++c)
-                    nb[c] = *reinterpret_cast<const uint4*>(raw + C::SIGN_B + (key >> 3) * 4 * D + c * 128 + (key & 7) * 16);
+                for (int k = 0; k < 4; ++k)
+                    sts128(to + (((4 * (w & 1) + k) ^ sw) << 4), tc_sign(sg, 4 * k, flip), tc_sign(sg, 4 * k + 1, flip),
+                           tc_sign(sg, 4 * k + 2, flip), tc_sign(sg, 4 * k + 3, flip));
+                if constexpr (COMP) {
+                    const uint32_t rs = *reinterpret_cast<const uint16_t*>(raw + C::RS_OFF + 2 * key);
+                    const __half2 r8 = __hmul2(bits_h2(rs | (rs << 16)), bits_h2(0x30003000u));  // rs / 8
+                    const uint4 nb = *reinterpret_cast<const uint4*>(raw + C::SIGN_B + (key >> 3) * 4 * D + w * 128 + (key & 7) * 16);
+                    const uint32_t w4[4] = {nb.x, nb.y, nb.z, nb.w};
+                    uint8_t* tc = op + ((D / 32 + w) >> 1) * (kTcTile * 128);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t o[4];
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) o[t] = h2_bits(__hmul2(tc_code(w4[j], t), r8));
+                        sts128(tc + (((4 * (w & 1) + j) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+                    }
+                }
             }
             __syncwarp();
             if (lane == 0) tc_arrive(&bar[kRawKEmpty + rs_]);
-            if (i >= 2) ok = ok && tc_wait(&bar[kKEmpty + b], (uint32_t)((i >> 1) - 1) & 1u, dead);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            uint8_t* op = smem + b * C::KOP_B + key * 128;
-            const int sw = key & 7;
-            const uint32_t flip = (bs | (bs << 16)) ^ 0x80008000u;
-#pragma unroll
-            for (int w = 0; w < NW; ++w)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int u = 4 * w + k;
-                    sts128(op + (u >> 3) * (kTcTile * 128) + (((u & 7) ^ sw) << 4), tc_sign(sg[w], 4 * k, flip),
-                           tc_sign(sg[w], 4 * k + 1, flip), tc_sign(sg[w], 4 * k + 2, flip), tc_sign(sg[w], 4 * k + 3, flip));
-                }
-            if constexpr (COMP) {
-                const __half2 r8 = __hmul2(bits_h2(rs | (rs << 16)), bits_h2(0x30003000u));  // rs / 8
-#pragma unroll
-                for (int c = 0; c < NW; ++c) {
-                    const uint32_t w4[4] = {nb[c].x, nb[c].y, nb[c].z, nb[c].w};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int u = D / 8 + 4 * c + w;
-                        uint32_t o[4];
-#pragma unroll
-                        for (int t = 0; t < 4; ++t) o[t] = h2_bits(__hmul2(tc_code(w4[w], t), r8));
-                        sts128(op + (u >> 3) * (kTcTile * 128) + (((u & 7) ^ sw) << 4), o[0], o[1], o[2], o[3]);
-                    }
-                }
-            }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) tc_arrive(&bar[kKFull + b]);
-            sh_next(a, L, cur);
         }
-    } else if (warp < 12) {
-        // ---------------- unpack V ----------------
-        const int key = tid - 256;
-        for (int i = 0; cur.left > 0; ++i) {
+    } else if (warp < 24) {
+        // ---------------- unpack V: chunks part NW / 2 .. ----------------
+        const int part = (warp - 8) >> 3, key = 32 * ((warp & 1) + ((warp >> 1) & 2)) + lane;
+        bool ok = true;
+        for (int i = 0; ok && cur.left > 0; sh_next_piece(a, L, cur)) {
+        int pos = (cur.x.tile0 + cur.tile) * kTcTile + key;
+#pragma unroll 1
+        for (const int end = i + sh_piece_tiles(cur); i < end; ++i, pos += kTcTile) {
             const int rs_ = i % kTcRaw, b = i % C::VST;
             const uint8_t* raw = smem + C::RAWV_OFF + rs_ * C::RAW_B;
-            bool ok = tc_wait(&bar[kRawVFull + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
-            uint32_t sg[NW];
-            uint4 nb[COMP ? NW : 1];
-#pragma unroll
-            for (int w = 0; w < NW; ++w) sg[w] = reinterpret_cast<const uint32_t*>(raw)[key * NW + w];
-            uint32_t bs = *reinterpret_cast<const uint16_t*>(raw + C::BS_OFF + 2 * key);
-            uint32_t rs = 0;
-            if constexpr (COMP) {
-                rs = *reinterpret_cast<const uint16_t*>(raw + C::RS_OFF + 2 * key);
-#pragma unroll
-                for (int c = 0; c < NW; ++c)
-                    nb[c] = *reinterpret_cast<const uint4*>(raw + C::SIGN_B + (key >> 3) * 4 * D + c * 128 + (key & 7) * 16);
-            }
-            // keys outside the prefix: P is 0 there, V has to be finite
-            const int pos = (cur.x.tile0 + cur.tile) * kTcTile + key;
-            if (vbad[i & 7] || pos < cur.x.lo || pos >= cur.x.hi) bs = rs = 0;
-            __syncwarp();
-            if (lane == 0) tc_arrive(&bar[kRawVEmpty + rs_]);
+            ok = tc_wait(&bar[kRawVFull + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
             if (i >= C::VST) ok = ok && tc_wait(&bar[kVEmpty + b], (uint32_t)(i / C::VST - 1) & 1u, dead);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            uint32_t bs = *reinterpret_cast<const uint16_t*>(raw + C::BS_OFF + 2 * key);
+            uint32_t rs = COMP ? *reinterpret_cast<const uint16_t*>(raw + C::RS_OFF + 2 * key) : 0;
+            // keys outside the prefix: P is 0 there, V has to be finite
+            if (vbad[i & 7] || pos < cur.x.lo || pos >= cur.x.hi) bs = rs = 0;
             uint8_t* op = smem + C::V_OFF + b * C::VOP_B + key * 128;
             const int sw = key & 7;
             const uint32_t flip = (bs | (bs << 16)) ^ 0x80008000u;
-            const __half r7 = __float2half_rn(__half2float(__ushort_as_half((uint16_t)rs)) * (1.0f / 7.0f));
-            const __half2 r72 = __half2half2(r7);
-#pragma unroll
-            for (int c = 0; c < NW; ++c) {
+            const __half2 r7 = __float2half2_rn(__half2float(__ushort_as_half((uint16_t)rs)) * (1.0f / 7.0f));
+            // chunk c: units 4c .. 4c + 3.  Nibble n of its word w is bit 4n + first of a sign
+            // word: word w, first c (head_dim 128); word w % 2, first 2c + w / 2 (64)
+            const uint32_t* sgw = reinterpret_cast<const uint32_t*>(raw) + key * NW;
+#pragma unroll 1
+            for (int c = part * (NW / 2); c < (part + 1) * (NW / 2); ++c) {
                 uint32_t w4[4] = {0, 0, 0, 0};
                 if constexpr (COMP) {
-                    w4[0] = nb[c].x;
-                    w4[1] = nb[c].y;
-                    w4[2] = nb[c].z;
-                    w4[3] = nb[c].w;
+                    const uint4 nb = *reinterpret_cast<const uint4*>(raw + C::SIGN_B + (key >> 3) * 4 * D + c * 128 + (key & 7) * 16);
+                    w4[0] = nb.x;
+                    w4[1] = nb.y;
+                    w4[2] = nb.z;
+                    w4[3] = nb.w;
                 }
+                uint8_t* to = op + (c >> 1) * (kTcTile * 128);
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    // nibble n of word w is bit 4n + first of sign word `word`
-                    const int word = D == 128 ? w : D == 64 ? w % 2 : 4 * (c / 4) + w;
-                    const int first = D == 128 ? c : D == 64 ? 2 * c + w / 2 : c % 4;
-                    const int u = 4 * c + w;
+                    const uint32_t sg = D == 128 ? sgw[w] >> c : sgw[w % 2] >> (2 * c + w / 2);
                     uint32_t o[4];
 #pragma unroll
                     for (int t = 0; t < 4; ++t) {
-                        const uint32_t s = tc_sign(sg[word], 4 * t + first, flip);
-                        o[t] = COMP ? h2_bits(__hfma2(tc_code(w4[w], t), r72, bits_h2(s))) : s;
+                        const uint32_t s = tc_sign(sg, 4 * t, flip);
+                        o[t] = COMP ? h2_bits(__hfma2(tc_code(w4[w], t), r7, bits_h2(s))) : s;
                     }
-                    sts128(op + (u >> 3) * (kTcTile * 128) + (((u & 7) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+                    sts128(to + (((4 * (c & 1) + w) ^ sw) << 4), o[0], o[1], o[2], o[3]);
                 }
             }
+            __syncwarp();
+            if (lane == 0) tc_arrive(&bar[kRawVEmpty + rs_]);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) tc_arrive(&bar[kVFull + b]);
-            sh_next(a, L, cur);
         }
-    } else if (warp == 12) {
+        }
+    } else if (warp == 24) {
         // ---------------- products ----------------
         if (lane == 0) {
-            const uint32_t k0 = smem_u32(smem), v0 = smem_u32(smem + C::V_OFF);
-            bool ok = true, pending = false, pv_first = true;
-            auto values = [&](int j) {  // O (+)= P(j) V(j)
+            const uint64_t kd = tc_desc(smem_u32(smem), 16), vd = tc_desc(smem_u32(smem + C::V_OFF), kTcTile * 128);
+            bool ok = true;
+            auto values = [&](int j, bool first) {  // O (+)= P(j) V(j)
                 ok = ok && tc_wait(&bar[kPFull + (j & 1)], (uint32_t)(j >> 1) & 1u, dead) &&
                      tc_wait(&bar[kVFull + j % C::VST], (uint32_t)(j / C::VST) & 1u, dead);
                 if (!ok) return;
                 tc_fence_after();
-                const uint32_t at = v0 + (j % C::VST) * C::VOP_B;
+                const uint64_t at = vd + (j % C::VST) * (C::VOP_B >> 4);
+                const uint32_t p = tmem + C::S_COL + 128 * (j & 1);
 #pragma unroll
                 for (int k = 0; k < kTcTile / 16; ++k)
-                    tc_mma(tmem + C::O_COL, tmem + C::S_COL + 128 * (j & 1) + 8 * k, tc_desc(at + 2048 * k, kTcTile * 128),
-                           tc_idesc(D, true), !(pv_first && k == 0));
+                    tc_mma(tmem + C::O_COL, p + 64 * (k / 4) + 8 * (k % 4), at + (2048 >> 4) * k, tc_idesc(D, true),
+                           !(first && k == 0));
                 tc_commit(&bar[kVEmpty + j % C::VST]);
                 tc_commit(&bar[kPvDone]);
             };
-            bool begin = true;
-            int i = 0, items = 0;
-            for (; ok && cur.left > 0; ++i) {
-                const int b = i & 1;
-                if (begin) {
-                    if (pending) values(i - 1);  // the next item's queries come after the last one's results
-                    pending = false;
-                    ok = ok && tc_wait(&bar[kQFull], (uint32_t)items & 1u, dead);
-                    ++items;
-                }
-                ok = ok && tc_wait(&bar[kKFull + b], (uint32_t)(i >> 1) & 1u, dead);
-                if (!ok) break;
-                tc_fence_after();
+            int i = 0;
+            for (int items = 0; ok && cur.left > 0; ++items, sh_next_piece(a, L, cur)) {
+                const int from = i, end = i + sh_piece_tiles(cur);
+                ok = tc_wait(&bar[kQFull], (uint32_t)items & 1u, dead);
+                // the scores of a tile go before the values of the one before it; a piece's last values
+                // before the next one's scores, whose queries are there only then
+#pragma unroll 1
+                for (; ok && i <= end; ++i) {
+                    if (i < end) {
+                        const int b = i & 1;
+                        ok = tc_wait(&bar[kKFull + b], (uint32_t)(i >> 1) & 1u, dead);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t at = kd + b * (C::KOP_B >> 4);
 #pragma unroll
-                for (int k = 0; k < C::KE / 16; ++k)
-                    tc_mma(tmem + C::S_COL + 128 * b, tmem + C::Q_COL + 8 * k,
-                           tc_desc(k0 + b * C::KOP_B + (k >> 2) * (kTcTile * 128) + (k & 3) * 32, 16), tc_idesc(kTcTile, false),
-                           k > 0);
-                tc_commit(&bar[kKEmpty + b]);
-                tc_commit(&bar[kSFull + b]);
-                if (pending) {
-                    values(i - 1);
-                    pv_first = false;
+                        for (int k = 0; k < C::KE / 16; ++k)
+                            tc_mma(tmem + C::S_COL + 128 * b, tmem + C::Q_COL + 8 * k,
+                                   at + (k >> 2) * (kTcTile * 128 >> 4) + (k & 3) * 2, tc_idesc(kTcTile, false), k > 0);
+                        tc_commit(&bar[kKEmpty + b]);
+                        tc_commit(&bar[kSFull + b]);
+                    }
+                    if (i > from) values(i - 1, i - 1 == from);
                 }
-                if (begin) pv_first = true;
-                pending = true;
-                begin = sh_next(a, L, cur);
+                i = end;
             }
-            if (pending) values(i - 1);
             if (!ok) raise_device_error(a.err, BC_DEVERR_TIMEOUT);
             tc_commit(&bar[kDrain]);
+#pragma unroll 1
             for (uint32_t it = 0; it < kTcSpin; ++it)
                 if (mbar_try_wait(&bar[kDrain], 0)) break;
         }
     } else {
-        // ---------------- packed tiles of K (warp 13) or V (warp 14) ----------------
+        // ---------------- packed tiles of K (warp 25) or V (warp 26) ----------------
         if (lane == 0) {
-            const bool is_v = warp == 14;
+            const bool is_v = warp == 26;
             const bc_kv_planes& P = is_v ? a.V : a.K;
             uint8_t* ring = smem + (is_v ? C::RAWV_OFF : C::RAWK_OFF);
             uint64_t* full = bar + (is_v ? kRawVFull : kRawKFull);
@@ -556,34 +620,42 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             volatile int* flag = is_v ? vbad : kbad;
             bool ok = true;
             int i = 0;
-            for (; cur.left > 0; ++i) {
-                const int s = i % kTcRaw;
-                if (i >= kTcRaw) ok = tc_wait(&empty[s], (uint32_t)(i / kTcRaw - 1) & 1u, dead);
-                if (!ok) break;
-                const int pos = (cur.x.tile0 + cur.tile) * kTcTile;
-                const int j = pos / a.pt.page_size;
-                const int pg = __ldg(a.pt.pages + ((int64_t)sh_lead(a, L, cur) * a.n_kv + cur.h) * a.pt.max_pages + j);
-                const bool here = pg >= 0 && pg < a.pt.n_pages;
-                flag[i & 7] = !here;
-                if (here) {
-                    const int64_t row = (int64_t)pg * a.pt.page_size + (pos - j * a.pt.page_size);
-                    uint8_t* dst = ring + s * C::RAW_B;
-                    fence_proxy_async_smem();
-                    mbar_arrive_expect_tx(&full[s], C::RAW_B);
-                    bulk_g2s(dst, (const uint8_t*)P.sign + row * (D / 8), C::SIGN_B, &full[s]);
-                    bulk_g2s(dst + C::BS_OFF, (const uint8_t*)P.bscale + row * 2, C::SC_B, &full[s]);
-                    if constexpr (COMP) {
-                        bulk_g2s(dst + C::SIGN_B, (const uint8_t*)P.nib + row * (D / 2), C::NIB_B, &full[s]);
-                        bulk_g2s(dst + C::RS_OFF, (const uint8_t*)P.rscale + row * 2, C::SC_B, &full[s]);
+            for (; ok && cur.left > 0; sh_next_piece(a, L, cur)) {
+                const int pos = (cur.x.tile0 + cur.tile) * kTcTile, j = pos / a.pt.page_size;
+                const int32_t* page = a.pt.pages + ((int64_t)sh_lead(a, L, cur) * a.n_kv + cur.h) * a.pt.max_pages + j;
+                int in_page = pos - j * a.pt.page_size, pg = __ldg(page);
+#pragma unroll 1
+                for (const int end = i + sh_piece_tiles(cur); i < end; ++i) {
+                    const int s = i % kTcRaw;
+                    if (i >= kTcRaw) ok = tc_wait(&empty[s], (uint32_t)(i / kTcRaw - 1) & 1u, dead);
+                    if (!ok) break;
+                    const bool here = pg >= 0 && pg < a.pt.n_pages;
+                    flag[i & 7] = !here;
+                    if (here) {
+                        const int64_t row = (int64_t)pg * a.pt.page_size + in_page;
+                        uint8_t* dst = ring + s * C::RAW_B;
+                        fence_proxy_async_smem();
+                        mbar_arrive_expect_tx(&full[s], C::RAW_B);
+                        bulk_g2s(dst, (const uint8_t*)P.sign + row * (D / 8), C::SIGN_B, &full[s]);
+                        bulk_g2s(dst + C::BS_OFF, (const uint8_t*)P.bscale + row * 2, C::SC_B, &full[s]);
+                        if constexpr (COMP) {
+                            bulk_g2s(dst + C::SIGN_B, (const uint8_t*)P.nib + row * (D / 2), C::NIB_B, &full[s]);
+                            bulk_g2s(dst + C::RS_OFF, (const uint8_t*)P.rscale + row * 2, C::SC_B, &full[s]);
+                        }
+                    } else {
+                        if (!is_v) raise_device_error(a.err, BC_DEVERR_PAGE);
+                        tc_arrive(&full[s]);
                     }
-                } else {
-                    if (!is_v) raise_device_error(a.err, BC_DEVERR_PAGE);
-                    tc_arrive(&full[s]);
+                    in_page += kTcTile;
+                    if (in_page == a.pt.page_size && i + 1 < end) {
+                        in_page = 0;
+                        pg = __ldg(++page);
+                    }
                 }
-                sh_next(a, L, cur);
             }
             // copies in flight land before the block's memory is given back (bounded)
             for (int t = max(0, i - kTcRaw); t < i; ++t)
+#pragma unroll 1
                 for (uint32_t it = 0; it < kTcSpin; ++it)
                     if (mbar_try_wait(&full[t % kTcRaw], (uint32_t)(t / kTcRaw) & 1u)) break;
         }
@@ -592,7 +664,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 12) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (warp == 24) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
 template <int D, bool COMP>
