@@ -39,31 +39,32 @@ namespace bc {
 namespace {
 
 constexpr int kTcTile = 128;
-constexpr int kTcThreads = 27 * 32;
+constexpr int kTcThreads = 28 * 32;
 constexpr int kTcUnpackWarps = 8;   // of K, and of V
 constexpr int kTcRaw = 3;        // packed tiles ahead
 constexpr int kTcItemCost = 2;   // an item's start and end, in tiles
-constexpr uint32_t kTcSpin = 1u << 22;
+constexpr uint32_t kTcSpin = 1u << 19;  // polls of a wait before it gives up: about a second
 
 template <int D, bool COMP>
 struct TcCfg {
     static constexpr int KE = COMP ? 2 * D : D;              // elements of a K row
-    static constexpr int KOP_B = kTcTile * KE * 2;
+    static constexpr int PARTS = COMP ? 2 : 1;               // sign part, code part
+    static constexpr int KOP_B = kTcTile * D * 2;            // one part of a K operand tile
     static constexpr int VOP_B = kTcTile * D * 2;
-    static constexpr int VST = D == 128 && COMP ? 1 : 2;     // V operand tiles
+    static constexpr int KST = 3, VST = 2;                   // K operand parts, V operand tiles
     static constexpr int SIGN_B = kTcTile * D / 8;
     static constexpr int NIB_B = COMP ? kTcTile * D / 2 : 0;
     static constexpr int SC_B = kTcTile * 2;
     static constexpr int BS_OFF = SIGN_B + NIB_B;
     static constexpr int RS_OFF = BS_OFF + SC_B;
     static constexpr int RAW_B = SIGN_B + NIB_B + SC_B * (COMP ? 2 : 1);
-    static constexpr int V_OFF = 2 * KOP_B;
+    static constexpr int V_OFF = KST * KOP_B;
     static constexpr int RAWK_OFF = V_OFF + VST * VOP_B;
     static constexpr int RAWV_OFF = RAWK_OFF + kTcRaw * RAW_B;
     static constexpr int SCAN_OFF = (RAWV_OFF + kTcRaw * RAW_B + 15) / 16 * 16;
     static constexpr int XCH_OFF = SCAN_OFF;  // [2][2][128] maxima of the row halves, once the sums are read
     static constexpr int BAR_OFF = SCAN_OFF + 512 * 4;
-    static constexpr int FLAG_OFF = BAR_OFF + 32 * 8;
+    static constexpr int FLAG_OFF = BAR_OFF + 34 * 8;
     static constexpr int SMEM_B = FLAG_OFF + 20 * 4 + 1024;  // + alignment to the swizzle atom
     // tensor memory columns
     static constexpr int S_COL = 0, O_COL = 256, Q_COL = 256 + D;
@@ -71,21 +72,33 @@ struct TcCfg {
 };
 
 enum TcBar {
-    kRawKFull = 0, kRawKEmpty = 3, kRawVFull = 6, kRawVEmpty = 9, kKFull = 12, kKEmpty = 14, kVFull = 16, kVEmpty = 18,
-    kSFull = 20, kPFull = 22, kQFull = 24, kPvDone = 25, kDrain = 26, kPair = 27, kTcBars = 31
+    kRawKFull = 0, kRawKEmpty = 3, kRawVFull = 6, kRawVEmpty = 9, kKFull = 12, kKEmpty = 15, kVFull = 18, kVEmpty = 20,
+    kSFull = 22, kPFull = 24, kQFull = 26, kPvDone = 27, kDrain = 28, kPair = 29, kDone = 33, kTcBars = 34
 };
 
 // ---- tcgen05 ---------------------------------------------------------------
-__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// The issuing warp runs its loop with all lanes, and `one` picks the lane that
+// issues: the addresses then live in uniform registers, which the instruction
+// wants (from one lane's branch each product cost some 150 clocks to issue).
+__device__ __forceinline__ uint32_t tc_elect() {
+    uint32_t one;
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate)
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one;
+}
+__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate, uint32_t one) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)accumulate), "r"(one)
         : "memory");
 }
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+__device__ __forceinline__ void tc_commit(uint64_t* bar, uint32_t one) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(one)
+        : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -112,6 +125,14 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) 
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
         "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tc_ld16(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
         : "memory");
 }
 __device__ __forceinline__ void tc_st16(uint32_t addr, const uint32_t (&r)[16]) {
@@ -148,6 +169,13 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
 }
 __device__ __forceinline__ void tc_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// A warp's end: its use of tensor memory is over.
+__device__ __forceinline__ void tc_leave(uint64_t* done) {
+    tc_fence_before();
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) tc_arrive(done);
 }
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<const uint32_t*>(&h); }
@@ -272,7 +300,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
     volatile int* vbad = flags + 8;    // [8]
     volatile int* dead = flags + 16;
     volatile uint32_t* tmem_at = reinterpret_cast<volatile uint32_t*>(flags + 17);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
     sh_wait_before();
     sh_let_next();
@@ -290,10 +318,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             mbar_init(&bar[kRawKEmpty + i], kTcUnpackWarps);
             mbar_init(&bar[kRawVEmpty + i], kTcUnpackWarps);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < C::KST; ++i) {
             mbar_init(&bar[kKFull + i], kTcUnpackWarps);
-            mbar_init(&bar[kVFull + i], kTcUnpackWarps);
             mbar_init(&bar[kKEmpty + i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar[kVFull + i], kTcUnpackWarps);
             mbar_init(&bar[kVEmpty + i], 1);
             mbar_init(&bar[kSFull + i], 1);
             mbar_init(&bar[kPFull + i], 8);
@@ -302,6 +332,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
         for (int i = 0; i < 4; ++i) mbar_init(&bar[kPair + i], 2);
         mbar_init(&bar[kPvDone], 1);
         mbar_init(&bar[kDrain], 1);
+        mbar_init(&bar[kDone], kTcThreads / 32 - 1);
         fence_mbar_init();
     }
     if (warp == 24) {
@@ -313,9 +344,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_at;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
 
+    // registers: 256 x 112 + 512 x 56 + 128 x 48 of the 896 x 72 launched
     if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
         // ---------------- softmax: row `rl` of the item's block, keys 64 half .. 64 half + 63 ----------------
         const int half = warp >> 2, quad = warp & 3;
         const uint32_t lane_at = tmem + ((uint32_t)(32 * quad) << 16);
@@ -345,80 +378,84 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             tc_fence_after();
             if (busy) {
                 const uint32_t s_at = lane_at + C::S_COL + 128 * b + 64 * half;
-                const bool bad = kbad[i & 7] != 0;
-                const int lo = bad ? 64 : cur.x.lo - first, hi = cur.x.hi - first;
-                uint32_t v[32];
-                if (lo > 0 || hi < 64) {  // keys outside the prefix: their scores to -inf, in place
-#pragma unroll 1
-                    for (int c = 0; c < 2; ++c) {
-                        tc_ld32(s_at + 32 * c, v);
-                        tc_wait_ld();
+                const int lo = kbad[i & 7] ? 64 : cur.x.lo - first, hi = cur.x.hi - first;
+                uint32_t v[64];
+                tc_ld32(s_at, *reinterpret_cast<uint32_t(*)[32]>(v));
+                tc_ld32(s_at + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+                tc_wait_ld();
+                if (lo > 0 || hi < 64) {  // keys outside the prefix
 #pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            if (32 * c + k < lo || 32 * c + k >= hi) v[k] = 0xFF800000u;
-                        tc_st32(s_at + 32 * c, v);
-                    }
-                    tc_wait_st();
+                    for (int k = 0; k < 64; ++k)
+                        if (k < lo || k >= hi) v[k] = 0xFF800000u;
                 }
-                float top = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    tc_ld32(s_at + 32 * c, v);
-                    tc_wait_ld();
-                    float m[4];
+                float m[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) m[k] = __uint_as_float(v[k]);
+                for (int k = 0; k < 4; ++k) m[k] = __uint_as_float(v[k]);
 #pragma unroll
-                    for (int k = 4; k < 32; k += 4)
+                for (int k = 4; k < 64; k += 4)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], __uint_as_float(v[k + j]));
-                    top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
-                }
+                    for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], __uint_as_float(v[k + j]));
+                float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                 xch[256 * (met & 1) + 128 * half] = top;
                 __syncwarp();
                 if (lane == 0) tc_arrive(pair);
-                ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead));
-                if (!ok) break;
-                top = fmaxf(top, xch[256 * (met & 1) + 128 * (half ^ 1)]) * sc;
-                ++met;
-                if (__any_sync(0xffffffffu, top - U > 15.0f)) {
-                    const float U1 = top - U > 15.0f ? top - 8.0f : U, f = exp2f(U - U1);
-                    U = U1;
-                    l *= f;
-                    if (!begin) {  // O holds the piece's tiles so far, once their products are through
-                        ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead));
-                        if (!ok) break;
-                        tc_fence_after();
+                // P with the U of the tiles so far; the maxima, the other half's too, are looked at
+                // afterwards, and in the rare case that U has to rise P is made once more
+                bool again = begin, seen = false;
+                float tile_sum;
 #pragma unroll 1
-                        for (int c = 0; c < D / 64; ++c) {
-                            const uint32_t at = lane_at + C::O_COL + D / 2 * half + 32 * c;
-                            tc_ld32(at, v);
-                            tc_wait_ld();
+                for (;;) {
+                    float2 sum = make_float2(0.0f, 0.0f);
+                    if (!again) {
+                        const float2 sc2 = make_float2(sc, sc), U2 = make_float2(-U, -U);
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
-                            tc_st32(at, v);
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t p[16];
+#pragma unroll
+                            for (int k = 0; k < 32; k += 2) {
+                                float2 e = tc_fma2(make_float2(__uint_as_float(v[32 * c + k]), __uint_as_float(v[32 * c + k + 1])),
+                                                   sc2, U2);
+                                e.x = exp2f(e.x);
+                                e.y = exp2f(e.y);
+                                sum = tc_add2(sum, e);
+                                p[k / 2] = h2_bits(__floats2half2_rn(e.x, e.y));
+                            }
+                            tc_st16(s_at + 16 * c, p);
                         }
-                        tc_wait_st();
                     }
-                }
-                float2 sum = make_float2(0.0f, 0.0f);
-                const float2 sc2 = make_float2(sc, sc), U2 = make_float2(-U, -U);
+                    tile_sum = sum.x + sum.y;
+                    if (seen) break;
+                    ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead));
+                    if (!ok) break;
+                    top = fmaxf(top, xch[256 * (met & 1) + 128 * (half ^ 1)]) * sc;
+                    const bool rise = __any_sync(0xffffffffu, top - U > 15.0f);
+                    if (!rise && !again) break;
+                    if (rise) {
+                        const float U1 = top - U > 15.0f ? top - 8.0f : U, f = exp2f(U - U1);
+                        U = U1;
+                        l *= f;
+                        if (!begin) {  // O holds the piece's tiles so far, once their products are through
+                            ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead));
+                            if (!ok) break;
+                            tc_fence_after();
 #pragma unroll 1
-                for (int c = 0; c < 2; ++c) {
-                    tc_ld32(s_at + 32 * c, v);
-                    tc_wait_ld();
-                    uint32_t p[16];
+                            for (int c = 0; c < D / 32; ++c) {
+                                const uint32_t at = lane_at + C::O_COL + D / 2 * half + 16 * c;
+                                uint32_t o[16];
+                                tc_ld16(at, o);
+                                tc_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        float2 e = tc_fma2(make_float2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])), sc2, U2);
-                        e.x = exp2f(e.x);
-                        e.y = exp2f(e.y);
-                        sum = tc_add2(sum, e);
-                        p[k / 2] = h2_bits(__floats2half2_rn(e.x, e.y));
+                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                tc_st16(at, o);
+                            }
+                        }
                     }
-                    tc_st16(s_at + 16 * c, p);
+                    seen = true;
+                    again = false;
                 }
-                l += sum.x + sum.y;
+                if (!ok) break;
+                ++met;
+                l += tile_sum;
                 tc_wait_st();
             }
             tc_fence_before();
@@ -457,116 +494,154 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                 tc_fence_before();
             }
         }
-    } else if (warp < 24 && !(warp & 2)) {
-        // ---------------- unpack K: key `key` of each tile, words part NW / 2 .. ----------------
-        const int part = (warp - 8) >> 3, key = 32 * ((warp & 1) + ((warp >> 1) & 2)) + lane;
+        tc_leave(&bar[kDone]);
+        return;
+    }
+    if (warp < 24) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        const int part = (warp - 8) >> 3, key = 32 * (warp & 3) + lane, sw = key & 7;
+        int i = 0;
         bool ok = true;
-        for (int i = 0; ok && cur.left > 0; sh_next_piece(a, L, cur))
+        if (!(warp & 4)) {
+            // ---------------- unpack K: words (and chunks) NW / 2 part .. of key `key` ----------------
+            int slot = 0;
+            uint32_t round = 0;  // of the operand ring
+            auto next = [&]() {
+                if (++slot == C::KST) {
+                    slot = 0;
+                    ++round;
+                }
+            };
+            for (; ok && cur.left > 0; sh_next_piece(a, L, cur))
 #pragma unroll 1
-        for (const int end = i + sh_piece_tiles(cur); i < end; ++i) {
-            const int rs_ = i % kTcRaw, b = i & 1;
-            const uint8_t* raw = smem + C::RAWK_OFF + rs_ * C::RAW_B;
-            ok = tc_wait(&bar[kRawKFull + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
-            if (i >= 2) ok = ok && tc_wait(&bar[kKEmpty + b], (uint32_t)((i >> 1) - 1) & 1u, dead);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            uint8_t* op = smem + b * C::KOP_B + key * 128;
-            const int sw = key & 7;
-            const uint32_t bs = *reinterpret_cast<const uint16_t*>(raw + C::BS_OFF + 2 * key);
-            const uint32_t flip = (bs | (bs << 16)) ^ 0x80008000u;
-            // word w: units 4w .. 4w + 3 of the sign part, and chunk w those of the code part
+                for (const int end = i + sh_piece_tiles(cur); i < end; ++i) {
+                    const int rs_ = i % kTcRaw;
+                    const uint8_t* raw = smem + C::RAWK_OFF + rs_ * C::RAW_B;
+                    ok = tc_wait(&bar[kRawKFull + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
+                    if (round) ok = ok && tc_wait(&bar[kKEmpty + slot], (round - 1) & 1u, dead);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    uint8_t* op = smem + slot * C::KOP_B + key * 128;
+                    const uint32_t bs = *reinterpret_cast<const uint16_t*>(raw + C::BS_OFF + 2 * key);
+                    const uint32_t flip = (bs | (bs << 16)) ^ 0x80008000u;
 #pragma unroll 1
-            for (int w = part * (NW / 2); w < (part + 1) * (NW / 2); ++w) {
-                const uint32_t sg = reinterpret_cast<const uint32_t*>(raw)[key * NW + w];
-                uint8_t* to = op + (w >> 1) * (kTcTile * 128);
+                    for (int w = part * (NW / 2); w < (part + 1) * (NW / 2); ++w) {
+                        const uint32_t sg = reinterpret_cast<const uint32_t*>(raw)[key * NW + w];
+                        uint8_t* to = op + (w >> 1) * (kTcTile * 128);
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    sts128(to + (((4 * (w & 1) + k) ^ sw) << 4), tc_sign(sg, 4 * k, flip), tc_sign(sg, 4 * k + 1, flip),
-                           tc_sign(sg, 4 * k + 2, flip), tc_sign(sg, 4 * k + 3, flip));
-                if constexpr (COMP) {
-                    const uint32_t rs = *reinterpret_cast<const uint16_t*>(raw + C::RS_OFF + 2 * key);
-                    const __half2 r8 = __hmul2(bits_h2(rs | (rs << 16)), bits_h2(0x30003000u));  // rs / 8
-                    const uint4 nb = *reinterpret_cast<const uint4*>(raw + C::SIGN_B + (key >> 3) * 4 * D + w * 128 + (key & 7) * 16);
-                    const uint32_t w4[4] = {nb.x, nb.y, nb.z, nb.w};
-                    uint8_t* tc = op + ((D / 32 + w) >> 1) * (kTcTile * 128);
+                        for (int k = 0; k < 4; ++k)
+                            sts128(to + (((4 * (w & 1) + k) ^ sw) << 4), tc_sign(sg, 4 * k, flip), tc_sign(sg, 4 * k + 1, flip),
+                                   tc_sign(sg, 4 * k + 2, flip), tc_sign(sg, 4 * k + 3, flip));
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) tc_arrive(&bar[kKFull + slot]);
+                    next();
+                    if constexpr (COMP) {
+                        if (round) ok = tc_wait(&bar[kKEmpty + slot], (round - 1) & 1u, dead);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (!ok) break;
+                        op = smem + slot * C::KOP_B + key * 128;
+                        const uint32_t rs = *reinterpret_cast<const uint16_t*>(raw + C::RS_OFF + 2 * key);
+                        const __half2 r8 = __hmul2(bits_h2(rs | (rs << 16)), bits_h2(0x30003000u));  // rs / 8
+#pragma unroll 1
+                        for (int c = part * (NW / 2); c < (part + 1) * (NW / 2); ++c) {
+                            const uint4 nb = *reinterpret_cast<const uint4*>(raw + C::SIGN_B + (key >> 3) * 4 * D + c * 128 + (key & 7) * 16);
+                            const uint32_t w4[4] = {nb.x, nb.y, nb.z, nb.w};
+                            uint8_t* to = op + (c >> 1) * (kTcTile * 128);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t o[4];
+                            for (int j = 0; j < 4; ++j) {
+                                uint32_t o[4];
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) o[t] = h2_bits(__hmul2(tc_code(w4[j], t), r8));
-                        sts128(tc + (((4 * (w & 1) + j) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+                                for (int t = 0; t < 4; ++t) o[t] = h2_bits(__hmul2(tc_code(w4[j], t), r8));
+                                sts128(to + (((4 * (c & 1) + j) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+                            }
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) tc_arrive(&bar[kKFull + slot]);
+                        next();
+                    }
+                    if (lane == 0) tc_arrive(&bar[kRawKEmpty + rs_]);
+                }
+        } else {
+            // ---------------- unpack V: chunks NW / 2 part .. ----------------
+            for (; ok && cur.left > 0; sh_next_piece(a, L, cur)) {
+                int pos = (cur.x.tile0 + cur.tile) * kTcTile + key;
+#pragma unroll 1
+                for (const int end = i + sh_piece_tiles(cur); i < end; ++i, pos += kTcTile) {
+                    const int rs_ = i % kTcRaw, b = i % C::VST;
+                    const uint8_t* raw = smem + C::RAWV_OFF + rs_ * C::RAW_B;
+                    ok = tc_wait(&bar[kRawVFull + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
+                    if (i >= C::VST) ok = ok && tc_wait(&bar[kVEmpty + b], (uint32_t)(i / C::VST - 1) & 1u, dead);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    uint32_t bs = *reinterpret_cast<const uint16_t*>(raw + C::BS_OFF + 2 * key);
+                    uint32_t rs = COMP ? *reinterpret_cast<const uint16_t*>(raw + C::RS_OFF + 2 * key) : 0;
+                    // keys outside the prefix: P is 0 there, V has to be finite
+                    if (vbad[i & 7] || pos < cur.x.lo || pos >= cur.x.hi) bs = rs = 0;
+                    uint8_t* op = smem + C::V_OFF + b * C::VOP_B + key * 128;
+                    const uint32_t flip = (bs | (bs << 16)) ^ 0x80008000u;
+                    const __half2 r7 = __float2half2_rn(__half2float(__ushort_as_half((uint16_t)rs)) * (1.0f / 7.0f));
+                    // chunk c: units 4c .. 4c + 3.  Nibble n of its word w is bit 4n + first of a sign
+                    // word: word w, first c (head_dim 128); word w % 2, first 2c + w / 2 (64)
+                    uint32_t sgw[NW];
+                    if constexpr (D == 128) {
+                        const uint4 x = *reinterpret_cast<const uint4*>(raw + key * 16);
+                        sgw[0] = x.x;
+                        sgw[1] = x.y;
+                        sgw[2] = x.z;
+                        sgw[3] = x.w;
+                    } else {
+                        const uint2 x = *reinterpret_cast<const uint2*>(raw + key * 8);
+                        sgw[0] = x.x;
+                        sgw[1] = x.y;
+                    }
+#pragma unroll 1
+                    for (int c = part * (NW / 2); c < (part + 1) * (NW / 2); ++c) {
+                        uint32_t w4[4] = {0, 0, 0, 0};
+                        if constexpr (COMP) {
+                            const uint4 nb = *reinterpret_cast<const uint4*>(raw + C::SIGN_B + (key >> 3) * 4 * D + c * 128 + (key & 7) * 16);
+                            w4[0] = nb.x;
+                            w4[1] = nb.y;
+                            w4[2] = nb.z;
+                            w4[3] = nb.w;
+                        }
+                        uint8_t* to = op + (c >> 1) * (kTcTile * 128);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t sg = D == 128 ? sgw[w % NW] >> c : sgw[w % 2] >> (2 * c + w / 2);
+                            uint32_t o[4];
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                const uint32_t x = tc_sign(sg, 4 * t, flip);
+                                o[t] = COMP ? h2_bits(__hfma2(tc_code(w4[w], t), r7, bits_h2(x))) : x;
+                            }
+                            sts128(to + (((4 * (c & 1) + w) ^ sw) << 4), o[0], o[1], o[2], o[3]);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tc_arrive(&bar[kVFull + b]);
+                        tc_arrive(&bar[kRawVEmpty + rs_]);
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) tc_arrive(&bar[kRawKEmpty + rs_]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) tc_arrive(&bar[kKFull + b]);
         }
-    } else if (warp < 24) {
-        // ---------------- unpack V: chunks part NW / 2 .. ----------------
-        const int part = (warp - 8) >> 3, key = 32 * ((warp & 1) + ((warp >> 1) & 2)) + lane;
-        bool ok = true;
-        for (int i = 0; ok && cur.left > 0; sh_next_piece(a, L, cur)) {
-        int pos = (cur.x.tile0 + cur.tile) * kTcTile + key;
-#pragma unroll 1
-        for (const int end = i + sh_piece_tiles(cur); i < end; ++i, pos += kTcTile) {
-            const int rs_ = i % kTcRaw, b = i % C::VST;
-            const uint8_t* raw = smem + C::RAWV_OFF + rs_ * C::RAW_B;
-            ok = tc_wait(&bar[kRawVFull + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
-            if (i >= C::VST) ok = ok && tc_wait(&bar[kVEmpty + b], (uint32_t)(i / C::VST - 1) & 1u, dead);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            uint32_t bs = *reinterpret_cast<const uint16_t*>(raw + C::BS_OFF + 2 * key);
-            uint32_t rs = COMP ? *reinterpret_cast<const uint16_t*>(raw + C::RS_OFF + 2 * key) : 0;
-            // keys outside the prefix: P is 0 there, V has to be finite
-            if (vbad[i & 7] || pos < cur.x.lo || pos >= cur.x.hi) bs = rs = 0;
-            uint8_t* op = smem + C::V_OFF + b * C::VOP_B + key * 128;
-            const int sw = key & 7;
-            const uint32_t flip = (bs | (bs << 16)) ^ 0x80008000u;
-            const __half2 r7 = __float2half2_rn(__half2float(__ushort_as_half((uint16_t)rs)) * (1.0f / 7.0f));
-            // chunk c: units 4c .. 4c + 3.  Nibble n of its word w is bit 4n + first of a sign
-            // word: word w, first c (head_dim 128); word w % 2, first 2c + w / 2 (64)
-            const uint32_t* sgw = reinterpret_cast<const uint32_t*>(raw) + key * NW;
-#pragma unroll 1
-            for (int c = part * (NW / 2); c < (part + 1) * (NW / 2); ++c) {
-                uint32_t w4[4] = {0, 0, 0, 0};
-                if constexpr (COMP) {
-                    const uint4 nb = *reinterpret_cast<const uint4*>(raw + C::SIGN_B + (key >> 3) * 4 * D + c * 128 + (key & 7) * 16);
-                    w4[0] = nb.x;
-                    w4[1] = nb.y;
-                    w4[2] = nb.z;
-                    w4[3] = nb.w;
-                }
-                uint8_t* to = op + (c >> 1) * (kTcTile * 128);
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t sg = D == 128 ? sgw[w] >> c : sgw[w % 2] >> (2 * c + w / 2);
-                    uint32_t o[4];
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const uint32_t s = tc_sign(sg, 4 * t, flip);
-                        o[t] = COMP ? h2_bits(__hfma2(tc_code(w4[w], t), r7, bits_h2(s))) : s;
-                    }
-                    sts128(to + (((4 * (c & 1) + w) ^ sw) << 4), o[0], o[1], o[2], o[3]);
-                }
-            }
-            __syncwarp();
-            if (lane == 0) tc_arrive(&bar[kRawVEmpty + rs_]);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) tc_arrive(&bar[kVFull + b]);
-        }
-        }
-    } else if (warp == 24) {
+        tc_leave(&bar[kDone]);
+        return;
+    }
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    if (warp == 24) {
         // ---------------- products ----------------
-        if (lane == 0) {
+        {
+            const uint32_t one = tc_elect();
             const uint64_t kd = tc_desc(smem_u32(smem), 16), vd = tc_desc(smem_u32(smem + C::V_OFF), kTcTile * 128);
             bool ok = true;
             auto values = [&](int j, bool first) {  // O (+)= P(j) V(j)
-                ok = ok && tc_wait(&bar[kPFull + (j & 1)], (uint32_t)(j >> 1) & 1u, dead) &&
-                     tc_wait(&bar[kVFull + j % C::VST], (uint32_t)(j / C::VST) & 1u, dead);
+                ok = __all_sync(0xffffffffu, ok && tc_wait(&bar[kPFull + (j & 1)], (uint32_t)(j >> 1) & 1u, dead) &&
+                                                 tc_wait(&bar[kVFull + j % C::VST], (uint32_t)(j / C::VST) & 1u, dead));
                 if (!ok) return;
                 tc_fence_after();
                 const uint64_t at = vd + (j % C::VST) * (C::VOP_B >> 4);
@@ -574,42 +649,62 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
 #pragma unroll
                 for (int k = 0; k < kTcTile / 16; ++k)
                     tc_mma(tmem + C::O_COL, p + 64 * (k / 4) + 8 * (k % 4), at + (2048 >> 4) * k, tc_idesc(D, true),
-                           !(first && k == 0));
-                tc_commit(&bar[kVEmpty + j % C::VST]);
-                tc_commit(&bar[kPvDone]);
+                           !(first && k == 0), one);
+                tc_commit(&bar[kVEmpty + j % C::VST], one);
+                tc_commit(&bar[kPvDone], one);
             };
-            int i = 0;
+            int i = 0, slot = 0;
+            uint32_t round = 0;
             for (int items = 0; ok && cur.left > 0; ++items, sh_next_piece(a, L, cur)) {
                 const int from = i, end = i + sh_piece_tiles(cur);
-                ok = tc_wait(&bar[kQFull], (uint32_t)items & 1u, dead);
+                ok = __all_sync(0xffffffffu, tc_wait(&bar[kQFull], (uint32_t)items & 1u, dead));
                 // the scores of a tile go before the values of the one before it; a piece's last values
                 // before the next one's scores, whose queries are there only then
 #pragma unroll 1
                 for (; ok && i <= end; ++i) {
                     if (i < end) {
                         const int b = i & 1;
-                        ok = tc_wait(&bar[kKFull + b], (uint32_t)(i >> 1) & 1u, dead);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint64_t at = kd + b * (C::KOP_B >> 4);
+#pragma unroll 1
+                        for (int part = 0; ok && part < C::PARTS; ++part) {
+                            ok = __all_sync(0xffffffffu, tc_wait(&bar[kKFull + slot], round & 1u, dead));
+                            if (!ok) break;
+                            tc_fence_after();
+                            const uint64_t at = kd + slot * (C::KOP_B >> 4);
+                            const uint32_t qat = tmem + C::Q_COL + D / 2 * part;
 #pragma unroll
-                        for (int k = 0; k < C::KE / 16; ++k)
-                            tc_mma(tmem + C::S_COL + 128 * b, tmem + C::Q_COL + 8 * k,
-                                   at + (k >> 2) * (kTcTile * 128 >> 4) + (k & 3) * 2, tc_idesc(kTcTile, false), k > 0);
-                        tc_commit(&bar[kKEmpty + b]);
-                        tc_commit(&bar[kSFull + b]);
+                            for (int k = 0; k < D / 16; ++k)
+                                tc_mma(tmem + C::S_COL + 128 * b, qat + 8 * k, at + (k >> 2) * (kTcTile * 128 >> 4) + (k & 3) * 2,
+                                       tc_idesc(kTcTile, false), part > 0 || k > 0, one);
+                            tc_commit(&bar[kKEmpty + slot], one);
+                            if (++slot == C::KST) {
+                                slot = 0;
+                                ++round;
+                            }
+                        }
+                        if (!ok) break;
+                        tc_commit(&bar[kSFull + b], one);
                     }
                     if (i > from) values(i - 1, i - 1 == from);
                 }
                 i = end;
             }
-            if (!ok) raise_device_error(a.err, BC_DEVERR_TIMEOUT);
-            tc_commit(&bar[kDrain]);
+            if (!ok && one) raise_device_error(a.err, BC_DEVERR_TIMEOUT);
+            tc_commit(&bar[kDrain], one);
 #pragma unroll 1
             for (uint32_t it = 0; it < kTcSpin; ++it)
                 if (mbar_try_wait(&bar[kDrain], 0)) break;
         }
-    } else {
+        __syncwarp();
+        // the tensor memory goes back once all warps are through with it (bounded, as every wait)
+#pragma unroll 1
+        for (uint32_t it = 0; it < kTcSpin; ++it)
+            if (mbar_try_wait(&bar[kDone], 0)) break;
+        __syncwarp();
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        return;
+    }
+    if (warp == 25 || warp == 26) {
         // ---------------- packed tiles of K (warp 25) or V (warp 26) ----------------
         if (lane == 0) {
             const bool is_v = warp == 26;
@@ -660,11 +755,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     if (mbar_try_wait(&full[t % kTcRaw], (uint32_t)(t / kTcRaw) & 1u)) break;
         }
     }
-    __syncwarp();
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    if (warp == 24) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    tc_leave(&bar[kDone]);
 }
 
 template <int D, bool COMP>

@@ -228,6 +228,22 @@ def test_non_finite_queries_and_cache_rows_stay_alone(cuda, n):
 
 
 @pytest.mark.parametrize("n", [4, 40])
+@pytest.mark.parametrize("where", [0, 70, 200])
+def test_infinite_scores(cuda, n, where):
+    """A key of the prefix whose scale is infinite: every score with it is +-inf, no wait is upset."""
+    b = Batch(cuda, [300] * n, [256], 1, 4, 128, True, 128, seed=16)
+    b.K.bscale[b.ids[0, 0, where // 128], where % 128] = float("inf")
+    got = b.run()
+    assert _lib.device_error() == 0
+    plus = ((b.q >= 0).float() * 2 - 1) @ (2 * ((b.K.sign[b.ids[0, 0, where // 128], where % 128][:, None]
+                                                 >> torch.arange(32, device=cuda)) & 1).flatten() - 1).float() > 0
+    assert got[plus].isnan().all()  # inf - inf
+    if where == 200:
+        b.K.bscale[b.ids[0, 0, 1], 72] = 1.0
+        b.check()
+
+
+@pytest.mark.parametrize("n", [4, 40])
 def test_infinite_values_past_a_short_sequence(cuda, n):
     """A row of the prefix that a sequence shorter than it must not see holds infinities."""
     lens = [100] + [300] * (n - 1)
