@@ -80,6 +80,8 @@ enum TcBar {
 // The issuing warp runs its loop with all lanes, and `one` picks the lane that
 // issues: the addresses then live in uniform registers, which the instruction
 // wants (from one lane's branch each product cost some 150 clocks to issue).
+// A value that all lanes hold, in a uniform register.
+__device__ __forceinline__ uint32_t tc_uniform(uint32_t x) { return __reduce_max_sync(0xffffffffu, x); }
 __device__ __forceinline__ uint32_t tc_elect() {
     uint32_t one;
     asm volatile(
@@ -300,7 +302,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
     volatile int* vbad = flags + 8;    // [8]
     volatile int* dead = flags + 16;
     volatile uint32_t* tmem_at = reinterpret_cast<volatile uint32_t*>(flags + 17);
-    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const int tid = threadIdx.x, warp = (int)tc_uniform(tid >> 5), lane = tid & 31;
 
     sh_wait_before();
     sh_let_next();
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_at, 0);
+    const uint32_t tmem = tc_uniform(*tmem_at);
 
     // registers: 256 x 112 + 512 x 56 + 128 x 48 of the 896 x 72 launched
     if (warp < 8) {
@@ -648,15 +650,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                 const uint32_t p = tmem + C::S_COL + 128 * (j & 1);
 #pragma unroll
                 for (int k = 0; k < kTcTile / 16; ++k)
-                    tc_mma(tmem + C::O_COL, p + 64 * (k / 4) + 8 * (k % 4), at + (2048 >> 4) * k, tc_idesc(D, true),
-                           !(first && k == 0), one);
+                    tc_mma(tmem + C::O_COL, p + 8 * k + 32 * (k >> 2), at + (2048 >> 4) * k, tc_idesc(D, true), !first || k > 0,
+                           one);
                 tc_commit(&bar[kVEmpty + j % C::VST], one);
                 tc_commit(&bar[kPvDone], one);
             };
             int i = 0, slot = 0;
             uint32_t round = 0;
-            for (int items = 0; ok && cur.left > 0; ++items, sh_next_piece(a, L, cur)) {
-                const int from = i, end = i + sh_piece_tiles(cur);
+            for (int items = 0; __all_sync(0xffffffffu, ok && cur.left > 0); ++items, sh_next_piece(a, L, cur)) {
+                const int from = i, end = i + (int)tc_uniform(sh_piece_tiles(cur));
                 ok = __all_sync(0xffffffffu, tc_wait(&bar[kQFull], (uint32_t)items & 1u, dead));
                 // the scores of a tile go before the values of the one before it; a piece's last values
                 // before the next one's scores, whose queries are there only then
@@ -673,8 +675,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                             const uint32_t qat = tmem + C::Q_COL + D / 2 * part;
 #pragma unroll
                             for (int k = 0; k < D / 16; ++k)
-                                tc_mma(tmem + C::S_COL + 128 * b, qat + 8 * k, at + (k >> 2) * (kTcTile * 128 >> 4) + (k & 3) * 2,
-                                       tc_idesc(kTcTile, false), part > 0 || k > 0, one);
+                                tc_mma(tmem + C::S_COL + 128 * b, qat + 8 * k, at + 2 * k + (k >> 2) * ((kTcTile * 128 >> 4) - 8),
+                                       tc_idesc(kTcTile, false), part + k > 0, one);
                             tc_commit(&bar[kKEmpty + slot], one);
                             if (++slot == C::KST) {
                                 slot = 0;

@@ -244,6 +244,19 @@ def test_infinite_scores(cuda, n, where):
 
 
 @pytest.mark.parametrize("n", [4, 40])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), 60000.0])
+def test_wild_scales_end_in_time(cuda, n, value):
+    """Scales of every kind in every key: results may be anything, but no wait gives up."""
+    b = Batch(cuda, [1300] * n, [1200], 1, 4, 128, True, 128, seed=17)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    for P in (b.K, b.V):
+        for x in (P.bscale, P.rscale):
+            x[torch.rand(x.shape, generator=g, device=cuda) < 0.5] = value
+    b.run()
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("n", [4, 40])
 def test_infinite_values_past_a_short_sequence(cuda, n):
     """A row of the prefix that a sequence shorter than it must not see holds infinities."""
     lens = [100] + [300] * (n - 1)
