@@ -43,7 +43,7 @@ constexpr int kTcThreads = 28 * 32;
 constexpr int kTcUnpackWarps = 8;   // of K, and of V
 constexpr int kTcRaw = 3;        // packed tiles ahead
 constexpr int kTcItemCost = 2;   // an item's start and end, in tiles
-constexpr uint32_t kTcSpin = 1u << 19;  // polls of a wait before it gives up: about a second
+constexpr uint64_t kTcPatience = 1000000000;  // ns before a wait gives up
 
 template <int D, bool COMP>
 struct TcCfg {
@@ -158,16 +158,44 @@ __host__ __device__ constexpr uint32_t tc_idesc(int n, bool b_mn) {
 }
 
 // ---- waits -----------------------------------------------------------------
-// Bounded; once one has given up (dead), all do, and the CTA winds down.
+// Bounded in time; once one has given up (dead), all do, and the CTA winds down.
+// The hint lets a waiting warp sleep until the phase ends: without it the polls of
+// a dozen waiting warps were a third of all instructions.
+__device__ __forceinline__ bool tc_try_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ uint64_t tc_now() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
 __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile int* dead) {
-    if (mbar_try_wait(bar, parity)) return true;
+    if (tc_try_wait(bar, parity)) return true;
+    const uint64_t limit = tc_now() + kTcPatience;
 #pragma unroll 1
-    for (uint32_t it = 0; it < kTcSpin; ++it) {
-        if (mbar_try_wait(bar, parity)) return true;
+    while (!tc_try_wait(bar, parity)) {
         if (*dead) return false;
+        if (tc_now() > limit) {
+            *dead = 1;
+            return false;
+        }
     }
-    *dead = 1;
-    return false;
+    return true;
+}
+// The last waits of a warp, for what it has set off itself.
+__device__ __forceinline__ void tc_settle(uint64_t* bar, uint32_t parity) {
+    const uint64_t limit = tc_now() + kTcPatience;
+#pragma unroll 1
+    while (!tc_try_wait(bar, parity) && tc_now() < limit) {
+    }
 }
 __device__ __forceinline__ void tc_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -362,6 +390,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
         bool ok = true;
         for (int i = 0; ok && cur.left > 0; sh_next_piece(a, L, cur)) {
             const int end = i + sh_piece_tiles(cur);
+            const bool single = end - i == 1;
             const __half* src = rl < L.rows ? sh_query(a, L, cur, cur.blk * L.rows + rl, D) : nullptr;
             const bool valid = src != nullptr, busy = __any_sync(0xffffffffu, valid);
             if (busy) sc = tc_query<D, COMP>(src, a.q_aligned, half, lane_at + C::Q_COL);
@@ -452,6 +481,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                             }
                         }
                     }
+                    tc_wait_st();  // the first P is down before the second goes over it
                     seen = true;
                     again = false;
                 }
@@ -474,7 +504,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     l += xch[256 * (met & 1) + 128 * (half ^ 1)];
                     ++met;
                 }
-                ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead));
+                // the last two products one after the other: the barrier tells odd phases from even ones, no more
+                ok = __all_sync(0xffffffffu, (single || tc_wait(&bar[kPvDone], (uint32_t)i & 1u, dead)) &&
+                                                 tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead));
                 if (!ok) break;
                 tc_fence_after();
                 if (busy) {
@@ -692,15 +724,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             }
             if (!ok && one) raise_device_error(a.err, BC_DEVERR_TIMEOUT);
             tc_commit(&bar[kDrain], one);
-#pragma unroll 1
-            for (uint32_t it = 0; it < kTcSpin; ++it)
-                if (mbar_try_wait(&bar[kDrain], 0)) break;
+            tc_settle(&bar[kDrain], 0);
         }
         __syncwarp();
         // the tensor memory goes back once all warps are through with it (bounded, as every wait)
-#pragma unroll 1
-        for (uint32_t it = 0; it < kTcSpin; ++it)
-            if (mbar_try_wait(&bar[kDone], 0)) break;
+            tc_settle(&bar[kDone], 0);
         __syncwarp();
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -752,9 +780,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             }
             // copies in flight land before the block's memory is given back (bounded)
             for (int t = max(0, i - kTcRaw); t < i; ++t)
-#pragma unroll 1
-                for (uint32_t it = 0; it < kTcSpin; ++it)
-                    if (mbar_try_wait(&full[t % kTcRaw], (uint32_t)(t / kTcRaw) & 1u)) break;
+            tc_settle(&full[t % kTcRaw], (uint32_t)(t / kTcRaw) & 1u);
         }
     }
     tc_leave(&bar[kDone]);

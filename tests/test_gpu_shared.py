@@ -197,6 +197,23 @@ def test_scores_that_rise_and_scales_that_differ(cuda, n):
     b.check()
 
 
+@pytest.mark.parametrize("n,d,comp", [(6, 128, True), (12, 128, False), (40, 64, True), (9, 64, False), (3, 128, True)])
+def test_long_pieces_whose_maximum_keeps_rising(cuda, n, d, comp):
+    """Enough keys that a CTA has several tiles of one prefix, with scores that rise all along it."""
+    b = Batch(cuda, [50100 + 3 * i for i in range(n)], [50000], 3, 4, d, comp, 256, seed=18)
+    b.check()
+    for h in range(3):
+        at = b.ids[0, h, :196].to(cuda)
+        ramp = (torch.arange(196 * 256, device=cuda).view(196, 256) / 50000) ** 2 * (3 + 3 * h) + 0.02
+        for i in range(n):  # the begun page of the prefix is copied
+            b.K.bscale[b.ids[i, h, 195], :80] = b.K.bscale[b.ids[0, h, 195], :80]
+        b.K.bscale[at[:195]] = (b.K.bscale[at[:195]].float() * ramp[:195]).half()
+        if comp:
+            b.K.rscale[at[:195]] = (b.K.rscale[at[:195]].float() * ramp[:195]).half()
+    b.check()
+    assert _lib.device_error() == 0
+
+
 def test_long_flat_context_keeps_its_tail(cuda):
     """40000 keys of tiny weight beside one of weight 1: the small ones still add up."""
     for n in (1, 40):
