@@ -617,32 +617,21 @@ __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a,
                     has = sh_tile_at(L, sh_begin(total[i], n_workers, c) - first, x[i].tiles) <
                           sh_tile_at(L, sh_begin(total[i], n_workers, c + 1) - first, x[i].tiles);
                 const float2 ul = has ? __ldcg(reinterpret_cast<const float2*>(rec + c * size + D)) : make_float2(kShNone, 0.0f);
-                float top = ul.x;
-#pragma unroll
-                for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                const float U = fmaxf(M, top), f = exp2f(M - U);
-                const float w = has ? exp2f(ul.x - U) : 0.0f;
-                float l = ul.y * w;
-#pragma unroll
-                for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
-                M = U;
-                sum = sum * f + l;
-#pragma unroll
-                for (int k = 0; k < VEC; ++k) o[k] *= f;
                 unsigned todo = __ballot_sync(0xffffffffu, has);
+                bool scaled = false;
+                float w = 0.0f;
                 while (todo) {
-                    constexpr int AT_ONCE = 8;  // records in flight: an L2 round trip each
-                    float v[AT_ONCE][VEC], wt[AT_ONCE];
+                    constexpr int AT_ONCE = VEC >= 8 ? 8 : 16;  // records in flight: an L2 round trip together
+                    float v[AT_ONCE][VEC];
+                    int src[AT_ONCE];
 #pragma unroll
                     for (int u = 0; u < AT_ONCE; ++u) {
-                        const int src = todo ? __ffs(todo) - 1 : 0;
-                        const bool on = todo != 0;
+                        src[u] = todo ? __ffs(todo) - 1 : -1;
                         todo &= todo - 1;
-                        wt[u] = __shfl_sync(0xffffffffu, w, src);
-                        const float* from = rec + (base + src) * size + VEC * lane;
+                        const float* from = rec + (base + src[u]) * size + VEC * lane;
 #pragma unroll
                         for (int k = 0; k < VEC; ++k) v[u][k] = 0.0f;
-                        if (on) {
+                        if (src[u] >= 0) {
                             if constexpr (VEC >= 4) {
 #pragma unroll
                                 for (int k = 0; k < VEC; k += 4)
@@ -651,14 +640,31 @@ __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a,
 #pragma unroll
                                 for (int k = 0; k < VEC; ++k) v[u][k] = __ldcg(from + k);
                             }
-                        } else {
-                            wt[u] = 0.0f;
                         }
                     }
+                    if (!scaled) {  // with the records on their way
+                        float top = ul.x;
 #pragma unroll
-                    for (int u = 0; u < AT_ONCE; ++u)
+                        for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+                        const float U = fmaxf(M, top), f = exp2f(M - U);
+                        w = has ? exp2f(ul.x - U) : 0.0f;
+                        float l = ul.y * w;
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) o[k] += v[u][k] * wt[u];
+                        for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+                        M = U;
+                        sum = sum * f + l;
+#pragma unroll
+                        for (int k = 0; k < VEC; ++k) o[k] *= f;
+                        scaled = true;
+                    }
+#pragma unroll
+                    for (int u = 0; u < AT_ONCE; ++u) {
+                        const float wt = __shfl_sync(0xffffffffu, w, src[u] & 31);
+                        if (src[u] >= 0) {
+#pragma unroll
+                            for (int k = 0; k < VEC; ++k) o[k] += v[u][k] * wt;
+                        }
+                    }
                 }
             }
         }
@@ -692,9 +698,9 @@ int sh_workers_on_device(int* n_workers) {
 
 // The prefix kernel takes the prefixes when `tc` is given, else the rows kernel has both.
 template <int D, bool COMP>
-int sh_run(const SharedArgs& a, ShList& L, const ShList* tc, cudaStream_t st) {
+int sh_run(const SharedArgs& a, ShList& L, const ShList* tc, void* scratch, cudaStream_t st) {
     int rc = sh_workers_on_device<D, COMP>(&L.n_workers);
-    if (!rc && tc) rc = sh_tc_run(a, *tc, D, COMP, st);
+    if (!rc && tc) rc = sh_tc_run(a, *tc, scratch, D, COMP, st);
     if (rc) return rc;
     cudaError_t e = sh_launch(k_shared_rows<D, COMP>, (L.n_workers + kShWarps - 1) / kShWarps + (tc ? 1 : 0), kShThreads,
                               ShCfg<D, COMP>::SMEM_B, st, a, L, tc != nullptr);
@@ -740,7 +746,9 @@ size_t bc_decode_shared_workspace_bytes(int n_seqs, int n_groups, int n_kv_heads
         return 0;
     const bool tc = sh_takes_tc(n_seqs, n_groups, group, head_dim);
     return sh_bytes(sh_list(n_seqs, n_groups, group, !tc), n_kv_heads, kShMaxWorkers, head_dim) +
-           (tc ? sh_bytes(sh_tc_list(n_seqs, n_groups, group), n_kv_heads, kShTcWorkers, head_dim) : 0);
+           (tc ? sh_bytes(sh_tc_list(n_seqs, n_groups, group), n_kv_heads, kShTcWorkers, head_dim) +
+                     sh_tc_scratch((int64_t)n_seqs * n_kv_heads * group, head_dim)
+               : 0);
 }
 
 int bc_decode_attention_shared(const void* q, bc_kv_planes K, bc_kv_planes V, bc_page_table pt,
@@ -788,17 +796,19 @@ int bc_decode_attention_shared(const void* q, bc_kv_planes K, bc_kv_planes V, bc
     const bool tc = sh_takes_tc(n_seqs, n_groups, group, head_dim) && prefix_lens;
     ShList L = sh_list(n_seqs, n_groups, group, !tc), T = sh_tc_list(n_seqs, n_groups, group);
     L.records = (float*)workspace;
+    void* scratch = nullptr;
     if (tc) {
         T.n_workers = kShTcWorkers;
         T.records = (float*)((char*)workspace + sh_bytes(L, n_kv_heads, kShMaxWorkers, head_dim));
+        scratch = (char*)T.records + sh_bytes(T, n_kv_heads, kShTcWorkers, head_dim);
     }
     cudaStream_t st = (cudaStream_t)stream;
     const ShList* t = tc ? &T : nullptr;
     switch (head_dim) {
-        case 32: return comp ? sh_run<32, true>(a, L, t, st) : sh_run<32, false>(a, L, t, st);
-        case 64: return comp ? sh_run<64, true>(a, L, t, st) : sh_run<64, false>(a, L, t, st);
-        case 128: return comp ? sh_run<128, true>(a, L, t, st) : sh_run<128, false>(a, L, t, st);
-        default: return comp ? sh_run<256, true>(a, L, t, st) : sh_run<256, false>(a, L, t, st);
+        case 32: return comp ? sh_run<32, true>(a, L, t, scratch, st) : sh_run<32, false>(a, L, t, scratch, st);
+        case 64: return comp ? sh_run<64, true>(a, L, t, scratch, st) : sh_run<64, false>(a, L, t, scratch, st);
+        case 128: return comp ? sh_run<128, true>(a, L, t, scratch, st) : sh_run<128, false>(a, L, t, scratch, st);
+        default: return comp ? sh_run<256, true>(a, L, t, scratch, st) : sh_run<256, false>(a, L, t, scratch, st);
     }
 }
 

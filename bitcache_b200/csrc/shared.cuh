@@ -123,9 +123,13 @@ static_assert(kShThreads == 128, "sh_scan: four sums per lane");
 // tiles.  A piece's record is number item + worker: along the list every new
 // piece raises one of the two.
 __device__ __forceinline__ int sh_workers(const ShList& L, int64_t total) { return (int)min((int64_t)L.n_workers, total); }
-__device__ __forceinline__ int64_t sh_begin(int64_t total, int n, int64_t w) { return total * w / n; }
+// (Quotients in double precision: the products are below 2^53, and a quotient that
+// is no whole number is further from one than the rounding of the division.)
+__device__ __forceinline__ int64_t sh_begin(int64_t total, int n, int64_t w) {
+    return (int64_t)((double)(total * w) / (double)n);
+}
 __device__ __forceinline__ int sh_worker_of(int64_t total, int n, int64_t at) {
-    return (int)(((at + 1) * n + total - 1) / total) - 1;
+    return (int)((double)((at + 1) * n + total - 1) / (double)total) - 1;
 }
 __device__ __forceinline__ int sh_tile_at(const ShList& L, int64_t at_in_item, int tiles) {
     return (int)max((int64_t)0, min((int64_t)tiles, at_in_item - L.cost));

@@ -191,10 +191,14 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, volatile
     return true;
 }
 // The last waits of a warp, for what it has set off itself.
-__device__ __forceinline__ void tc_settle(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ void tc_settle(uint64_t* bar, uint32_t parity, volatile int* dead) {
     const uint64_t limit = tc_now() + kTcPatience;
 #pragma unroll 1
-    while (!tc_try_wait(bar, parity) && tc_now() < limit) {
+    while (!tc_try_wait(bar, parity)) {
+        if (tc_now() > limit) {
+            *dead = 1;
+            return;
+        }
     }
 }
 __device__ __forceinline__ void tc_arrive(uint64_t* bar) {
@@ -238,87 +242,46 @@ __device__ __forceinline__ float2 tc_add2(float2 x, float2 y) {
     return *reinterpret_cast<float2*>(&r);
 }
 
-// Dims 32 w .. 32 w + 31 of a query row as fp16 pairs (zeros without a row).
-__device__ __forceinline__ void tc_row_word(const __half* src, bool aligned, int w, uint32_t (&x)[16]) {
-    if (!src) {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) x[k] = 0;
-    } else if (aligned) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const uint4 v = reinterpret_cast<const uint4*>(src)[4 * w + k];
-            x[4 * k] = v.x;
-            x[4 * k + 1] = v.y;
-            x[4 * k + 2] = v.z;
-            x[4 * k + 3] = v.w;
-        }
-    } else {
-        const uint16_t* s16 = reinterpret_cast<const uint16_t*>(src) + 32 * w;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) x[k] = s16[2 * k] | ((uint32_t)s16[2 * k + 1] << 16);
-    }
-}
-__device__ __forceinline__ void tc_st4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
-                 : "memory");
-}
-
-// A thread's query row into tensor memory (part 0: h sgn q, part 1: 8/7 q / f, in
-// the order of K's elements); returns the scale of its scores in log2 units.
+// The query rows as A operands, one warp a row: [h sgn q | 8/7 q / f] in the order
+// of K's elements, and the scale of the row's scores in log2 units.  A kernel of
+// its own: a softmax thread that made its row itself ran some 800 instructions
+// once, at the pace of their fetch (12000 clocks a piece).
+constexpr int kTcQueryWarps = 8;
 template <int D, bool COMP>
-__device__ __forceinline__ float tc_query(const __half* src, bool aligned, int part, uint32_t at) {
-    constexpr int NW = D / 32;
-    uint32_t x[16];
+__global__ void __launch_bounds__(32 * kTcQueryWarps) k_shared_queries(const __half* __restrict__ q,
+                                                                       uint32_t* __restrict__ ops,
+                                                                       float* __restrict__ scales, int64_t rows) {
+    constexpr int WORDS = (COMP ? 2 : 1) * D / 2;
+    sh_wait_before();
+    sh_let_next();
+    const int64_t row = (int64_t)blockIdx.x * kTcQueryWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= rows) return;
+    const __half* x = q + row * D;
     float mag = 0.0f;
-#pragma unroll 1
-    for (int w = 0; w < NW; ++w) {
-        tc_row_word(src, aligned, w, x);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const float2 f = __half22float2(bits_h2(x[k]));
-            mag += fabsf(f.x) + fabsf(f.y);
-        }
-    }
+    for (int k = 0; k < D / 32; ++k) mag += fabsf(__half2float(x[32 * k + lane]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mag += __shfl_xor_sync(0xffffffffu, mag, o);
     const float mean = mag * (1.0f / D);
     const __half h = __float2half_rn(mean);
-    const float hf = __half2float(h);
-    const float f = hf == 0.0f ? 1.0f : mean / hf;
-    auto dim = [&](int d) { return d % 2 ? __high2float(bits_h2(x[d / 2])) : __low2float(bits_h2(x[d / 2])); };
-    if (part == 0) {
-        const uint32_t hb = __half_as_ushort(h);
-#pragma unroll 1
-        for (int w = 0; w < NW; ++w) {
-            tc_row_word(src, aligned, w, x);
-            uint32_t r[16];  // pairs (i, i + 16) of the word
+    const float hf = __half2float(h), f = hf == 0.0f ? 1.0f : mean / hf, g = (8.0f / 7.0f) / f;
+    if (lane == 0) scales[row] = f * kShLog2e * rsqrtf((float)D);
+    const uint32_t hb = __half_as_ushort(h);
 #pragma unroll
-            for (int p = 0; p < 16; ++p)
-                r[p] = (hb | (dim(p) >= 0.0f ? 0u : 0x8000u)) | ((hb | (dim(p + 16) >= 0.0f ? 0u : 0x8000u)) << 16);
-            tc_st16(at + 16 * w, r);
-        }
-    } else if constexpr (COMP) {
-        const float g = (8.0f / 7.0f) / f;
-#pragma unroll 1
-        for (int w = 0; w < NW; ++w) {
-            tc_row_word(src, aligned, w, x);
-            // the code words made of these dims: word w of every chunk (head_dim 128), words w and w + 2 (64)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const int first = D == 128 ? u : 2 * (u / 2) + u % 2;  // bit of the byte that nibble 0 holds
-                const int unit = D == 128 ? 4 * u + w : 4 * (u / 2) + w + 2 * (u % 2);
-                uint32_t r[4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t)  // nibbles t, t + 4: dims 4 t + first, 4 t + 16 + first of the word
-                    r[t] = h2_bits(__floats2half2_rn(dim(4 * t + first) * g, dim(4 * t + 16 + first) * g));
-                tc_st4(at + D / 2 + 4 * unit, r[0], r[1], r[2], r[3]);
-            }
-        }
+    for (int k = 0; k < D / 64; ++k) {
+        const int c = 32 * k + lane, d0 = 32 * (c / 16) + c % 16;
+        ops[row * WORDS + c] = (hb | (__half2float(x[d0]) >= 0.0f ? 0u : 0x8000u)) |
+                               ((hb | (__half2float(x[d0 + 16]) >= 0.0f ? 0u : 0x8000u)) << 16);
+        if constexpr (COMP)
+            ops[row * WORDS + D / 2 + c] = h2_bits(__floats2half2_rn(__half2float(x[sh_code_dim(D, 2 * c)]) * g,
+                                                                     __half2float(x[sh_code_dim(D, 2 * c + 1)]) * g));
     }
-    tc_wait_st();
-    return f * kShLog2e * rsqrtf((float)D);
 }
 
 template <int D, bool COMP>
-__global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArgs a, const ShList L) {
+__global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArgs a, const ShList L, const uint32_t* __restrict__ ops,
+                                                                    const float* __restrict__ scales) {
     using C = TcCfg<D, COMP>;
     constexpr int NW = D / 32;
     extern __shared__ uint8_t tc_raw[];
@@ -332,7 +295,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
     volatile uint32_t* tmem_at = reinterpret_cast<volatile uint32_t*>(flags + 17);
     const int tid = threadIdx.x, warp = (int)tc_uniform(tid >> 5), lane = tid & 31;
 
-    sh_wait_before();
+    // the queries' kernel has waited for all that came before; only its own results are waited for below
     sh_let_next();
     const int64_t total = sh_scan(a, L, scan);
     const int n_workers = sh_workers(L, total);
@@ -387,13 +350,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
         uint64_t* pair = &bar[kPair + quad];
         uint32_t met = 0;  // exchanges with the row's other warp
         float sc = 0.0f, U = kShNone, l = 0.0f;
+        sh_wait_before();
         bool ok = true;
         for (int i = 0; ok && cur.left > 0; sh_next_piece(a, L, cur)) {
             const int end = i + sh_piece_tiles(cur);
-            const bool single = end - i == 1;
             const __half* src = rl < L.rows ? sh_query(a, L, cur, cur.blk * L.rows + rl, D) : nullptr;
             const bool valid = src != nullptr, busy = __any_sync(0xffffffffu, valid);
-            if (busy) sc = tc_query<D, COMP>(src, a.q_aligned, half, lane_at + C::Q_COL);
+            if (busy && half < C::PARTS) {
+                const uint32_t* op = ops + (valid ? (src - a.q) / D : 0) * (C::KE / 2) + D / 2 * half;
+                uint32_t x[D / 2];
+#pragma unroll
+                for (int k = 0; k < D / 2; k += 4) {
+                    const uint4 w = valid ? __ldcg(reinterpret_cast<const uint4*>(op + k)) : make_uint4(0, 0, 0, 0);
+                    x[k] = w.x;
+                    x[k + 1] = w.y;
+                    x[k + 2] = w.z;
+                    x[k + 3] = w.w;
+                }
+#pragma unroll
+                for (int k = 0; k < D / 2; k += 16)
+                    tc_st16(lane_at + C::Q_COL + D / 2 * half + k, *reinterpret_cast<uint32_t(*)[16]>(x + k));
+                tc_wait_st();
+            }
+            sc = valid ? __ldcg(scales + (src - a.q) / D) : 1.0f;
             tc_fence_before();
             __syncwarp();
             if (lane == 0) tc_arrive(&bar[kQFull]);
@@ -456,7 +435,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     }
                     tile_sum = sum.x + sum.y;
                     if (seen) break;
-                    ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead));
+                    // the products up to the tile before are through as well: O may be scaled, and every phase of
+                    // that barrier is seen by each warp that reads it (it tells odd phases from even ones, no more)
+                    ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead) &&
+                                                     (begin || tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead)));
                     if (!ok) break;
                     top = fmaxf(top, xch[256 * (met & 1) + 128 * (half ^ 1)]) * sc;
                     const bool rise = __any_sync(0xffffffffu, top - U > 15.0f);
@@ -465,9 +447,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                         const float U1 = top - U > 15.0f ? top - 8.0f : U, f = exp2f(U - U1);
                         U = U1;
                         l *= f;
-                        if (!begin) {  // O holds the piece's tiles so far, once their products are through
-                            ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead));
-                            if (!ok) break;
+                        if (!begin) {  // O holds the piece's tiles so far
                             tc_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < D / 32; ++c) {
@@ -504,9 +484,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     l += xch[256 * (met & 1) + 128 * (half ^ 1)];
                     ++met;
                 }
-                // the last two products one after the other: the barrier tells odd phases from even ones, no more
-                ok = __all_sync(0xffffffffu, (single || tc_wait(&bar[kPvDone], (uint32_t)i & 1u, dead)) &&
-                                                 tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead));
+                ok = __all_sync(0xffffffffu, !busy || tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead));
                 if (!ok) break;
                 tc_fence_after();
                 if (busy) {
@@ -722,14 +700,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                 }
                 i = end;
             }
-            if (!ok && one) raise_device_error(a.err, BC_DEVERR_TIMEOUT);
             tc_commit(&bar[kDrain], one);
-            tc_settle(&bar[kDrain], 0);
+            tc_settle(&bar[kDrain], 0, dead);
         }
         __syncwarp();
         // the tensor memory goes back once all warps are through with it (bounded, as every wait)
-            tc_settle(&bar[kDone], 0);
+        tc_settle(&bar[kDone], 0, dead);
         __syncwarp();
+        if (*dead && lane == 0) raise_device_error(a.err, BC_DEVERR_TIMEOUT);
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
         return;
@@ -780,14 +758,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             }
             // copies in flight land before the block's memory is given back (bounded)
             for (int t = max(0, i - kTcRaw); t < i; ++t)
-            tc_settle(&full[t % kTcRaw], (uint32_t)(t / kTcRaw) & 1u);
+            tc_settle(&full[t % kTcRaw], (uint32_t)(t / kTcRaw) & 1u, dead);
         }
     }
     tc_leave(&bar[kDone]);
 }
 
 template <int D, bool COMP>
-int tc_run(const SharedArgs& a, const ShList& L, cudaStream_t st) {
+int tc_run(const SharedArgs& a, const ShList& L, void* scratch, cudaStream_t st) {
     constexpr int smem = TcCfg<D, COMP>::SMEM_B;
     static_assert(smem <= 232448, "shared memory of one CTA");
     static bool ready[64] = {};
@@ -800,7 +778,14 @@ int tc_run(const SharedArgs& a, const ShList& L, cudaStream_t st) {
         if (e != cudaSuccess) return BC_ERR_CUDA_BASE + (int)e;
         ready[dev] = true;
     }
-    e = sh_launch(k_shared_prefix<D, COMP>, L.n_workers, kTcThreads, smem, st, a, L);
+    const int64_t rows = (int64_t)a.n_seqs * a.n_kv * a.group;
+    uint32_t* ops = (uint32_t*)scratch;
+    float* scales = (float*)(ops + rows * (TcCfg<D, COMP>::KE / 2));
+    e = sh_launch(k_shared_queries<D, COMP>, (int)((rows + kTcQueryWarps - 1) / kTcQueryWarps), 32 * kTcQueryWarps, 0, st,
+                  a.q, ops, scales, rows);
+    if (e == cudaSuccess)
+        e = sh_launch(k_shared_prefix<D, COMP>, L.n_workers, kTcThreads, smem, st, a, L, (const uint32_t*)ops,
+                      (const float*)scales);
     return e == cudaSuccess ? BC_OK : BC_ERR_CUDA_BASE + (int)e;
 }
 
@@ -819,9 +804,11 @@ ShList sh_tc_list(int n_seqs, int n_groups, int group) {
     return L;
 }
 
-int sh_tc_run(const SharedArgs& a, const ShList& L, int head_dim, bool compensated, cudaStream_t st) {
-    if (head_dim == 128) return compensated ? tc_run<128, true>(a, L, st) : tc_run<128, false>(a, L, st);
-    return compensated ? tc_run<64, true>(a, L, st) : tc_run<64, false>(a, L, st);
+size_t sh_tc_scratch(int64_t rows, int head_dim) { return (size_t)rows * (4 * head_dim + 16); }
+
+int sh_tc_run(const SharedArgs& a, const ShList& L, void* scratch, int head_dim, bool compensated, cudaStream_t st) {
+    if (head_dim == 128) return compensated ? tc_run<128, true>(a, L, scratch, st) : tc_run<128, false>(a, L, scratch, st);
+    return compensated ? tc_run<64, true>(a, L, scratch, st) : tc_run<64, false>(a, L, scratch, st);
 }
 
 }  // namespace bc
