@@ -173,8 +173,405 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope_rows(const RopeArgs a)
     }
 }
 
+// ---------------------------------------------------------------------------
+// head_dim 64, 128, 256 on 16-byte boundaries: head_dim / 16 lanes a row, lane r
+// with elements 8r .. 8r + 7 ("slot 0") and head_dim / 2 + 8r .. ("slot 1"), so a
+// row is two 16-byte loads per lane, rotation pairs head_dim / 2 apart are a
+// lane's own, and a sign byte and its nibble bytes are too.  A warp takes several
+// heads of one token at a time (4 at 128), with the token's cosines and sines in
+// registers.  HBM-bound in intent: the tree sums cost 10 shuffles for 4 rows here,
+// 20 in the kernel above, whose 2-byte loads also keep too little in flight.
+// ---------------------------------------------------------------------------
+template <int D>
+struct Lanes {
+    static constexpr int LPR = D / 16;   // lanes of a row
+    static constexpr int ROWS = 32 / LPR;  // rows of a warp
+};
+
+// The encoders' tree: leaf t holds v_t, strides 128, 64, ..., 1.  p[j] is the sum
+// over both slots already (the first stride).  Lanes halve the eight positions
+// they are responsible for at each stride, then the positions meet.
+template <int D>
+__device__ __forceinline__ float group_tree(float (&p)[8], int lane) {
+    constexpr int LPR = Lanes<D>::LPR;
+    int n = 8;
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) {
+        if (n > 1) {
+            const bool up = lane & o;
+            n >>= 1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j < n) {
+                    const float give = up ? p[j] : p[j + n], keep = up ? p[j + n] : p[j];
+                    p[j] = __fadd_rn(keep, __shfl_xor_sync(0xffffffffu, give, o));
+                }
+        } else {
+            p[0] = __fadd_rn(p[0], __shfl_xor_sync(0xffffffffu, p[0], o));
+        }
+    }
+    if constexpr (LPR == 4) {  // lanes 2, 1 hold position bits 2, 1; bit 0 is local
+#pragma unroll
+        for (int o = 2; o > 0; o >>= 1)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) p[j] = __fadd_rn(p[j], __shfl_xor_sync(0xffffffffu, p[j], o));
+        return __fadd_rn(p[0], p[1]);
+    } else {
+#pragma unroll
+        for (int o = LPR / 2; o > LPR / 16; o >>= 1) p[0] = __fadd_rn(p[0], __shfl_xor_sync(0xffffffffu, p[0], o));
+        return p[0];
+    }
+}
+
+// Eight elements of 16 (or 32) contiguous bytes.
+__device__ __forceinline__ void load8(const __half* p, float (&x)[8]) {
+    const uint4 v = ldg_nc_v4(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
+    const uint4 v = ldg_nc_v4(p);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+    const uint4 v = ldg_nc_v4(p), w = ldg_nc_v4(p + 4);
+    x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
+    x[4] = __uint_as_float(w.x), x[5] = __uint_as_float(w.y), x[6] = __uint_as_float(w.z), x[7] = __uint_as_float(w.w);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename O>
+__device__ __forceinline__ void store8(O* p, const float (&x)[8]) {
+    if constexpr (sizeof(O) == 4) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        *reinterpret_cast<uint4*>(p) = make_uint4(pack2(x[0], x[1], O{}), pack2(x[2], x[3], O{}), pack2(x[4], x[5], O{}),
+                                                  pack2(x[6], x[7], O{}));
+    }
+}
+__device__ __forceinline__ void load8f(const float* p, float (&x)[8]) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+
+// 4 x 4 bytes transposed over lanes a = 0 .. 3: lane a gets byte a of each lane's word.
+__device__ __forceinline__ uint32_t transpose4(uint32_t x, int a) {
+    const uint32_t y = __shfl_xor_sync(0xffffffffu, x, 1);
+    const uint32_t u = a & 1 ? __byte_perm(x, y, 0x3715) : __byte_perm(x, y, 0x6240);
+    const uint32_t z = __shfl_xor_sync(0xffffffffu, u, 2);
+    return a & 2 ? __byte_perm(u, z, 0x3276) : __byte_perm(u, z, 0x5410);
+}
+
+enum { kPairsNone = 0, kPairsHalf = 1, kPairsApart = 2, kPairsNext = 3 };  // head_dim / 2 apart, rotary_dim / 2 apart, adjacent
+
+template <int D, typename T, typename O, bool APPEND>
+__global__ void __launch_bounds__(kRopeWarps * 32) k_rope_lanes(const RopeArgs a, int style, int per, int res) {
+    constexpr int LPR = Lanes<D>::LPR, ROWS = Lanes<D>::ROWS;
+    const int lane = threadIdx.x & 31, r = lane % LPR, sub = lane / LPR;
+    const int heads = a.n_heads + (APPEND ? 2 : 1) * a.n_kv_heads;
+    const int groups = (heads + ROWS - 1) / ROWS, runs = (groups + per - 1) / per;
+    const int64_t job = (int64_t)blockIdx.x * kRopeWarps + (threadIdx.x >> 5);
+    if (job >= a.n_tokens * runs) return;
+    const int64_t t = job / runs;
+    const int g0 = (int)(job - t * runs) * per, g1 = min(groups, g0 + per);
+    int pos = a.positions[t];
+    bool bad = a.rope.cos && pos >= a.rope.n_positions;
+    int seq = 0;
+    if constexpr (APPEND) {
+        seq = a.seq_ids[t];
+        bad = bad || (pos >= 0 && (seq < 0 || seq >= a.n_seqs || pos >= (int64_t)a.pt.max_pages * a.pt.page_size));
+    }
+    if (bad) {
+        if (lane == 0) raise_device_error(a.err, BC_DEVERR_INDEX);
+        pos = -1;
+    }
+    const int half = a.rope.rotary_dim / 2;
+    int page = 0, in_page = 0;
+    float c[2][8], s[2][8];  // slot by slot; kPairsHalf has the first only, kPairsNext four pairs a slot
+    if (pos >= 0) {
+        const float *cp = a.rope.cos + (int64_t)pos * half, *sp = a.rope.sin + (int64_t)pos * half;
+        if (style == kPairsHalf) {
+            load8f(cp + 8 * r, c[0]);
+            load8f(sp + 8 * r, s[0]);
+        } else if (style != kPairsNone) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int i = D / 2 * x + 8 * r;
+                if (i >= 2 * half) continue;
+                if (style == kPairsApart) {
+                    load8f(cp + (i < half ? i : i - half), c[x]);
+                    load8f(sp + (i < half ? i : i - half), s[x]);
+                } else {
+                    const float4 u = __ldg(reinterpret_cast<const float4*>(cp + i / 2)), v = __ldg(reinterpret_cast<const float4*>(sp + i / 2));
+                    c[x][0] = u.x, c[x][1] = u.y, c[x][2] = u.z, c[x][3] = u.w;
+                    s[x][0] = v.x, s[x][1] = v.y, s[x][2] = v.z, s[x][3] = v.w;
+                }
+            }
+        }
+        if constexpr (APPEND) {
+            page = pos / a.pt.page_size;
+            in_page = pos - page * a.pt.page_size;
+        }
+    }
+    auto source = [&](int g, int& kind, int& h) -> const T* {
+        h = g * ROWS + sub;
+        if (h >= heads) return nullptr;
+        kind = h < a.n_heads ? 0 : h < a.n_heads + a.n_kv_heads ? 1 : 2;
+        h -= kind == 0 ? 0 : kind == 1 ? a.n_heads : a.n_heads + a.n_kv_heads;
+        const bc_heads& in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+        return reinterpret_cast<const T*>(in.data) + t * in.token_stride + (int64_t)h * in.head_stride + 8 * r;
+    };
+    float next[2][8];
+    int next_kind = 0, next_h = 0;
+    const T* src = source(g0, next_kind, next_h);
+    if (src && pos >= 0) {
+        load8(src, next[0]);
+        load8(src + D / 2, next[1]);
+    }
+    for (int g = g0; g < g1; ++g) {
+        float x[2][8];
+        const bool live = src != nullptr;
+        const int kind = next_kind, h = next_h;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[0][j] = live && pos >= 0 ? next[0][j] : 0.0f;
+            x[1][j] = live && pos >= 0 ? next[1][j] : 0.0f;
+        }
+        if (g + 1 < g1) {  // the next rows are on their way while these are worked on
+            src = source(g + 1, next_kind, next_h);
+            if (src && pos >= 0) {
+                load8(src, next[0]);
+                load8(src + D / 2, next[1]);
+            }
+        }
+        const float* w = kind == 0 ? a.rope.q_weight : kind == 1 ? a.rope.k_weight : nullptr;
+        if (__any_sync(0xffffffffu, live && w)) {
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = __fadd_rn(__fmul_rn(x[0][j], x[0][j]), __fmul_rn(x[1][j], x[1][j]));
+            const float mean = __fdiv_rn(group_tree<D>(p, lane), (float)D);
+            const float n = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, a.rope.eps)));
+            if (live && w) {
+                float wv[8];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    load8f(w + D / 2 * y + 8 * r, wv);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[y][j] = __fmul_rn(__fmul_rn(x[y][j], n), wv[j]);
+                }
+            }
+        }
+        if (style == kPairsHalf) {
+            if (kind != 2) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float u = x[0][j], v = x[1][j];
+                    x[0][j] = __fsub_rn(__fmul_rn(u, c[0][j]), __fmul_rn(v, s[0][j]));
+                    x[1][j] = __fadd_rn(__fmul_rn(v, c[0][j]), __fmul_rn(u, s[0][j]));
+                }
+            }
+        } else if (style == kPairsNext) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+                if (kind != 2 && D / 2 * y + 8 * r < 2 * half) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float u = x[y][2 * j], v = x[y][2 * j + 1];
+                        x[y][2 * j] = __fsub_rn(__fmul_rn(u, c[y][j]), __fmul_rn(v, s[y][j]));
+                        x[y][2 * j + 1] = __fadd_rn(__fmul_rn(v, c[y][j]), __fmul_rn(u, s[y][j]));
+                    }
+                }
+        } else if (style == kPairsApart) {  // partners are whole chunks of 8, in another lane or slot
+            float z[2][8];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int i = D / 2 * y + 8 * r, chunk = (i < half ? i + half : i - half) / 8;
+                const bool turn = i < 2 * half;
+                const int from = sub * LPR + (turn ? chunk % LPR : r);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v0 = __shfl_sync(0xffffffffu, x[0][j], from), v1 = __shfl_sync(0xffffffffu, x[1][j], from);
+                    const float own = __fmul_rn(x[y][j], c[y][j]), other = __fmul_rn(chunk < LPR ? v0 : v1, s[y][j]);
+                    z[y][j] = !turn || kind == 2 ? x[y][j] : i < half ? __fsub_rn(own, other) : __fadd_rn(own, other);
+                }
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[y][j] = z[y][j];
+        }
+        O* out = reinterpret_cast<O*>(kind == 0 ? a.q_out : kind == 1 ? a.k_out : a.v_out);
+        if (out) out += (t * (kind == 0 ? a.n_heads : a.n_kv_heads) + h) * D + 8 * r;
+        const bool encode = APPEND && live && kind != 0;
+        if (live && !encode) {
+            store8(out, x[0]);
+            store8(out + D / 2, x[1]);
+        }
+        if constexpr (APPEND) {
+            if (!__any_sync(0xffffffffu, encode)) continue;
+            int64_t row = -1;
+            if (encode && pos >= 0) {
+                const int pg = __ldg(a.pt.pages + ((int64_t)seq * a.n_kv_heads + h) * a.pt.max_pages + page);
+                if (pg >= 0 && pg < a.pt.n_pages)
+                    row = (int64_t)pg * a.pt.page_size + in_page;
+                else if (r == 0)
+                    raise_device_error(a.err, BC_DEVERR_PAGE);
+            }
+            // sign bytes, mean |z|, residual, codes: encode_row's arithmetic
+            float p[8];
+            uint32_t byte[2] = {0, 0};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[j] = __fadd_rn(fabsf(x[0][j]), fabsf(x[1][j]));
+                byte[0] |= (x[0][j] >= 0.0f ? 1u : 0u) << j;
+                byte[1] |= (x[1][j] >= 0.0f ? 1u : 0u) << j;
+            }
+            const float mean = __fdiv_rn(group_tree<D>(p, lane), (float)D);
+            const uint16_t sb = f2h_bits(mean);
+            const float held = __half2float(__ushort_as_half(sb));
+            const float scale = res == BC_RES_FP16_SCALE ? held : mean;
+            uint32_t word[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                uint32_t v = byte[y] << (8 * (r & 3));
+                v |= __shfl_xor_sync(0xffffffffu, v, 1);
+                word[y] = v | __shfl_xor_sync(0xffffffffu, v, 2);
+            }
+            const bc_kv_planes& P = kind == 1 ? a.K : a.V;
+            if (row >= 0) {
+                uint32_t* sg = reinterpret_cast<uint32_t*>(P.sign) + row * (D / 32);
+                if ((r & 3) < 2) sg[(r & 1) * (D / 64) + r / 4] = word[r & 1];
+                if (r == 0) reinterpret_cast<uint16_t*>(P.bscale)[row] = sb;
+            }
+            float code[2][8], rs = 0.0f;
+            if (res != BC_RES_NONE) {
+                float most = 0.0f;
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        code[y][j] = __fsub_rn(x[y][j], byte[y] >> j & 1 ? scale : -scale);
+                        most = fmaxf(most, fabsf(code[y][j]));
+                    }
+#pragma unroll
+                for (int o = LPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const float inv = most > 0.0f ? __fdiv_rn(7.0f, most) : 0.0f;
+                // |residual * inv| <= 7 (1 + 2^-23), so adding 1.5 * 2^23 + 8 rounds to the nearest whole
+                // number, ties to even, and leaves code + 8 in the low bits; inv is 0 for zero and
+                // non-finite rows, whose codes are all 0
+                constexpr float kRound = 12582920.0f;
+                const bool any = inv > 0.0f;
+                const uint16_t rb = f2h_bits(most);
+                rs = __half2float(__ushort_as_half(rb));
+                uint32_t nib[2] = {0, 0};
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float q = any ? __fadd_rn(__fmul_rn(code[y][j], inv), kRound) : kRound;
+                        // nibble byte t (of 4) holds bits t (low) and t + 4 (high) of the sign byte
+                        nib[y] |= (__float_as_uint(q) & 15u) << (8 * (j & 3) + 4 * (j >> 2));
+                        code[y][j] = __fsub_rn(q, kRound);
+                    }
+                    nib[y] = transpose4(nib[y], r & 3);  // nibble word of t = r % 4, sign bytes 4 (r / 4) .. + 3
+                }
+                if (row >= 0) {
+                    const int t4 = r & 3, g4 = r / 4;
+                    uint8_t* nb = reinterpret_cast<uint8_t*>(P.nib);
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const int chunk = D == 128 ? t4 : D == 256 ? 4 * y + t4 : t4 / 2;
+                        const int at = D == 128 ? 8 * y + 4 * g4 : D == 256 ? 4 * g4 : 8 * (t4 & 1) + 4 * y;
+                        *reinterpret_cast<uint32_t*>(nb + nib_chunk_offset(row, chunk, D) + at) = nib[y];
+                    }
+                    if (r == 0) reinterpret_cast<uint16_t*>(P.rscale)[row] = rb;
+                }
+            }
+            if (encode && out) {  // the rows as the planes hold them
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        v[j] = byte[y] >> j & 1 ? held : -held;
+                        if (res != BC_RES_NONE) {
+                            // code / 7 rounded to nearest: one correction of the product with 1 / 7
+                            constexpr float k7 = 1.0f / 7.0f;
+                            const float q0 = __fmul_rn(code[y][j], k7);
+                            const float q = __fmaf_rn(__fmaf_rn(q0, -7.0f, code[y][j]), k7, q0);
+                            v[j] = __fadd_rn(v[j], __fmul_rn(q, rs));
+                        }
+                        if (row < 0) v[j] = 0.0f;
+                    }
+                    store8(out + D / 2 * y, v);
+                }
+            }
+        }
+    }
+}
+
+// Whether k_rope_lanes takes a call, and in which of its styles.
+static bool lanes_style(const RopeArgs& a, int head_dim, uintptr_t size, bool append, int* style) {
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return false;
+    const bc_heads* in[3] = {&a.q, &a.k, &a.v};
+    const int n[3] = {a.n_heads, a.n_kv_heads, append ? a.n_kv_heads : 0};
+    for (int i = 0; i < 3; ++i)
+        if (n[i] && (!bc_aligned(in[i]->data, 16) || in[i]->token_stride * (int64_t)size % 16 ||
+                     in[i]->head_stride * (int64_t)size % 16))
+            return false;
+    const void* p[7] = {a.q_out, a.k_out, a.v_out, a.rope.q_weight, a.rope.k_weight, a.rope.cos, a.rope.sin};
+    for (const void* x : p)
+        if (!bc_aligned(x, 16)) return false;
+    const int rot = a.rope.rotary_dim;
+    *style = kPairsNone;
+    if (!a.rope.cos) return true;
+    if (a.rope.interleaved) {
+        *style = kPairsNext;
+        return rot % 8 == 0;
+    }
+    *style = rot == head_dim ? kPairsHalf : kPairsApart;
+    return rot % 16 == 0;
+}
+
+template <int D, typename T, typename O, bool APPEND>
+static int launch_lanes(const RopeArgs& a, int style, int res, cudaStream_t st) {
+    const int heads = a.n_heads + (APPEND ? 2 : 1) * a.n_kv_heads;
+    const int groups = (heads + Lanes<D>::ROWS - 1) / Lanes<D>::ROWS;
+    // runs of heads: long ones keep a token's cosines, short ones fill the GPU (some 32 warps on each of 148 SMs)
+    const int64_t fill = a.n_tokens * groups / (148 * 32);
+    const int per = (int)(fill < 1 ? 1 : fill > groups ? groups : fill);
+    const int64_t blocks = (a.n_tokens * ((groups + per - 1) / per) + kRopeWarps - 1) / kRopeWarps;
+    if (blocks > INT32_MAX) return BC_ERR_TOO_LARGE;
+    k_rope_lanes<D, T, O, APPEND><<<(unsigned)blocks, kRopeWarps * 32, 0, st>>>(a, style, per, res);
+    BC_LAUNCH_CHECK();
+    return BC_OK;
+}
+
 template <typename T, typename O, bool APPEND, int RES>
 static int launch_rope(const RopeArgs& a, int head_dim, cudaStream_t st) {
+    int style = 0;
+    if (lanes_style(a, head_dim, sizeof(T), APPEND, &style)) {
+        if (head_dim == 64) return launch_lanes<64, T, O, APPEND>(a, style, RES, st);
+        if (head_dim == 128) return launch_lanes<128, T, O, APPEND>(a, style, RES, st);
+        return launch_lanes<256, T, O, APPEND>(a, style, RES, st);
+    }
     const int64_t jobs = a.n_tokens * (a.n_heads + (APPEND ? 2 : 1) * (int64_t)a.n_kv_heads);
     const int64_t blocks = (jobs + kRopeWarps - 1) / kRopeWarps;
     if (blocks > INT32_MAX) return BC_ERR_TOO_LARGE;
