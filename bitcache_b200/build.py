@@ -4,8 +4,8 @@ Each CUDA source under csrc/ is compiled with nvcc for sm_100a only and linked
 into ``bitcache_b200/libbitcache_b200.so`` next to this file.  The flags match
 the reference build (``-O3 --use_fast_math``): the encoders rely on the same
 fast-math division as the reference kernels to produce bit-identical INT4
-codes and scales.  Sources in IEEE_SOURCES are compiled without fast-math:
-their results are defined by correctly rounded operations.
+codes and scales.  Sources in IEEE_SOURCES are compiled without fast-math and
+without contraction: their results are defined by correctly rounded operations.
 
 Usage: ``python -m bitcache_b200.build`` (rebuilds what changed).
 """
@@ -48,7 +48,7 @@ def _stale(target: str, deps: list[str]) -> bool:
 def _compile(src: str, extra: list[str]) -> str:
     obj = os.path.join(BUILD, os.path.basename(src) + ".o")
     if _stale(obj, [src] + _deps()):
-        fast = [] if os.path.basename(src) in IEEE_SOURCES else ["--use_fast_math"]
+        fast = ["-fmad=false"] if os.path.basename(src) in IEEE_SOURCES else ["--use_fast_math"]
         cmd = [nvcc(), *ARCH, *NVCC_FLAGS, *fast, *extra, "-c", src, "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:

@@ -223,9 +223,25 @@ __device__ __forceinline__ float group_tree(float (&p)[8], int lane) {
     }
 }
 
-// Eight elements of 16 (or 32) contiguous bytes.
-__device__ __forceinline__ void load8(const __half* p, float (&x)[8]) {
-    const uint4 v = ldg_nc_v4(p);
+// A lane's own ring of copies: `stages` ahead of use, without a register and
+// without a barrier, since each lane reads back what it has asked for.
+template <typename T>
+struct Ring {
+    static constexpr int UNITS = sizeof(T) == 4 ? 4 : 2;   // 16-byte units of a lane's 16 elements
+    static constexpr int STAGES = sizeof(T) == 4 ? 3 : 4;
+    static constexpr int WARP_B = STAGES * UNITS * 512;
+};
+__device__ __forceinline__ void copy16(uint8_t* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 read16(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(smem_u32(p)) : "memory");
+    return v;
+}
+// Slot y of the lane's 16 elements in a stage at `at` (the lane's first unit).
+__device__ __forceinline__ void load8(const uint8_t* at, int y, __half, float (&x)[8]) {
+    const uint4 v = read16(at + 512 * y);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -234,8 +250,8 @@ __device__ __forceinline__ void load8(const __half* p, float (&x)[8]) {
         x[2 * i + 1] = f.y;
     }
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
-    const uint4 v = ldg_nc_v4(p);
+__device__ __forceinline__ void load8(const uint8_t* at, int y, __nv_bfloat16, float (&x)[8]) {
+    const uint4 v = read16(at + 512 * y);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -243,10 +259,24 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
         x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
 }
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-    const uint4 v = ldg_nc_v4(p), w = ldg_nc_v4(p + 4);
+__device__ __forceinline__ void load8(const uint8_t* at, int y, float, float (&x)[8]) {
+    const uint4 v = read16(at + 1024 * y), w = read16(at + 1024 * y + 512);
     x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w);
     x[4] = __uint_as_float(w.x), x[5] = __uint_as_float(w.y), x[6] = __uint_as_float(w.z), x[7] = __uint_as_float(w.w);
+}
+
+// Two products at once, each rounded as alone.  Only for products of products: the
+// assembler contracts a packed product with a packed sum behind it, whatever
+// rounding both name.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return *reinterpret_cast<float2*>(&r);
+}
+__device__ __forceinline__ float2 pair(const float (&x)[8], int j) { return make_float2(x[j], x[j + 1]); }
+__device__ __forceinline__ void put(float (&x)[8], int j, float2 v) {
+    x[j] = v.x;
+    x[j + 1] = v.y;
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -281,9 +311,12 @@ __device__ __forceinline__ uint32_t transpose4(uint32_t x, int a) {
 
 enum { kPairsNone = 0, kPairsHalf = 1, kPairsApart = 2, kPairsNext = 3 };  // head_dim / 2 apart, rotary_dim / 2 apart, adjacent
 
-template <int D, typename T, typename O, bool APPEND>
-__global__ void __launch_bounds__(kRopeWarps * 32) k_rope_lanes(const RopeArgs a, int style, int per, int res) {
+// APART: kPairsApart (twice the cosines, and shuffles); otherwise `style`.
+template <int D, typename T, typename O, bool APPEND, bool APART>
+__global__ void __launch_bounds__(kRopeWarps * 32, APPEND ? 2 : 3) k_rope_lanes(const RopeArgs a, int style, int per, int res) {
     constexpr int LPR = Lanes<D>::LPR, ROWS = Lanes<D>::ROWS;
+    using R = Ring<T>;
+    __shared__ __align__(16) uint8_t ring[kRopeWarps * R::WARP_B];
     const int lane = threadIdx.x & 31, r = lane % LPR, sub = lane / LPR;
     const int heads = a.n_heads + (APPEND ? 2 : 1) * a.n_kv_heads;
     const int groups = (heads + ROWS - 1) / ROWS, runs = (groups + per - 1) / per;
@@ -291,6 +324,32 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope_lanes(const RopeArgs a
     if (job >= a.n_tokens * runs) return;
     const int64_t t = job / runs;
     const int g0 = (int)(job - t * runs) * per, g1 = min(groups, g0 + per);
+    uint8_t* mine = ring + (threadIdx.x >> 5) * R::WARP_B + lane * 16;
+
+    // row g of this lane's: what it is, where it lies
+    auto place = [&](int g, int& kind, int& h) {
+        h = g * ROWS + sub;
+        kind = h < a.n_heads ? 0 : h < a.n_heads + a.n_kv_heads ? 1 : 2;
+        h -= kind == 0 ? 0 : kind == 1 ? a.n_heads : a.n_heads + a.n_kv_heads;
+    };
+    auto fetch = [&](int g) {
+        if (g < g1 && g * ROWS + sub < heads) {
+            int kind, h;
+            place(g, kind, h);
+            const bc_heads& in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+            const T* src = reinterpret_cast<const T*>(in.data) + t * in.token_stride + h * in.head_stride + 8 * r;
+            uint8_t* dst = mine + (g - g0) % R::STAGES * (R::UNITS * 512);
+#pragma unroll
+            for (int u = 0; u < R::UNITS / 2; ++u) {
+                copy16(dst + 512 * u, reinterpret_cast<const uint8_t*>(src) + 16 * u);
+                copy16(dst + 512 * (R::UNITS / 2 + u), reinterpret_cast<const uint8_t*>(src + D / 2) + 16 * u);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < R::STAGES; ++i) fetch(g0 + i);
+
     int pos = a.positions[t];
     bool bad = a.rope.cos && pos >= a.rope.n_positions;
     int seq = 0;
@@ -304,25 +363,28 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope_lanes(const RopeArgs a
     }
     const int half = a.rope.rotary_dim / 2;
     int page = 0, in_page = 0;
-    float c[2][8], s[2][8];  // slot by slot; kPairsHalf has the first only, kPairsNext four pairs a slot
+    float c[APART ? 2 : 1][8], s[APART ? 2 : 1][8];  // not APART: 8 pairs (kPairsHalf), or 4 of each slot (kPairsNext)
     if (pos >= 0) {
         const float *cp = a.rope.cos + (int64_t)pos * half, *sp = a.rope.sin + (int64_t)pos * half;
-        if (style == kPairsHalf) {
-            load8f(cp + 8 * r, c[0]);
-            load8f(sp + 8 * r, s[0]);
-        } else if (style != kPairsNone) {
+        if constexpr (APART) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 const int i = D / 2 * x + 8 * r;
                 if (i >= 2 * half) continue;
-                if (style == kPairsApart) {
-                    load8f(cp + (i < half ? i : i - half), c[x]);
-                    load8f(sp + (i < half ? i : i - half), s[x]);
-                } else {
-                    const float4 u = __ldg(reinterpret_cast<const float4*>(cp + i / 2)), v = __ldg(reinterpret_cast<const float4*>(sp + i / 2));
-                    c[x][0] = u.x, c[x][1] = u.y, c[x][2] = u.z, c[x][3] = u.w;
-                    s[x][0] = v.x, s[x][1] = v.y, s[x][2] = v.z, s[x][3] = v.w;
-                }
+                load8f(cp + (i < half ? i : i - half), c[x]);
+                load8f(sp + (i < half ? i : i - half), s[x]);
+            }
+        } else if (style == kPairsHalf) {
+            load8f(cp + 8 * r, c[0]);
+            load8f(sp + 8 * r, s[0]);
+        } else if (style == kPairsNext) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int i = D / 2 * x + 8 * r;
+                if (i >= 2 * half) continue;
+                const float4 u = __ldg(reinterpret_cast<const float4*>(cp + i / 2)), v = __ldg(reinterpret_cast<const float4*>(sp + i / 2));
+                c[0][4 * x] = u.x, c[0][4 * x + 1] = u.y, c[0][4 * x + 2] = u.z, c[0][4 * x + 3] = u.w;
+                s[0][4 * x] = v.x, s[0][4 * x + 1] = v.y, s[0][4 * x + 2] = v.z, s[0][4 * x + 3] = v.w;
             }
         }
         if constexpr (APPEND) {
@@ -330,75 +392,37 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope_lanes(const RopeArgs a
             in_page = pos - page * a.pt.page_size;
         }
     }
-    auto source = [&](int g, int& kind, int& h) -> const T* {
-        h = g * ROWS + sub;
-        if (h >= heads) return nullptr;
-        kind = h < a.n_heads ? 0 : h < a.n_heads + a.n_kv_heads ? 1 : 2;
-        h -= kind == 0 ? 0 : kind == 1 ? a.n_heads : a.n_heads + a.n_kv_heads;
-        const bc_heads& in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-        return reinterpret_cast<const T*>(in.data) + t * in.token_stride + (int64_t)h * in.head_stride + 8 * r;
-    };
-    float next[2][8];
-    int next_kind = 0, next_h = 0;
-    const T* src = source(g0, next_kind, next_h);
-    if (src && pos >= 0) {
-        load8(src, next[0]);
-        load8(src + D / 2, next[1]);
-    }
     for (int g = g0; g < g1; ++g) {
         float x[2][8];
-        const bool live = src != nullptr;
-        const int kind = next_kind, h = next_h;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[0][j] = live && pos >= 0 ? next[0][j] : 0.0f;
-            x[1][j] = live && pos >= 0 ? next[1][j] : 0.0f;
+        const bool live = g * ROWS + sub < heads;
+        int kind, h;
+        place(g, kind, h);
+        asm volatile("cp.async.wait_group %0;" ::"n"(R::STAGES - 1) : "memory");
+        {
+            const uint8_t* at = mine + (g - g0) % R::STAGES * (R::UNITS * 512);
+            load8(at, 0, T{}, x[0]);
+            load8(at, 1, T{}, x[1]);
         }
-        if (g + 1 < g1) {  // the next rows are on their way while these are worked on
-            src = source(g + 1, next_kind, next_h);
-            if (src && pos >= 0) {
-                load8(src, next[0]);
-                load8(src + D / 2, next[1]);
-            }
-        }
+        fetch(g + R::STAGES);
         const float* w = kind == 0 ? a.rope.q_weight : kind == 1 ? a.rope.k_weight : nullptr;
         if (__any_sync(0xffffffffu, live && w)) {
             float p[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) p[j] = __fadd_rn(__fmul_rn(x[0][j], x[0][j]), __fmul_rn(x[1][j], x[1][j]));
-            const float mean = __fdiv_rn(group_tree<D>(p, lane), (float)D);
-            const float n = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(mean, a.rope.eps)));
+            const float mean = __fmul_rn(group_tree<D>(p, lane), 1.0f / D);  // D is a power of two: the quotient
+            const float n = __frcp_rn(__fsqrt_rn(__fadd_rn(mean, a.rope.eps)));
             if (live && w) {
                 float wv[8];
+                const float2 n2 = make_float2(n, n);
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                     load8f(w + D / 2 * y + 8 * r, wv);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) x[y][j] = __fmul_rn(__fmul_rn(x[y][j], n), wv[j]);
+                    for (int j = 0; j < 8; j += 2) put(x[y], j, mul2(mul2(pair(x[y], j), n2), pair(wv, j)));
                 }
             }
         }
-        if (style == kPairsHalf) {
-            if (kind != 2) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float u = x[0][j], v = x[1][j];
-                    x[0][j] = __fsub_rn(__fmul_rn(u, c[0][j]), __fmul_rn(v, s[0][j]));
-                    x[1][j] = __fadd_rn(__fmul_rn(v, c[0][j]), __fmul_rn(u, s[0][j]));
-                }
-            }
-        } else if (style == kPairsNext) {
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-                if (kind != 2 && D / 2 * y + 8 * r < 2 * half) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float u = x[y][2 * j], v = x[y][2 * j + 1];
-                        x[y][2 * j] = __fsub_rn(__fmul_rn(u, c[y][j]), __fmul_rn(v, s[y][j]));
-                        x[y][2 * j + 1] = __fadd_rn(__fmul_rn(v, c[y][j]), __fmul_rn(u, s[y][j]));
-                    }
-                }
-        } else if (style == kPairsApart) {  // partners are whole chunks of 8, in another lane or slot
+        if constexpr (APART) {  // partners are whole chunks of 8, in another lane or slot
             float z[2][8];
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
@@ -416,6 +440,30 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope_lanes(const RopeArgs a
             for (int y = 0; y < 2; ++y)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) x[y][j] = z[y][j];
+        } else if (style == kPairsHalf) {
+            if (kind != 2) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float u = x[0][j], v = x[1][j];
+                    x[0][j] = __fsub_rn(__fmul_rn(u, c[0][j]), __fmul_rn(v, s[0][j]));
+                    x[1][j] = __fadd_rn(__fmul_rn(v, c[0][j]), __fmul_rn(u, s[0][j]));
+                }
+            }
+        } else if (style == kPairsNext) {
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+                if (kind != 2 && D / 2 * y + 8 * r < 2 * half) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float u = x[y][2 * j], v = x[y][2 * j + 1], cc = c[0][4 * y + j], ss = s[0][4 * y + j];
+                        x[y][2 * j] = __fsub_rn(__fmul_rn(u, cc), __fmul_rn(v, ss));
+                        x[y][2 * j + 1] = __fadd_rn(__fmul_rn(v, cc), __fmul_rn(u, ss));
+                    }
+                }
+        }
+        if (pos < 0) {  // padding
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[0][j] = x[1][j] = 0.0f;
         }
         O* out = reinterpret_cast<O*>(kind == 0 ? a.q_out : kind == 1 ? a.k_out : a.v_out);
         if (out) out += (t * (kind == 0 ? a.n_heads : a.n_kv_heads) + h) * D + 8 * r;
@@ -443,7 +491,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope_lanes(const RopeArgs a
                 byte[0] |= (x[0][j] >= 0.0f ? 1u : 0u) << j;
                 byte[1] |= (x[1][j] >= 0.0f ? 1u : 0u) << j;
             }
-            const float mean = __fdiv_rn(group_tree<D>(p, lane), (float)D);
+            const float mean = __fmul_rn(group_tree<D>(p, lane), 1.0f / D);
             const uint16_t sb = f2h_bits(mean);
             const float held = __half2float(__ushort_as_half(sb));
             const float scale = res == BC_RES_FP16_SCALE ? held : mean;
@@ -559,7 +607,10 @@ static int launch_lanes(const RopeArgs& a, int style, int res, cudaStream_t st) 
     const int per = (int)(fill < 1 ? 1 : fill > groups ? groups : fill);
     const int64_t blocks = (a.n_tokens * ((groups + per - 1) / per) + kRopeWarps - 1) / kRopeWarps;
     if (blocks > INT32_MAX) return BC_ERR_TOO_LARGE;
-    k_rope_lanes<D, T, O, APPEND><<<(unsigned)blocks, kRopeWarps * 32, 0, st>>>(a, style, per, res);
+    if (style == kPairsApart)
+        k_rope_lanes<D, T, O, APPEND, true><<<(unsigned)blocks, kRopeWarps * 32, 0, st>>>(a, style, per, res);
+    else
+        k_rope_lanes<D, T, O, APPEND, false><<<(unsigned)blocks, kRopeWarps * 32, 0, st>>>(a, style, per, res);
     BC_LAUNCH_CHECK();
     return BC_OK;
 }
