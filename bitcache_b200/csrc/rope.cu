@@ -482,14 +482,19 @@ __global__ void __launch_bounds__(kRopeWarps * 32, APPEND ? 2 : 3) k_rope_lanes(
                 else if (r == 0)
                     raise_device_error(a.err, BC_DEVERR_PAGE);
             }
-            // sign bytes, mean |z|, residual, codes: encode_row's arithmetic
+            // sign bytes, mean |z|, residual, codes: encode_row's arithmetic.  |z - rec| is ||z| - s|
+            // and the code of z that of |z| with z's sign (rounding is symmetric), `pos_mask` the reference's
+            // z >= 0 (so -0 is, NaN is not).
             float p[8];
-            uint32_t byte[2] = {0, 0};
+            uint32_t byte[2] = {0, 0}, pos_mask[2][8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 p[j] = __fadd_rn(fabsf(x[0][j]), fabsf(x[1][j]));
-                byte[0] |= (x[0][j] >= 0.0f ? 1u : 0u) << j;
-                byte[1] |= (x[1][j] >= 0.0f ? 1u : 0u) << j;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    asm("set.ge.u32.f32 %0, %1, 0f00000000;" : "=r"(pos_mask[y][j]) : "f"(x[y][j]));
+                    byte[y] |= pos_mask[y][j] & (1u << j);
+                }
             }
             const float mean = __fmul_rn(group_tree<D>(p, lane), 1.0f / D);
             const uint16_t sb = f2h_bits(mean);
@@ -508,36 +513,41 @@ __global__ void __launch_bounds__(kRopeWarps * 32, APPEND ? 2 : 3) k_rope_lanes(
                 if ((r & 3) < 2) sg[(r & 1) * (D / 64) + r / 4] = word[r & 1];
                 if (r == 0) reinterpret_cast<uint16_t*>(P.bscale)[row] = sb;
             }
-            float code[2][8], rs = 0.0f;
+            // |residual * inv| <= 7 (1 + 2^-23), so adding 1.5 * 2^23 + 8 rounds to the nearest whole number,
+            // ties to even, and leaves code + 8 in the low bits
+            constexpr float kRound = 12582920.0f;
+            float rs = 0.0f;
+            bool any = false;
             if (res != BC_RES_NONE) {
                 float most = 0.0f;
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        code[y][j] = __fsub_rn(x[y][j], byte[y] >> j & 1 ? scale : -scale);
-                        most = fmaxf(most, fabsf(code[y][j]));
+                        // the residual as if z were positive, then its code as fp32 bits
+                        x[y][j] = __fsub_rn(fabsf(x[y][j]), scale);
+                        most = fmaxf(most, fabsf(x[y][j]));
                     }
 #pragma unroll
                 for (int o = LPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
                 const float inv = most > 0.0f ? __fdiv_rn(7.0f, most) : 0.0f;
-                // |residual * inv| <= 7 (1 + 2^-23), so adding 1.5 * 2^23 + 8 rounds to the nearest whole
-                // number, ties to even, and leaves code + 8 in the low bits; inv is 0 for zero and
-                // non-finite rows, whose codes are all 0
-                constexpr float kRound = 12582920.0f;
-                const bool any = inv > 0.0f;
+                any = inv > 0.0f;  // else (rows of zeros, rows that are not finite) all codes are 0
                 const uint16_t rb = f2h_bits(most);
                 rs = __half2float(__ushort_as_half(rb));
-                uint32_t nib[2] = {0, 0};
+                uint32_t nib[2];
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
+                    uint32_t q[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float q = any ? __fadd_rn(__fmul_rn(code[y][j], inv), kRound) : kRound;
-                        // nibble byte t (of 4) holds bits t (low) and t + 4 (high) of the sign byte
-                        nib[y] |= (__float_as_uint(q) & 15u) << (8 * (j & 3) + 4 * (j >> 2));
-                        code[y][j] = __fsub_rn(q, kRound);
+                        const uint32_t m = __float_as_uint(__fmul_rn(x[y][j], inv)) ^ (~pos_mask[y][j] & 0x80000000u);
+                        x[y][j] = __fadd_rn(__uint_as_float(m), kRound);
+                        q[j] = __float_as_uint(x[y][j]);
                     }
+                    // nibble byte t (of 4) holds bits t (low) and t + 4 (high) of the sign byte
+                    const uint32_t lo = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+                    const uint32_t hi = __byte_perm(__byte_perm(q[4], q[5], 0x0040), __byte_perm(q[6], q[7], 0x0040), 0x5410);
+                    nib[y] = any ? (lo & 0x0F0F0F0Fu) | (hi << 4 & 0xF0F0F0F0u) : 0x88888888u;
                     nib[y] = transpose4(nib[y], r & 3);  // nibble word of t = r % 4, sign bytes 4 (r / 4) .. + 3
                 }
                 if (row >= 0) {
@@ -558,12 +568,12 @@ __global__ void __launch_bounds__(kRopeWarps * 32, APPEND ? 2 : 3) k_rope_lanes(
                     float v[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        v[j] = byte[y] >> j & 1 ? held : -held;
-                        if (res != BC_RES_NONE) {
+                        v[j] = __uint_as_float(__float_as_uint(held) ^ (~pos_mask[y][j] & 0x80000000u));
+                        if (any) {
                             // code / 7 rounded to nearest: one correction of the product with 1 / 7
                             constexpr float k7 = 1.0f / 7.0f;
-                            const float q0 = __fmul_rn(code[y][j], k7);
-                            const float q = __fmaf_rn(__fmaf_rn(q0, -7.0f, code[y][j]), k7, q0);
+                            const float code = __fsub_rn(x[y][j], kRound), q0 = __fmul_rn(code, k7);
+                            const float q = __fmaf_rn(__fmaf_rn(q0, -7.0f, code), k7, q0);
                             v[j] = __fadd_rn(v[j], __fmul_rn(q, rs));
                         }
                         if (row < 0) v[j] = 0.0f;
