@@ -387,12 +387,13 @@ class Rope:
         self.cos, self.sin, self.interleaved, self.eps = cos, sin, bool(interleaved), float(eps)
         self.q_weight, self.k_weight = (None if w is None else w.float().contiguous() for w in (q_weight, k_weight))
         n, half = (0, 0) if cos is None else cos.shape
+        self._rotary = 2 * half
         self._c = _lib.Rope(_lib.ptr(cos), _lib.ptr(sin), _lib.ptr(self.q_weight), _lib.ptr(self.k_weight), n,
                             2 * half, 1 if interleaved else 0, self.eps)
 
     def c(self, head_dim: int) -> _lib.Rope:
-        if self._c.rotary_dim > head_dim:
-            raise RuntimeError(f"rotary_dim {self._c.rotary_dim} exceeds head_dim {head_dim}")
+        if self._rotary > head_dim:
+            raise RuntimeError(f"rotary_dim {self._rotary} exceeds head_dim {head_dim}")
         for w in (self.q_weight, self.k_weight):
             if w is not None and not (w.is_cuda and w.numel() == head_dim):
                 raise RuntimeError(f"norm weights must be CUDA tensors of {head_dim} elements")
@@ -400,26 +401,30 @@ class Rope:
 
 
 def _heads(x: torch.Tensor, name: str, n_tokens: int, head_dim: int, dtype: torch.dtype) -> _lib.Heads:
+    shape, stride = x.shape, x.stride()
     if not x.is_cuda:
         raise RuntimeError(f"{name} must be a CUDA tensor")
-    if x.dim() != 3 or x.shape[0] != n_tokens or x.shape[2] != head_dim:
+    if len(shape) != 3 or shape[0] != n_tokens or shape[2] != head_dim:
         raise RuntimeError(f"{name} must be [n_tokens, heads, head_dim]")
-    if x.dtype != dtype:
+    if x.dtype is not dtype:
         raise RuntimeError(f"{name} must be {dtype} like the others")
-    if head_dim > 1 and x.stride(2) != 1:
+    if stride[2] != 1 and head_dim > 1:
         raise RuntimeError(f"{name}: the elements of a head must be contiguous")
-    return _lib.Heads(x.data_ptr(), x.stride(0), x.stride(1))
+    return _lib.Heads(x.data_ptr(), stride[0], stride[1])
 
 
 def _index(x: torch.Tensor, name: str, n: int) -> int:
-    if not (x.is_cuda and x.dtype == torch.int32 and x.is_contiguous() and x.numel() == n):
+    if not (x.is_cuda and x.dtype is torch.int32 and x.numel() == n and x.is_contiguous()):
         raise RuntimeError(f"{name} must be a contiguous int32 CUDA tensor of {n} elements")
     return x.data_ptr()
 
 
-def _like(x: torch.Tensor | None, name: str, shape: tuple, dtypes, device: torch.device) -> torch.Tensor:
+def _like(x: torch.Tensor | None, name: str, shape: tuple, dtypes, like: torch.Tensor) -> torch.Tensor:
+    """x, checked, or a new contiguous tensor of that shape and the first of the types, on like's device."""
     if x is None:
-        return torch.empty(shape, dtype=dtypes[0], device=device)
+        if like.dtype is dtypes[0] and tuple(like.shape) == shape:
+            return torch.empty_like(like, memory_format=torch.contiguous_format)
+        return torch.empty(shape, dtype=dtypes[0], device=like.device)
     if not (x.is_cuda and x.is_contiguous() and tuple(x.shape) == shape and x.dtype in dtypes):
         raise RuntimeError(f"{name} must be a contiguous CUDA tensor {shape} of {' or '.join(map(str, dtypes))}")
     return x
@@ -434,15 +439,17 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, rope
     token and head strides are free (slices of a packed projection).  positions int32
     [n_tokens]; a negative one marks a padding token, whose rows come back zero.  Outputs are
     contiguous, of the inputs' type unless q_out and k_out (of one type) are given."""
-    n, _, d = q.shape
-    cq, ck = _heads(q, "q", n, d, q.dtype), _heads(k, "k", n, d, q.dtype)
-    if q.dtype not in _DTYPES:
+    n, hq, d = q.shape
+    dtype = q.dtype
+    cq, ck = _heads(q, "q", n, d, dtype), _heads(k, "k", n, d, dtype)
+    hkv = k.shape[1]
+    if dtype not in _DTYPES:
         raise RuntimeError("q and k must be float16, bfloat16 or float32")
     types = tuple(_DTYPES) if q_out is not None else (q.dtype,)
-    q_out = _like(q_out, "q_out", tuple(q.shape), types, q.device)
-    k_out = _like(k_out, "k_out", tuple(k.shape), (q_out.dtype,), q.device)
+    q_out = _like(q_out, "q_out", (n, hq, d), types, q)
+    k_out = _like(k_out, "k_out", (n, hkv, d), (q_out.dtype,), k)
     _lib.check(_lib.load().bc_qk_norm_rope(cq, ck, _index(positions, "positions", n), rope.c(d), q_out.data_ptr(),
-                                           k_out.data_ptr(), n, q.shape[1], k.shape[1], d, _DTYPES[q.dtype],
+                                           k_out.data_ptr(), n, hq, hkv, d, _DTYPES[dtype],
                                            _DTYPES[q_out.dtype], _stream(q)), "qk_norm_rope")
     return q_out, k_out
 
@@ -471,7 +478,7 @@ def append_qkv_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, K: Plane
     if residual_mode != RES_NONE and not (K.compensated and V.compensated):
         raise RuntimeError("a residual mode needs compensated (residual) caches")
     _check_pool(K, V, pt)
-    q_out = _like(q_out, "q_out", (n, hq, d), (torch.float16,), q.device)
+    q_out = _like(q_out, "q_out", (n, hq, d), (torch.float16,), q)
     hats = [torch.empty((n, hkv, d), dtype=torch.float16, device=q.device) for _ in range(2 * want_hat)]
     kh, vh = (h.data_ptr() for h in hats) if want_hat else (None, None)
     _lib.check(_lib.load().bc_append_qkv_paged(cq, ck, cv, _index(seq_ids, "seq_ids", n),
@@ -508,7 +515,7 @@ def decode_attention_shared(q: torch.Tensor, K: Planes, V: Planes, pt: PageTable
     groups = n if prefix_lens is None else prefix_lens.numel()
     if n and (groups == 0 or n % groups):
         raise RuntimeError("prefix_lens must split the sequences into equal groups")
-    out = _like(out, "out", (n, heads, d), (torch.float16,), q.device)
+    out = _like(out, "out", (n, heads, d), (torch.float16,), q)
     lens = _index(seq_lens, "seq_lens", n)
     pre = None if prefix_lens is None else _index(prefix_lens, "prefix_lens", groups)
     if n == 0:
