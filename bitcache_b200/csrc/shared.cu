@@ -560,40 +560,44 @@ __global__ void __launch_bounds__(kShThreads) k_shared_rows(const SharedArgs a, 
     }
 }
 
-// One CTA per (sequence, kv head): joins the pieces of each query row, of its
-// group's prefix (list P) and of its own keys (list O, which may hold both).
+// One warp per query row: joins its pieces, those of its group's prefix (list P)
+// and of its own keys (list O, which may hold both).
 template <int D>
 __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a, const ShList P, const ShList O, bool two) {
     constexpr int VEC = D / 32;  // consecutive floats of a lane
-    __shared__ int64_t scan[2][kShThreads + 1], at[2];
-    const int b = blockIdx.x / a.n_kv, h = blockIdx.x % a.n_kv;
+    __shared__ int64_t scan[2][kShThreads + 1];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t head = (int64_t)blockIdx.x * kShWarps + warp, slot = head / a.group;
+    const int b = (int)(slot / a.n_kv), h = (int)(slot - (int64_t)b * a.n_kv), g = (int)(head - slot * a.group);
+    const bool live = b < a.n_seqs;
     sh_let_next();
     // the lengths are older than the launches before this one, the records are theirs
     const ShList* lists[2] = {&P, &O};
-    const int want[2] = {b / a.per, O.n_pre + b};
-    int64_t total[2];
+    const int want[2] = {live ? b / a.per : 0, O.n_pre + (live ? b : 0)};
+    int64_t total[2], at[2];
     ShEntry x[2];
     total[1] = sh_scan(a, O, scan[1]);
     total[0] = two ? sh_scan(a, P, scan[0]) : total[1];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const ShList& L = *lists[i];
-        const int n = L.n_pre + L.n_own, chunk = (n + kShThreads - 1) / kShThreads;
         x[i].tiles = 0;
+        at[i] = 0;
         if (i == 0 && L.n_pre == 0) continue;
-        if ((int)threadIdx.x == want[i] / chunk) {
-            int64_t sum = scan[two ? i : 1][threadIdx.x];
-            for (int e = threadIdx.x * chunk; e < want[i]; ++e) sum += sh_weight(a, L, sh_entry(a, L, e));
-            at[i] = sum;
+        // the weight before entry want[i]: the run's start, and the run's entries before it, lane by lane
+        const int n = L.n_pre + L.n_own, chunk = (n + kShThreads - 1) / kShThreads, run = want[i] / chunk;
+        int64_t sum = 0;
+        for (int e = run * chunk + lane; e < want[i]; e += 32) sum += sh_weight(a, L, sh_entry(a, L, e));
+        if (chunk > 1) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
+        at[i] = scan[two ? i : 1][run] + sum;
         x[i] = sh_entry(a, L, want[i]);
     }
-    if (sh_len(a, b) < x[0].hi) x[0].tiles = 0;  // takes no part in the prefix
-    __syncthreads();
+    if (live && sh_len(a, b) < x[0].hi) x[0].tiles = 0;  // takes no part in the prefix
     sh_wait_before();
-    for (int g = warp; g < a.group; g += kShWarps) {
-        const int64_t head = ((int64_t)b * a.n_kv + h) * a.group + g;
+    if (live) {
         float M = kShNone, sum = 0.0f, o[VEC];
 #pragma unroll
         for (int k = 0; k < VEC; ++k) o[k] = 0.0f;
@@ -621,7 +625,7 @@ __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a,
                 bool scaled = false;
                 float w = 0.0f;
                 while (todo) {
-                    constexpr int AT_ONCE = VEC >= 8 ? 8 : 16;  // records in flight: an L2 round trip together
+                    constexpr int AT_ONCE = VEC >= 4 ? 8 : 16;  // records in flight: an L2 round trip together
                     float v[AT_ONCE][VEC];
                     int src[AT_ONCE];
 #pragma unroll
@@ -705,7 +709,8 @@ int sh_run(const SharedArgs& a, ShList& L, const ShList* tc, void* scratch, cuda
     cudaError_t e = sh_launch(k_shared_rows<D, COMP>, (L.n_workers + kShWarps - 1) / kShWarps + (tc ? 1 : 0), kShThreads,
                               ShCfg<D, COMP>::SMEM_B, st, a, L, tc != nullptr);
     if (e == cudaSuccess)
-        e = sh_launch(k_shared_merge<D>, a.n_seqs * a.n_kv, kShThreads, 0, st, a, tc ? *tc : L, L, tc != nullptr);
+        e = sh_launch(k_shared_merge<D>, (int)(((int64_t)a.n_seqs * a.n_kv * a.group + kShWarps - 1) / kShWarps), kShThreads, 0,
+                      st, a, tc ? *tc : L, L, tc != nullptr);
     return e == cudaSuccess ? BC_OK : BC_ERR_CUDA_BASE + (int)e;
 }
 
@@ -761,7 +766,7 @@ int bc_decode_attention_shared(const void* q, bc_kv_planes K, bc_kv_planes V, bc
     if (mode != BC_MODE_BINARY && mode != BC_MODE_COMPENSATED) return BC_ERR_ARG;
     if (n_seqs == 0) return BC_OK;
     if (n_groups <= 0 || n_seqs % n_groups) return BC_ERR_ARG;
-    if ((int64_t)n_seqs * n_kv_heads > INT32_MAX || (int64_t)n_seqs * group > INT32_MAX) return BC_ERR_TOO_LARGE;
+    if ((int64_t)n_seqs * n_kv_heads > INT32_MAX / group) return BC_ERR_TOO_LARGE;
     if (!q || !out || !seq_lens) return BC_ERR_ARG;
     if (!pt.pages || pt.page_size <= 0 || pt.page_size % 128 != 0 || pt.n_pages <= 0 || pt.max_pages <= 0)
         return BC_ERR_ARG;
