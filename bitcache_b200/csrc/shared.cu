@@ -611,16 +611,19 @@ __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a,
             const int64_t first = at[i] + it * sh_item_weight(L, x[i]);
             const int c0 = sh_worker_of(total[i], n_workers, first);
             const int c1 = sh_worker_of(total[i], n_workers, first + sh_item_weight(L, x[i]) - 1);
-            const int64_t size = (int64_t)L.rows * (D + 4);
+            const int64_t part = (int64_t)L.rows * (D + 4), size = part * L.copies;
             const float* rec = L.records + (sh_first_item(L, a.n_kv, want[i]) + it) * size + (r % L.rows) * (D + 4);
-            // 32 workers at a time: units and sums lane by lane, then the sums over dims
-            for (int base = c0; base <= c1; base += 32) {
-                const int c = base + lane;
-                bool has = c <= c1;
+            // 32 records at a time (a worker's copies one after the other): units and sums lane by lane, then
+            // the sums over dims
+            const int count = (c1 - c0 + 1) * L.copies;
+            rec += c0 * size;
+            for (int base = 0; base < count; base += 32) {
+                const int c = c0 + (base + lane) / L.copies;
+                bool has = base + lane < count;
                 if (has)
                     has = sh_tile_at(L, sh_begin(total[i], n_workers, c) - first, x[i].tiles) <
                           sh_tile_at(L, sh_begin(total[i], n_workers, c + 1) - first, x[i].tiles);
-                const float2 ul = has ? __ldcg(reinterpret_cast<const float2*>(rec + c * size + D)) : make_float2(kShNone, 0.0f);
+                const float2 ul = has ? __ldcg(reinterpret_cast<const float2*>(rec + (base + lane) * part + D)) : make_float2(kShNone, 0.0f);
                 unsigned todo = __ballot_sync(0xffffffffu, has);
                 bool scaled = false;
                 float w = 0.0f;
@@ -632,7 +635,7 @@ __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a,
                     for (int u = 0; u < AT_ONCE; ++u) {
                         src[u] = todo ? __ffs(todo) - 1 : -1;
                         todo &= todo - 1;
-                        const float* from = rec + (base + src[u]) * size + VEC * lane;
+                        const float* from = rec + (base + src[u]) * part + VEC * lane;
 #pragma unroll
                         for (int k = 0; k < VEC; ++k) v[u][k] = 0.0f;
                         if (src[u] >= 0) {
@@ -717,7 +720,7 @@ int sh_run(const SharedArgs& a, ShList& L, const ShList* tc, void* scratch, cuda
 bool sh_head_dim(int d) { return d == 32 || d == 64 || d == 128 || d == 256; }
 
 // More query rows than this behind one prefix: the prefix kernel.
-constexpr int kShTcRows = 16;
+constexpr int kShTcRows = 8;
 bool sh_takes_tc(int n_seqs, int n_groups, int group, int head_dim) {
     return (head_dim == 64 || head_dim == 128) && (int64_t)(n_seqs / n_groups) * group > kShTcRows && n_seqs > n_groups;
 }
@@ -731,12 +734,13 @@ ShList sh_list(int n_seqs, int n_groups, int group, bool prefixes) {
     L.own_blocks = (group + kShRows - 1) / kShRows;
     L.tile = kShTile;
     L.rows = kShRows;
+    L.copies = 1;
     L.cost = kShItemCost;
     return L;
 }
 
 size_t sh_bytes(const ShList& L, int n_kv, int max_workers, int d) {
-    return (size_t)(sh_first_item(L, n_kv, L.n_pre + L.n_own) + max_workers) * L.rows * (d + 4) * sizeof(float);
+    return (size_t)(sh_first_item(L, n_kv, L.n_pre + L.n_own) + max_workers) * L.copies * L.rows * (d + 4) * sizeof(float);
 }
 
 }  // namespace

@@ -29,7 +29,8 @@ struct SharedArgs {
 struct ShList {
     int n_pre, n_own;
     int pre_blocks, own_blocks;  // blocks of `rows` query rows of a prefix / of a sequence
-    int tile, rows;              // keys of a tile; query rows of a block, and of a record
+    int tile, rows;              // keys of a tile; query rows of a block
+    int copies;                  // rows of a record for each query row: the keys of a tile may be split among copies of it
     int cost;                    // an item's start and end, in tiles
     int n_workers;
     float* records;
@@ -195,7 +196,7 @@ __device__ __forceinline__ void sh_next_piece(const SharedArgs& a, const ShList&
 // The cursor's tile is the last of its piece.
 __device__ __forceinline__ bool sh_piece_ends(const ShCursor& c) { return c.left <= 1 || c.tile + 1 == c.x.tiles; }
 __device__ __forceinline__ float* sh_record(const SharedArgs& a, const ShList& L, const ShCursor& c, int worker, int d) {
-    return L.records + (sh_first_item(L, a.n_kv, c.e) + (int64_t)c.h * c.x.blocks + c.blk + worker) * L.rows * (d + 4);
+    return L.records + (sh_first_item(L, a.n_kv, c.e) + (int64_t)c.h * c.x.blocks + c.blk + worker) * L.copies * L.rows * (d + 4);
 }
 __device__ __forceinline__ int sh_lead(const SharedArgs& a, const ShList& L, const ShCursor& c) {
     return c.e < L.n_pre ? c.e * a.per : c.e - L.n_pre;  // the sequence whose block table is read

@@ -32,6 +32,11 @@
 // Scores are scaled so that P = 2^(s - U) lies below 2^15, U rising when it would
 // not, to 2^8 above the largest; the elements of K, V, Q and P are rounded to fp16
 // once each, sums are fp32.
+//
+// A barrier tells odd phases from even ones, no more: whoever waits on one has to
+// know that the phase before is over.  The value products have two in turn, because
+// the scores of tile i tell (the tensor cores work in order) that the values of
+// tile i - 2 are through, which is the phase before that of tile i.
 #include "shared.cuh"
 #include "shared_tc.h"
 
@@ -64,7 +69,7 @@ struct TcCfg {
     static constexpr int SCAN_OFF = (RAWV_OFF + kTcRaw * RAW_B + 15) / 16 * 16;
     static constexpr int XCH_OFF = SCAN_OFF;  // [2][2][128] maxima of the row halves, once the sums are read
     static constexpr int BAR_OFF = SCAN_OFF + 512 * 4;
-    static constexpr int FLAG_OFF = BAR_OFF + 34 * 8;
+    static constexpr int FLAG_OFF = BAR_OFF + 36 * 8;
     static constexpr int SMEM_B = FLAG_OFF + 20 * 4 + 1024;  // + alignment to the swizzle atom
     // tensor memory columns
     static constexpr int S_COL = 0, O_COL = 256, Q_COL = 256 + D;
@@ -73,7 +78,7 @@ struct TcCfg {
 
 enum TcBar {
     kRawKFull = 0, kRawKEmpty = 3, kRawVFull = 6, kRawVEmpty = 9, kKFull = 12, kKEmpty = 15, kVFull = 18, kVEmpty = 20,
-    kSFull = 22, kPFull = 24, kQFull = 26, kPvDone = 27, kDrain = 28, kPair = 29, kDone = 33, kTcBars = 34
+    kSFull = 22, kPFull = 24, kQFull = 26, kPvDone = 27, kDrain = 29, kPair = 30, kDone = 34, kTcBars = 35
 };
 
 // ---- tcgen05 ---------------------------------------------------------------
@@ -128,6 +133,11 @@ __device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) 
         "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
+}
+__device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tc_ld16(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile(
@@ -324,6 +334,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
         mbar_init(&bar[kQFull], 8);
         for (int i = 0; i < 4; ++i) mbar_init(&bar[kPair + i], 2);
         mbar_init(&bar[kPvDone], 1);
+        mbar_init(&bar[kPvDone + 1], 1);
         mbar_init(&bar[kDrain], 1);
         mbar_init(&bar[kDone], kTcThreads / 32 - 1);
         fence_mbar_init();
@@ -345,8 +356,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
         // ---------------- softmax: row `rl` of the item's block, keys 64 half .. 64 half + 63 ----------------
         const int half = warp >> 2, quad = warp & 3;
         const uint32_t lane_at = tmem + ((uint32_t)(32 * quad) << 16);
-        const int rl = 32 * quad + lane;
-        float* xch = reinterpret_cast<float*>(smem + C::XCH_OFF) + rl;  // [2][2][128]: parity, half, row
+        // few rows: copies of them fill the 128 lanes, and each copy takes its share of a tile's keys
+        const int copies = L.copies, copy = quad * copies >> 2, rl = 32 * quad + lane - copy * (128 / copies);
+        const int width = 64 / copies, key0 = (128 / copies) * copy + width * half;  // this warp's keys of a tile
+        float* xch = reinterpret_cast<float*>(smem + C::XCH_OFF) + 32 * quad + lane;  // [2][2][128]: parity, half, row
         uint64_t* pair = &bar[kPair + quad];
         uint32_t met = 0;  // exchanges with the row's other warp
         float sc = 0.0f, U = kShNone, l = 0.0f;
@@ -378,7 +391,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             if (lane == 0) tc_arrive(&bar[kQFull]);
             U = kShNone;
             l = 0.0f;
-            int first = (cur.x.tile0 + cur.tile) * kTcTile + 64 * half;
+            int first = (cur.x.tile0 + cur.tile) * kTcTile + key0;
             bool begin = true;
 #pragma unroll 1
             for (; i < end; ++i, first += kTcTile, begin = false) {
@@ -387,31 +400,33 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             if (!ok) break;
             tc_fence_after();
             if (busy) {
-                const uint32_t s_at = lane_at + C::S_COL + 128 * b + 64 * half;
+                const uint32_t s_at = lane_at + C::S_COL + 128 * b;
                 const int lo = kbad[i & 7] ? 64 : cur.x.lo - first, hi = cur.x.hi - first;
                 uint32_t v[64];
-                tc_ld32(s_at, *reinterpret_cast<uint32_t(*)[32]>(v));
-                tc_ld32(s_at + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    if (16 * c < width) tc_ld16(s_at + key0 + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(v + 16 * c));
                 tc_wait_ld();
-                if (lo > 0 || hi < 64) {  // keys outside the prefix
+                if (lo > 0 || hi < width) {  // keys outside the prefix
 #pragma unroll
                     for (int k = 0; k < 64; ++k)
                         if (k < lo || k >= hi) v[k] = 0xFF800000u;
                 }
-                float m[4];
+                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) m[k] = __uint_as_float(v[k]);
+                for (int c = 0; c < 4; ++c)
+                    if (16 * c < width) {
 #pragma unroll
-                for (int k = 4; k < 64; k += 4)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) m[j] = fmaxf(m[j], __uint_as_float(v[k + j]));
+                        for (int k = 16 * c; k < 16 * c + 16; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
+                    }
                 float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
                 xch[256 * (met & 1) + 128 * half] = top;
                 __syncwarp();
                 if (lane == 0) tc_arrive(pair);
                 // P with the U of the tiles so far; the maxima, the other half's too, are looked at
                 // afterwards, and in the rare case that U has to rise P is made once more
-                bool again = begin, seen = false;
+                // (with copies, the row's other warp may still read scores where this one's P and zeros go: wait)
+                bool again = begin || copies > 1, seen = false;
                 float tile_sum;
 #pragma unroll 1
                 for (;;) {
@@ -419,26 +434,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     if (!again) {
                         const float2 sc2 = make_float2(sc, sc), U2 = make_float2(-U, -U);
 #pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            uint32_t p[16];
+                        for (int c = 0; c < 4; ++c) {
+                            if (16 * c >= width) continue;
+                            uint32_t p[8];
 #pragma unroll
-                            for (int k = 0; k < 32; k += 2) {
-                                float2 e = tc_fma2(make_float2(__uint_as_float(v[32 * c + k]), __uint_as_float(v[32 * c + k + 1])),
+                            for (int k = 0; k < 16; k += 2) {
+                                float2 e = tc_fma2(make_float2(__uint_as_float(v[16 * c + k]), __uint_as_float(v[16 * c + k + 1])),
                                                    sc2, U2);
                                 e.x = exp2f(e.x);
                                 e.y = exp2f(e.y);
                                 sum = tc_add2(sum, e);
                                 p[k / 2] = h2_bits(__floats2half2_rn(e.x, e.y));
                             }
-                            tc_st16(s_at + 16 * c, p);
+                            // P of key k: column k / 2 of the half tile that it is in, 64 columns apart
+                            tc_st8(s_at + 64 * (key0 >> 6) + ((key0 & 63) >> 1) + 8 * c, p);
+                        }
+                        if (copies > 1) {  // the other copies' keys: P is 0
+                            uint32_t z[16] = {};
+                            tc_st16(s_at + 64 * ((key0 >> 6) ^ 1) + 16 * half, z);
+                            if (copies == 4)
+                                tc_st8(s_at + 64 * (key0 >> 6) + 16 * ((copy & 1) ^ 1) + 8 * half,
+                                       *reinterpret_cast<uint32_t(*)[8]>(z));
                         }
                     }
                     tile_sum = sum.x + sum.y;
                     if (seen) break;
-                    // the products up to the tile before are through as well: O may be scaled, and every phase of
-                    // that barrier is seen by each warp that reads it (it tells odd phases from even ones, no more)
-                    ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead) &&
-                                                     (begin || tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead)));
+                    ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead));
                     if (!ok) break;
                     top = fmaxf(top, xch[256 * (met & 1) + 128 * (half ^ 1)]) * sc;
                     const bool rise = __any_sync(0xffffffffu, top - U > 15.0f);
@@ -447,7 +468,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                         const float U1 = top - U > 15.0f ? top - 8.0f : U, f = exp2f(U - U1);
                         U = U1;
                         l *= f;
-                        if (!begin) {  // O holds the piece's tiles so far
+                        if (!begin) {  // O holds the piece's tiles so far, once their products are through
+                            ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone + ((i - 1) & 1)], (uint32_t)((i - 1) >> 1) & 1u, dead));
+                            if (!ok) break;
                             tc_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < D / 32; ++c) {
@@ -461,7 +484,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                             }
                         }
                     }
-                    tc_wait_st();  // the first P is down before the second goes over it
+                    if (!again) tc_wait_st();  // the first P is down before the second goes over it
                     seen = true;
                     again = false;
                 }
@@ -484,11 +507,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     l += xch[256 * (met & 1) + 128 * (half ^ 1)];
                     ++met;
                 }
-                ok = __all_sync(0xffffffffu, !busy || tc_wait(&bar[kPvDone], (uint32_t)(i - 1) & 1u, dead));
+                ok = __all_sync(0xffffffffu, !busy || tc_wait(&bar[kPvDone + ((i - 1) & 1)], (uint32_t)((i - 1) >> 1) & 1u, dead));
                 if (!ok) break;
                 tc_fence_after();
                 if (busy) {
-                    float* row = sh_record(a, L, cur, blockIdx.x, D) + rl * (D + 4);
+                    float* row = sh_record(a, L, cur, blockIdx.x, D) + (copy * L.rows + rl) * (D + 4);
 #pragma unroll 1
                     for (int c = 0; c < D / 64; ++c) {
                         uint32_t v[32];
@@ -663,7 +686,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     tc_mma(tmem + C::O_COL, p + 8 * k + 32 * (k >> 2), at + (2048 >> 4) * k, tc_idesc(D, true), !first || k > 0,
                            one);
                 tc_commit(&bar[kVEmpty + j % C::VST], one);
-                tc_commit(&bar[kPvDone], one);
+                tc_commit(&bar[kPvDone + (j & 1)], one);
             };
             int i = 0, slot = 0;
             uint32_t round = 0;
@@ -798,6 +821,7 @@ ShList sh_tc_list(int n_seqs, int n_groups, int group) {
     L.pre_blocks = (int)((rows + 127) / 128);
     L.rows = (int)((rows + L.pre_blocks - 1) / L.pre_blocks);
     L.rows = (L.rows + 7) / 8 * 8;
+    L.copies = L.rows <= 32 ? 4 : L.rows <= 64 ? 2 : 1;
     L.own_blocks = 1;
     L.tile = kTcTile;
     L.cost = kTcItemCost;
