@@ -40,6 +40,7 @@ namespace {
 
 constexpr int kShWarps = kShThreads / 32;
 constexpr int kShTile = 32;        // keys per tile
+static_assert(kShTile == 1 << 5, "the list's shift");
 constexpr int kShRows = 8;         // query rows per item
 constexpr int kShStages = 2;
 constexpr int kShItemCost = 2;     // an item's start and end, in tiles
@@ -719,8 +720,11 @@ int sh_run(const SharedArgs& a, ShList& L, const ShList* tc, void* scratch, cuda
 
 bool sh_head_dim(int d) { return d == 32 || d == 64 || d == 128 || d == 256; }
 
-// More query rows than this behind one prefix: the prefix kernel.
-constexpr int kShTcRows = 8;
+// More query rows than this behind one prefix: the prefix kernel, else the rows kernel, which reads the
+// prefix once per 8 rows.  At 65536 keys, rows kernel against prefix kernel: 16 rows 71.6 / 87.3 us, 20 rows
+// 89.6 / 87.2, 32 rows 111.5 / 88.3.  (Up to 8192 keys 32 rows too are still 5 us faster there, but lengths
+// are on the device.)
+constexpr int kShTcRows = 16;
 bool sh_takes_tc(int n_seqs, int n_groups, int group, int head_dim) {
     return (head_dim == 64 || head_dim == 128) && (int64_t)(n_seqs / n_groups) * group > kShTcRows && n_seqs > n_groups;
 }
@@ -732,7 +736,7 @@ ShList sh_list(int n_seqs, int n_groups, int group, bool prefixes) {
     L.n_own = n_seqs;
     L.pre_blocks = (int)((shared + kShRows - 1) / kShRows);
     L.own_blocks = (group + kShRows - 1) / kShRows;
-    L.tile = kShTile;
+    L.shift = 5;
     L.rows = kShRows;
     L.copies = 1;
     L.cost = kShItemCost;

@@ -29,7 +29,7 @@ struct SharedArgs {
 struct ShList {
     int n_pre, n_own;
     int pre_blocks, own_blocks;  // blocks of `rows` query rows of a prefix / of a sequence
-    int tile, rows;              // keys of a tile; query rows of a block
+    int shift, rows;             // keys of a tile: 2^shift; query rows of a block
     int copies;                  // rows of a record for each query row: the keys of a tile may be split among copies of it
     int cost;                    // an item's start and end, in tiles
     int n_workers;
@@ -69,8 +69,8 @@ __device__ __forceinline__ ShEntry sh_entry(const SharedArgs& a, const ShList& L
         x.lo = x.hi < prefix ? 0 : prefix;
         x.blocks = L.own_blocks;
     }
-    x.tile0 = x.lo / L.tile;
-    x.tiles = x.hi > x.lo ? (x.hi + L.tile - 1) / L.tile - x.tile0 : 0;
+    x.tile0 = x.lo >> L.shift;
+    x.tiles = x.hi > x.lo ? ((x.hi - 1) >> L.shift) + 1 - x.tile0 : 0;
     return x;
 }
 __device__ __forceinline__ int sh_item_weight(const ShList& L, const ShEntry& x) { return x.tiles ? x.tiles + L.cost : 0; }
@@ -162,10 +162,10 @@ __device__ __forceinline__ void sh_seek(const SharedArgs& a, const ShList& L, co
         at -= weight;
     }
     const int one = sh_item_weight(L, c.x);
-    const int64_t it = at / one;
-    const int in = (int)(at - it * one);
-    c.blk = (int)(it % c.x.blocks);
-    c.h = (int)(it / c.x.blocks);
+    const int it = (int)((double)at / (double)one);  // (exact: as sh_begin)
+    const int in = (int)(at - (int64_t)it * one);
+    c.h = it / c.x.blocks;
+    c.blk = it - c.h * c.x.blocks;
     c.tile = sh_tile_at(L, in, c.x.tiles);
     c.left -= max(0, L.cost - in);
 }

@@ -9,12 +9,14 @@
 //   f = mean|q| / h:  s = f Q . K
 // (f carries what the rounding of the row's mean would lose).  V = bs sgn v + rs/7 n.
 //
-// Roles of the 27 warps of a CTA, one CTA per SM:
+// Roles of the 28 warps of a CTA, one CTA per SM:
 //   0-7    softmax: a thread owns a query row and half of a tile's keys (warps 0-3
 //          keys 0-63, 4-7 the others; the two warps of a row exchange maxima).
-//          Writes the row's Q into tensor memory, then per tile reads its scores,
-//          keeps U and l, writes P (fp16, over the scores) and, when U moves,
-//          rescales O.
+//          Writes the row's Q (made by k_shared_queries) into tensor memory, then per
+//          tile reads its scores, keeps U and l, writes P (fp16, over the scores) and,
+//          when U moves, rescales O.  Up to 32 rows stand four times in the 128 lanes,
+//          each copy with a quarter of the tile's keys; the copies are joined with the
+//          pieces.
 //   8-23   unpack: packed bytes -> fp16 operand rows in shared memory, two threads
 //          to a key.  K on the first two schedulers, K-major (128-byte swizzle,
 //          blocks of 64 elements); V on the other two, MN-major (dims contiguous).
@@ -23,11 +25,18 @@
 //          more than everything else (13600 clocks a tile, 4200 with rolled loops).
 //   24     issues the products: Q (tensor memory) x K, P (tensor memory) x V.
 //   25, 26 bring K's / V's packed tiles with 1-D bulk copies, three ahead.
+//   27     fills the last warpgroup.
+// K's operand ring holds three half tiles (the sign part, the code part), V's two
+// tiles.
 // Keeping Q in tensor memory spares half of the score product's shared-memory
-// reads, which with the operands' own writes are what bounds the kernel: per
-// tile 96 KB written, 96 KB read by the tensor cores and 43 KB of packed bytes in
-// and out at 128 B per clock are 1900 clocks, the products 1536, the exponentials
-// of 128 rows 1024, and the unpacking about 800 issue slots per scheduler.
+// reads.  Per tile 96 KB are written, 96 KB read by the tensor cores and 43 KB of
+// packed bytes go in and out, 1900 clocks at 128 B each; the products take 1536, the
+// exponentials of 128 rows 1024, the unpacking about 800 issue slots a scheduler.
+// What bounds it is none of these but the chain from one tile to the next (scores,
+// softmax, P, values) with two tiles under way: about 3300 clocks a tile, and the
+// start and end of an item besides.  128 sequences with 8192 keys before them, 32 / 8
+// heads of 128: 83 us with the batch's own keys, of which the products at the tensor
+// cores' rate would take 15.
 //
 // Scores are scaled so that P = 2^(s - U) lies below 2^15, U rising when it would
 // not, to 2^8 above the largest; the elements of K, V, Q and P are rounded to fp16
@@ -124,14 +133,17 @@ __device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t (&r)[32]) {
         : "r"(addr)
         : "memory");
 }
-__device__ __forceinline__ void tc_st32(uint32_t addr, const uint32_t (&r)[32]) {
+// 64 columns of 16 lanes: lane t gets columns 8 j + 2 (t % 4), + 1 of rows t / 4 (r[4 j], r[4 j + 1]) and
+// t / 4 + 8, so that four lanes hold 32 consecutive bytes of a row.
+__device__ __forceinline__ void tc_ld_rows(uint32_t addr, uint32_t (&r)[32]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
         : "memory");
 }
 __device__ __forceinline__ void tc_st8(uint32_t addr, const uint32_t (&r)[8]) {
@@ -253,21 +265,26 @@ __device__ __forceinline__ float2 tc_add2(float2 x, float2 y) {
 }
 
 // The query rows as A operands, one warp a row: [h sgn q | 8/7 q / f] in the order
-// of K's elements, and the scale of the row's scores in log2 units.  A kernel of
-// its own: a softmax thread that made its row itself ran some 800 instructions
+// of K's elements, and the scale of the row's scores in log2 units.  Ordered as the
+// prefix kernel's lanes read them: by group and kv head, then 16-byte unit, then
+// row.  A kernel of its own: a softmax thread that made its row itself ran some 800 instructions
 // once, at the pace of their fetch (12000 clocks a piece).
 constexpr int kTcQueryWarps = 8;
 template <int D, bool COMP>
-__global__ void __launch_bounds__(32 * kTcQueryWarps) k_shared_queries(const __half* __restrict__ q,
-                                                                       uint32_t* __restrict__ ops,
-                                                                       float* __restrict__ scales, int64_t rows) {
+__global__ void __launch_bounds__(32 * kTcQueryWarps) k_shared_queries(const SharedArgs a, uint32_t* __restrict__ ops,
+                                                                       float* __restrict__ scales) {
     constexpr int WORDS = (COMP ? 2 : 1) * D / 2;
     sh_wait_before();
     sh_let_next();
-    const int64_t row = (int64_t)blockIdx.x * kTcQueryWarps + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= rows) return;
-    const __half* x = q + row * D;
+    const int64_t head = (int64_t)blockIdx.x * kTcQueryWarps + (threadIdx.x >> 5), slot = head / a.group;
+    const int lane = threadIdx.x & 31, b = (int)(slot / a.n_kv);
+    if (b >= a.n_seqs) return;
+    // query row r of (group of sequences, kv head) `item`, of `rows`
+    const int rows = a.per * a.group, seq = b % a.per;
+    const int64_t item = (int64_t)(b / a.per) * a.n_kv + (slot - (int64_t)b * a.n_kv);
+    const int r = seq * a.group + (int)(head - slot * a.group);
+    uint32_t* op = ops + item * rows * WORDS + 4 * r;
+    const __half* x = a.q + head * D;
     float mag = 0.0f;
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) mag += fabsf(__half2float(x[32 * k + lane]));
@@ -276,16 +293,16 @@ __global__ void __launch_bounds__(32 * kTcQueryWarps) k_shared_queries(const __h
     const float mean = mag * (1.0f / D);
     const __half h = __float2half_rn(mean);
     const float hf = __half2float(h), f = hf == 0.0f ? 1.0f : mean / hf, g = (8.0f / 7.0f) / f;
-    if (lane == 0) scales[row] = f * kShLog2e * rsqrtf((float)D);
+    if (lane == 0) scales[item * rows + r] = f * kShLog2e * rsqrtf((float)D);
     const uint32_t hb = __half_as_ushort(h);
 #pragma unroll
     for (int k = 0; k < D / 64; ++k) {
         const int c = 32 * k + lane, d0 = 32 * (c / 16) + c % 16;
-        ops[row * WORDS + c] = (hb | (__half2float(x[d0]) >= 0.0f ? 0u : 0x8000u)) |
-                               ((hb | (__half2float(x[d0 + 16]) >= 0.0f ? 0u : 0x8000u)) << 16);
+        op[(int64_t)(c / 4) * rows * 4 + c % 4] = (hb | (__half2float(x[d0]) >= 0.0f ? 0u : 0x8000u)) |
+                                                  ((hb | (__half2float(x[d0 + 16]) >= 0.0f ? 0u : 0x8000u)) << 16);
         if constexpr (COMP)
-            ops[row * WORDS + D / 2 + c] = h2_bits(__floats2half2_rn(__half2float(x[sh_code_dim(D, 2 * c)]) * g,
-                                                                     __half2float(x[sh_code_dim(D, 2 * c + 1)]) * g));
+            op[(int64_t)(D / 8 + c / 4) * rows * 4 + c % 4] =
+                h2_bits(__floats2half2_rn(__half2float(x[sh_code_dim(D, 2 * c)]) * g, __half2float(x[sh_code_dim(D, 2 * c + 1)]) * g));
     }
 }
 
@@ -367,25 +384,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
         bool ok = true;
         for (int i = 0; ok && cur.left > 0; sh_next_piece(a, L, cur)) {
             const int end = i + sh_piece_tiles(cur);
-            const __half* src = rl < L.rows ? sh_query(a, L, cur, cur.blk * L.rows + rl, D) : nullptr;
-            const bool valid = src != nullptr, busy = __any_sync(0xffffffffu, valid);
+            const int rows = a.per * a.group, r = cur.blk * L.rows + rl;
+            const int64_t item = (int64_t)cur.e * a.n_kv + cur.h;
+            const bool valid = rl < L.rows && r < rows, busy = __any_sync(0xffffffffu, valid);
             if (busy && half < C::PARTS) {
-                const uint32_t* op = ops + (valid ? (src - a.q) / D : 0) * (C::KE / 2) + D / 2 * half;
-                uint32_t x[D / 2];
+                const uint32_t* op = ops + (item * (C::KE / 2) + D / 2 * half) * rows + 4 * (valid ? r : 0);
 #pragma unroll
-                for (int k = 0; k < D / 2; k += 4) {
-                    const uint4 w = valid ? __ldcg(reinterpret_cast<const uint4*>(op + k)) : make_uint4(0, 0, 0, 0);
-                    x[k] = w.x;
-                    x[k + 1] = w.y;
-                    x[k + 2] = w.z;
-                    x[k + 3] = w.w;
+                for (int k0 = 0; k0 < D / 2; k0 += 32) {
+                    uint32_t x[32];
+#pragma unroll
+                    for (int k = 0; k < 32; k += 4) {
+                        const uint4 w = valid ? __ldcg(reinterpret_cast<const uint4*>(op + (int64_t)(k0 + k) * rows)) : make_uint4(0, 0, 0, 0);
+                        x[k] = w.x;
+                        x[k + 1] = w.y;
+                        x[k + 2] = w.z;
+                        x[k + 3] = w.w;
+                    }
+                    const uint32_t to = lane_at + C::Q_COL + D / 2 * half + k0;
+                    tc_st16(to, *reinterpret_cast<uint32_t(*)[16]>(x));
+                    tc_st16(to + 16, *reinterpret_cast<uint32_t(*)[16]>(x + 16));
                 }
-#pragma unroll
-                for (int k = 0; k < D / 2; k += 16)
-                    tc_st16(lane_at + C::Q_COL + D / 2 * half + k, *reinterpret_cast<uint32_t(*)[16]>(x + k));
                 tc_wait_st();
             }
-            sc = valid ? __ldcg(scales + (src - a.q) / D) : 1.0f;
+            sc = valid ? __ldcg(scales + item * rows + r) : 1.0f;
             tc_fence_before();
             __syncwarp();
             if (lane == 0) tc_arrive(&bar[kQFull]);
@@ -395,107 +416,106 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             bool begin = true;
 #pragma unroll 1
             for (; i < end; ++i, first += kTcTile, begin = false) {
-            const int b = i & 1;
-            ok = __all_sync(0xffffffffu, tc_wait(&bar[kSFull + b], (uint32_t)(i >> 1) & 1u, dead));
-            if (!ok) break;
-            tc_fence_after();
-            if (busy) {
-                const uint32_t s_at = lane_at + C::S_COL + 128 * b;
-                const int lo = kbad[i & 7] ? 64 : cur.x.lo - first, hi = cur.x.hi - first;
-                uint32_t v[64];
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (16 * c < width) tc_ld16(s_at + key0 + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(v + 16 * c));
-                tc_wait_ld();
-                if (lo > 0 || hi < width) {  // keys outside the prefix
-#pragma unroll
-                    for (int k = 0; k < 64; ++k)
-                        if (k < lo || k >= hi) v[k] = 0xFF800000u;
-                }
-                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    if (16 * c < width) {
-#pragma unroll
-                        for (int k = 16 * c; k < 16 * c + 16; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
+                const int b = i & 1;
+                ok = __all_sync(0xffffffffu, tc_wait(&bar[kSFull + b], (uint32_t)(i >> 1) & 1u, dead));
+                if (!ok) break;
+                tc_fence_after();
+                if (busy) {
+                    const uint32_t s_at = lane_at + C::S_COL + 128 * b;
+                    const int lo = kbad[i & 7] ? 64 : cur.x.lo - first, hi = cur.x.hi - first;
+                    uint32_t v[64];
+    #pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (16 * c < width) tc_ld16(s_at + key0 + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(v + 16 * c));
+                    tc_wait_ld();
+                    if (lo > 0 || hi < width) {  // keys outside the prefix
+    #pragma unroll
+                        for (int k = 0; k < 64; ++k)
+                            if (k < lo || k >= hi) v[k] = 0xFF800000u;
                     }
-                float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-                xch[256 * (met & 1) + 128 * half] = top;
-                __syncwarp();
-                if (lane == 0) tc_arrive(pair);
-                // P with the U of the tiles so far; the maxima, the other half's too, are looked at
-                // afterwards, and in the rare case that U has to rise P is made once more
-                // (with copies, the row's other warp may still read scores where this one's P and zeros go: wait)
-                bool again = begin || copies > 1, seen = false;
-                float tile_sum;
-#pragma unroll 1
-                for (;;) {
-                    float2 sum = make_float2(0.0f, 0.0f);
-                    if (!again) {
-                        const float2 sc2 = make_float2(sc, sc), U2 = make_float2(-U, -U);
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            if (16 * c >= width) continue;
-                            uint32_t p[8];
-#pragma unroll
-                            for (int k = 0; k < 16; k += 2) {
-                                float2 e = tc_fma2(make_float2(__uint_as_float(v[16 * c + k]), __uint_as_float(v[16 * c + k + 1])),
-                                                   sc2, U2);
-                                e.x = exp2f(e.x);
-                                e.y = exp2f(e.y);
-                                sum = tc_add2(sum, e);
-                                p[k / 2] = h2_bits(__floats2half2_rn(e.x, e.y));
-                            }
-                            // P of key k: column k / 2 of the half tile that it is in, 64 columns apart
-                            tc_st8(s_at + 64 * (key0 >> 6) + ((key0 & 63) >> 1) + 8 * c, p);
+                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    #pragma unroll
+                    for (int c = 0; c < 4; ++c)
+                        if (16 * c < width) {
+    #pragma unroll
+                            for (int k = 16 * c; k < 16 * c + 16; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
                         }
-                        if (copies > 1) {  // the other copies' keys: P is 0
-                            uint32_t z[16] = {};
-                            tc_st16(s_at + 64 * ((key0 >> 6) ^ 1) + 16 * half, z);
-                            if (copies == 4)
+                    float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+                    xch[256 * (met & 1) + 128 * half] = top;
+                    __syncwarp();
+                    if (lane == 0) tc_arrive(pair);
+                    // P with the U of the tiles so far; the maxima, the other half's too, are looked at
+                    // afterwards, and in the rare case that U has to rise P is made once more
+                    // (with copies, the row's other warp may still read scores where this one's P and zeros go: wait)
+                    bool again = begin || copies > 1, seen = false;
+                    float tile_sum;
+    #pragma unroll 1
+                    for (;;) {
+                        float2 sum = make_float2(0.0f, 0.0f);
+                        if (!again) {
+                            const float2 sc2 = make_float2(sc, sc), U2 = make_float2(-U, -U);
+    #pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                if (16 * c >= width) continue;
+                                uint32_t p[8];
+    #pragma unroll
+                                for (int k = 0; k < 16; k += 2) {
+                                    float2 e = tc_fma2(make_float2(__uint_as_float(v[16 * c + k]), __uint_as_float(v[16 * c + k + 1])),
+                                                       sc2, U2);
+                                    e.x = exp2f(e.x);
+                                    e.y = exp2f(e.y);
+                                    sum = tc_add2(sum, e);
+                                    p[k / 2] = h2_bits(__floats2half2_rn(e.x, e.y));
+                                }
+                                // P of key k: column k / 2 of the half tile that it is in, 64 columns apart
+                                tc_st8(s_at + 64 * (key0 >> 6) + ((key0 & 63) >> 1) + 8 * c, p);
+                            }
+                            if (copies > 1) {  // the other copies' keys: P is 0
+                                uint32_t z[16] = {};
+                                tc_st16(s_at + 64 * ((key0 >> 6) ^ 1) + 16 * half, z);
                                 tc_st8(s_at + 64 * (key0 >> 6) + 16 * ((copy & 1) ^ 1) + 8 * half,
                                        *reinterpret_cast<uint32_t(*)[8]>(z));
-                        }
-                    }
-                    tile_sum = sum.x + sum.y;
-                    if (seen) break;
-                    ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead));
-                    if (!ok) break;
-                    top = fmaxf(top, xch[256 * (met & 1) + 128 * (half ^ 1)]) * sc;
-                    const bool rise = __any_sync(0xffffffffu, top - U > 15.0f);
-                    if (!rise && !again) break;
-                    if (rise) {
-                        const float U1 = top - U > 15.0f ? top - 8.0f : U, f = exp2f(U - U1);
-                        U = U1;
-                        l *= f;
-                        if (!begin) {  // O holds the piece's tiles so far, once their products are through
-                            ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone + ((i - 1) & 1)], (uint32_t)((i - 1) >> 1) & 1u, dead));
-                            if (!ok) break;
-                            tc_fence_after();
-#pragma unroll 1
-                            for (int c = 0; c < D / 32; ++c) {
-                                const uint32_t at = lane_at + C::O_COL + D / 2 * half + 16 * c;
-                                uint32_t o[16];
-                                tc_ld16(at, o);
-                                tc_wait_ld();
-#pragma unroll
-                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                                tc_st16(at, o);
                             }
                         }
+                        tile_sum = sum.x + sum.y;
+                        if (seen) break;
+                        ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead));
+                        if (!ok) break;
+                        top = fmaxf(top, xch[256 * (met & 1) + 128 * (half ^ 1)]) * sc;
+                        const bool rise = __any_sync(0xffffffffu, top - U > 15.0f);
+                        if (!rise && !again) break;
+                        if (rise) {
+                            const float U1 = top - U > 15.0f ? top - 8.0f : U, f = exp2f(U - U1);
+                            U = U1;
+                            l *= f;
+                            if (!begin) {  // O holds the piece's tiles so far, once their products are through
+                                ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone + ((i - 1) & 1)], (uint32_t)((i - 1) >> 1) & 1u, dead));
+                                if (!ok) break;
+                                tc_fence_after();
+    #pragma unroll 1
+                                for (int c = 0; c < D / 32; ++c) {
+                                    const uint32_t at = lane_at + C::O_COL + D / 2 * half + 16 * c;
+                                    uint32_t o[16];
+                                    tc_ld16(at, o);
+                                    tc_wait_ld();
+    #pragma unroll
+                                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                    tc_st16(at, o);
+                                }
+                            }
+                        }
+                        if (!again) tc_wait_st();  // the first P is down before the second goes over it
+                        seen = true;
+                        again = false;
                     }
-                    if (!again) tc_wait_st();  // the first P is down before the second goes over it
-                    seen = true;
-                    again = false;
+                    if (!ok) break;
+                    ++met;
+                    l += tile_sum;
+                    tc_wait_st();
                 }
-                if (!ok) break;
-                ++met;
-                l += tile_sum;
-                tc_wait_st();
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) tc_arrive(&bar[kPFull + b]);
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc_arrive(&bar[kPFull + b]);
             }
             if (ok) {
                 if (busy) {  // the row's sum: both halves'
@@ -512,16 +532,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                 tc_fence_after();
                 if (busy) {
                     float* row = sh_record(a, L, cur, blockIdx.x, D) + (copy * L.rows + rl) * (D + 4);
+                    const unsigned live = __ballot_sync(0xffffffffu, valid);
+                    // 64 columns at a time (all of them at head_dim 64: one warp each half of the rows)
 #pragma unroll 1
-                    for (int c = 0; c < D / 64; ++c) {
+                    for (int s16 = D == 64 ? half : 0; s16 < (D == 64 ? half + 1 : 2); ++s16) {
                         uint32_t v[32];
-                        tc_ld32(lane_at + C::O_COL + D / 2 * half + 32 * c, v);
+                        const int col = D == 64 ? 0 : 64 * half;
+                        tc_ld_rows(lane_at + ((uint32_t)(16 * s16) << 16) + C::O_COL + col, v);
                         tc_wait_ld();
-                        if (valid) {
 #pragma unroll
-                            for (int k = 0; k < 32; k += 4)
-                                *reinterpret_cast<uint4*>(row + D / 2 * half + 32 * c + k) =
-                                    make_uint4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                        for (int y = 0; y < 2; ++y) {
+                            const int at = 16 * s16 + 8 * y + (lane >> 2);  // the row's lane
+                            float* to = row + (at - lane) * (D + 4) + col + 2 * (lane & 3);
+                            if (live >> at & 1) {
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+                                    *reinterpret_cast<uint2*>(to + 8 * j) = make_uint2(v[4 * j + 2 * y], v[4 * j + 2 * y + 1]);
+                            }
                         }
                     }
                     if (valid && half == 0) *reinterpret_cast<float2*>(row + D) = make_float2(U, l);
@@ -781,7 +808,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             }
             // copies in flight land before the block's memory is given back (bounded)
             for (int t = max(0, i - kTcRaw); t < i; ++t)
-            tc_settle(&full[t % kTcRaw], (uint32_t)(t / kTcRaw) & 1u, dead);
+                tc_settle(&full[t % kTcRaw], (uint32_t)(t / kTcRaw) & 1u, dead);
         }
     }
     tc_leave(&bar[kDone]);
@@ -805,7 +832,7 @@ int tc_run(const SharedArgs& a, const ShList& L, void* scratch, cudaStream_t st)
     uint32_t* ops = (uint32_t*)scratch;
     float* scales = (float*)(ops + rows * (TcCfg<D, COMP>::KE / 2));
     e = sh_launch(k_shared_queries<D, COMP>, (int)((rows + kTcQueryWarps - 1) / kTcQueryWarps), 32 * kTcQueryWarps, 0, st,
-                  a.q, ops, scales, rows);
+                  a, ops, scales);
     if (e == cudaSuccess)
         e = sh_launch(k_shared_prefix<D, COMP>, L.n_workers, kTcThreads, smem, st, a, L, (const uint32_t*)ops,
                       (const float*)scales);
@@ -821,9 +848,12 @@ ShList sh_tc_list(int n_seqs, int n_groups, int group) {
     L.pre_blocks = (int)((rows + 127) / 128);
     L.rows = (int)((rows + L.pre_blocks - 1) / L.pre_blocks);
     L.rows = (L.rows + 7) / 8 * 8;
-    L.copies = L.rows <= 32 ? 4 : L.rows <= 64 ? 2 : 1;
+    // Up to 32 rows: four copies of the rows, each with a quarter of a tile's keys, so that all softmax lanes
+    // work (32 rows and 200000 keys: 212 us, 227 with one copy).  Two copies of 33 to 64 rows cost more than
+    // they spare (64 rows, 32768 keys: 70.4 us, 68.8 with one): the tile's chain of waits is then the longer.
+    L.copies = L.rows <= 32 ? 4 : 1;
     L.own_blocks = 1;
-    L.tile = kTcTile;
+    L.shift = 7;
     L.cost = kTcItemCost;
     return L;
 }
