@@ -561,124 +561,156 @@ __global__ void __launch_bounds__(kShThreads) k_shared_rows(const SharedArgs a, 
     }
 }
 
-// One warp per query row: joins its pieces, those of its group's prefix (list P)
-// and of its own keys (list O, which may hold both).
-template <int D>
+// Joins a query row's pieces, those of its group's prefix (list P) and of its own
+// keys (list O, which may hold both): WPR warps per row.  All that the lengths tell
+// is worked out before the wait for the launches that write the records; behind it
+// a row's records come in one L2 round trip as long as they are few.
+template <int D, int WPR>
 __global__ void __launch_bounds__(kShThreads) k_shared_merge(const SharedArgs a, const ShList P, const ShList O, bool two) {
     constexpr int VEC = D / 32;  // consecutive floats of a lane
+    constexpr int AT_ONCE = WPR == 1 || VEC > 4 ? 8 : 16;  // records in flight
     __shared__ int64_t scan[2][kShThreads + 1];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t head = (int64_t)blockIdx.x * kShWarps + warp, slot = head / a.group;
+    __shared__ float parts[WPR > 1 ? kShWarps : 1][D], marks[2][kShWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, mine = warp % WPR;
+    const int64_t head = ((int64_t)blockIdx.x * kShWarps + warp) / WPR, slot = head / a.group;
     const int b = (int)(slot / a.n_kv), h = (int)(slot - (int64_t)b * a.n_kv), g = (int)(head - slot * a.group);
     const bool live = b < a.n_seqs;
     sh_let_next();
     // the lengths are older than the launches before this one, the records are theirs
-    const ShList* lists[2] = {&P, &O};
-    const int want[2] = {live ? b / a.per : 0, O.n_pre + (live ? b : 0)};
-    int64_t total[2], at[2];
-    ShEntry x[2];
+    int64_t total[2], first[2] = {0, 0}, size[2];
+    int n_workers[2], tiles[2], c0[2] = {0, 0}, count[2] = {0, 0};
+    const float* rec[2] = {nullptr, nullptr};
     total[1] = sh_scan(a, O, scan[1]);
     total[0] = two ? sh_scan(a, P, scan[0]) : total[1];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const ShList& L = *lists[i];
-        x[i].tiles = 0;
-        at[i] = 0;
+        const ShList& L = i ? O : P;
+        const int want = i ? O.n_pre + (live ? b : 0) : live ? b / a.per : 0;
+        size[i] = (int64_t)L.rows * (D + 4) * L.copies;
+        n_workers[i] = tiles[i] = 0;
         if (i == 0 && L.n_pre == 0) continue;
-        // the weight before entry want[i]: the run's start, and the run's entries before it, lane by lane
-        const int n = L.n_pre + L.n_own, chunk = (n + kShThreads - 1) / kShThreads, run = want[i] / chunk;
+        // the weight before entry `want`: the run's start, and the run's entries before it, lane by lane
+        const int n = L.n_pre + L.n_own, chunk = (n + kShThreads - 1) / kShThreads, run = want / chunk;
         int64_t sum = 0;
-        for (int e = run * chunk + lane; e < want[i]; e += 32) sum += sh_weight(a, L, sh_entry(a, L, e));
+        for (int e = run * chunk + lane; e < want; e += 32) sum += sh_weight(a, L, sh_entry(a, L, e));
         if (chunk > 1) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
-        at[i] = scan[two ? i : 1][run] + sum;
-        x[i] = sh_entry(a, L, want[i]);
+        const ShEntry x = sh_entry(a, L, want);
+        if (!live || x.tiles == 0 || (i == 0 && sh_len(a, b) < x.hi)) continue;  // (a shorter sequence takes no part in the prefix)
+        tiles[i] = x.tiles;
+        n_workers[i] = sh_workers(L, total[i]);
+        const int r = i == 0 ? (b % a.per) * a.group + g : g;
+        const int it = h * x.blocks + r / L.rows;
+        first[i] = scan[two ? i : 1][run] + sum + (int64_t)it * sh_item_weight(L, x);
+        c0[i] = sh_worker_of(total[i], n_workers[i], first[i]);
+        count[i] = (sh_worker_of(total[i], n_workers[i], first[i] + sh_item_weight(L, x) - 1) - c0[i] + 1) * L.copies;
+        rec[i] = L.records + (sh_first_item(L, a.n_kv, want) + it + c0[i]) * size[i] + (r % L.rows) * (D + 4);
     }
-    if (live && sh_len(a, b) < x[0].hi) x[0].tiles = 0;  // takes no part in the prefix
+    // record q: the prefix's (a worker's copies one after the other), then the own keys'; null where a
+    // worker's stretch holds no tile of the item
+    const int all = count[0] + count[1], copies = P.copies;
+    auto record = [&](int q) -> const float* {
+        const bool own = q >= count[0];
+        const int at = own ? q - count[0] : q, c = own ? at : at / copies;
+        const ShList& L = own ? O : P;
+        const int64_t from = own ? first[1] : first[0], sum = own ? total[1] : total[0], step = own ? size[1] : size[0] / copies;
+        const int n = own ? n_workers[1] : n_workers[0], w = c + (own ? c0[1] : c0[0]), t = own ? tiles[1] : tiles[0];
+        if (q >= all || sh_tile_at(L, sh_begin(sum, n, w) - from, t) >= sh_tile_at(L, sh_begin(sum, n, w + 1) - from, t)) return nullptr;
+        return (own ? rec[1] : rec[0]) + at * step;
+    };
+    float M = kShNone, sum = 0.0f, o[VEC];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) o[k] = 0.0f;
+    const float* from = record(WPR * lane + mine);
     sh_wait_before();
-    if (live) {
-        float M = kShNone, sum = 0.0f, o[VEC];
+#pragma unroll 1
+    for (int base = 0; base < all; from = record((base += 32 * WPR) + WPR * lane + mine)) {
+        const float2 ul = from ? __ldcg(reinterpret_cast<const float2*>(from + D)) : make_float2(kShNone, 0.0f);
+        unsigned todo = __ballot_sync(0xffffffffu, from != nullptr);
+        bool scaled = false;
+        float w = 0.0f;
+        while (todo) {
+            float v[AT_ONCE][VEC];
+            int src[AT_ONCE];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) o[k] = 0.0f;
+            for (int u = 0; u < AT_ONCE; ++u) {
+                src[u] = todo ? __ffs(todo) - 1 : -1;
+                todo &= todo - 1;
+                const float* x = reinterpret_cast<const float*>(
+                                     __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(from), src[u] & 31)) + VEC * lane;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (x[i].tiles == 0) continue;
-            const ShList& L = *lists[i];
-            const int n_workers = sh_workers(L, total[i]);
-            const int r = i == 0 ? (b % a.per) * a.group + g : g;
-            const int64_t it = (int64_t)h * x[i].blocks + r / L.rows;
-            const int64_t first = at[i] + it * sh_item_weight(L, x[i]);
-            const int c0 = sh_worker_of(total[i], n_workers, first);
-            const int c1 = sh_worker_of(total[i], n_workers, first + sh_item_weight(L, x[i]) - 1);
-            const int64_t part = (int64_t)L.rows * (D + 4), size = part * L.copies;
-            const float* rec = L.records + (sh_first_item(L, a.n_kv, want[i]) + it) * size + (r % L.rows) * (D + 4);
-            // 32 records at a time (a worker's copies one after the other): units and sums lane by lane, then
-            // the sums over dims
-            const int count = (c1 - c0 + 1) * L.copies;
-            rec += c0 * size;
-            for (int base = 0; base < count; base += 32) {
-                const int c = c0 + (base + lane) / L.copies;
-                bool has = base + lane < count;
-                if (has)
-                    has = sh_tile_at(L, sh_begin(total[i], n_workers, c) - first, x[i].tiles) <
-                          sh_tile_at(L, sh_begin(total[i], n_workers, c + 1) - first, x[i].tiles);
-                const float2 ul = has ? __ldcg(reinterpret_cast<const float2*>(rec + (base + lane) * part + D)) : make_float2(kShNone, 0.0f);
-                unsigned todo = __ballot_sync(0xffffffffu, has);
-                bool scaled = false;
-                float w = 0.0f;
-                while (todo) {
-                    constexpr int AT_ONCE = VEC >= 4 ? 8 : 16;  // records in flight: an L2 round trip together
-                    float v[AT_ONCE][VEC];
-                    int src[AT_ONCE];
+                for (int k = 0; k < VEC; ++k) v[u][k] = 0.0f;
+                if (src[u] >= 0) {
+                    if constexpr (VEC >= 4) {
 #pragma unroll
-                    for (int u = 0; u < AT_ONCE; ++u) {
-                        src[u] = todo ? __ffs(todo) - 1 : -1;
-                        todo &= todo - 1;
-                        const float* from = rec + (base + src[u]) * part + VEC * lane;
+                        for (int k = 0; k < VEC; k += 4)
+                            *reinterpret_cast<float4*>(&v[u][k]) = __ldcg(reinterpret_cast<const float4*>(x + k));
+                    } else {
 #pragma unroll
-                        for (int k = 0; k < VEC; ++k) v[u][k] = 0.0f;
-                        if (src[u] >= 0) {
-                            if constexpr (VEC >= 4) {
-#pragma unroll
-                                for (int k = 0; k < VEC; k += 4)
-                                    *reinterpret_cast<float4*>(&v[u][k]) = __ldcg(reinterpret_cast<const float4*>(from + k));
-                            } else {
-#pragma unroll
-                                for (int k = 0; k < VEC; ++k) v[u][k] = __ldcg(from + k);
-                            }
-                        }
-                    }
-                    if (!scaled) {  // with the records on their way
-                        float top = ul.x;
-#pragma unroll
-                        for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-                        const float U = fmaxf(M, top), f = exp2f(M - U);
-                        w = has ? exp2f(ul.x - U) : 0.0f;
-                        float l = ul.y * w;
-#pragma unroll
-                        for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
-                        M = U;
-                        sum = sum * f + l;
-#pragma unroll
-                        for (int k = 0; k < VEC; ++k) o[k] *= f;
-                        scaled = true;
-                    }
-#pragma unroll
-                    for (int u = 0; u < AT_ONCE; ++u) {
-                        const float wt = __shfl_sync(0xffffffffu, w, src[u] & 31);
-                        if (src[u] >= 0) {
-#pragma unroll
-                            for (int k = 0; k < VEC; ++k) o[k] += v[u][k] * wt;
-                        }
+                        for (int k = 0; k < VEC; ++k) v[u][k] = __ldcg(x + k);
                     }
                 }
             }
-        }
-        const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;  // no keys: zeros
+            if (!scaled) {  // with the records on their way
+                float top = ul.x;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) a.out[head * D + sh_code_dim(D, VEC * lane + k)] = __float2half_rn(o[k] * inv);
+                for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+                const float U = fmaxf(M, top), f = exp2f(M - U);
+                w = from ? exp2f(ul.x - U) : 0.0f;
+                float l = ul.y * w;
+#pragma unroll
+                for (int s = 16; s > 0; s >>= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+                M = U;
+                sum = sum * f + l;
+#pragma unroll
+                for (int k = 0; k < VEC; ++k) o[k] *= f;
+                scaled = true;
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const float wt = __shfl_sync(0xffffffffu, w, src[u] & 31);
+                if (src[u] >= 0) {
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) o[k] += v[u][k] * wt;
+                }
+            }
+        }
+    }
+    // no keys: zeros
+    if constexpr (WPR == 1) {
+        const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+        if (live) {
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) a.out[head * D + sh_code_dim(D, VEC * lane + k)] = __float2half_rn(o[k] * inv);
+        }
+    } else {
+        static_assert(WPR == kShWarps, "a CTA per row");
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) parts[warp][VEC * lane + k] = o[k];
+        if (lane == 0) {
+            marks[0][warp] = M;
+            marks[1][warp] = sum;
+        }
+        __syncthreads();
+        float f[WPR], U = kShNone, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < WPR; ++i) U = fmaxf(U, marks[0][i]);
+#pragma unroll
+        for (int i = 0; i < WPR; ++i) {
+            f[i] = exp2f(marks[0][i] - U);
+            l += marks[1][i] * f[i];
+        }
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        if (live) {
+            for (int at = threadIdx.x; at < D; at += kShThreads) {
+                float x = 0.0f;
+#pragma unroll
+                for (int i = 0; i < WPR; ++i) x += parts[i][at] * f[i];
+                a.out[head * D + sh_code_dim(D, at)] = __float2half_rn(x * inv);
+            }
+        }
     }
 }
 
@@ -704,17 +736,25 @@ int sh_workers_on_device(int* n_workers) {
     return BC_OK;
 }
 
+// Up to this many query rows the merge gives each a CTA's four warps, which share its records, else a warp.
+// One warp / four: 128 rows 14.8 / 12.2 us (the whole call), 256 rows 209 / 199, 512 rows 68.1 / 60.9; 768 rows
+// 54.7 / 58.8, 4096 rows 82 / 110, where the CTAs' sums over the list cost more than the records.
+constexpr int64_t kShSplitRows = 4 * 148;
+
 // The prefix kernel takes the prefixes when `tc` is given, else the rows kernel has both.
 template <int D, bool COMP>
 int sh_run(const SharedArgs& a, ShList& L, const ShList* tc, void* scratch, cudaStream_t st) {
     int rc = sh_workers_on_device<D, COMP>(&L.n_workers);
     if (!rc && tc) rc = sh_tc_run(a, *tc, scratch, D, COMP, st);
     if (rc) return rc;
+    const int64_t rows = (int64_t)a.n_seqs * a.n_kv * a.group;
+    const ShList& P = tc ? *tc : L;
     cudaError_t e = sh_launch(k_shared_rows<D, COMP>, (L.n_workers + kShWarps - 1) / kShWarps + (tc ? 1 : 0), kShThreads,
                               ShCfg<D, COMP>::SMEM_B, st, a, L, tc != nullptr);
     if (e == cudaSuccess)
-        e = sh_launch(k_shared_merge<D>, (int)(((int64_t)a.n_seqs * a.n_kv * a.group + kShWarps - 1) / kShWarps), kShThreads, 0,
-                      st, a, tc ? *tc : L, L, tc != nullptr);
+        e = rows <= kShSplitRows ? sh_launch(k_shared_merge<D, kShWarps>, (int)rows, kShThreads, 0, st, a, P, L, tc != nullptr)
+                                 : sh_launch(k_shared_merge<D, 1>, (int)((rows + kShWarps - 1) / kShWarps), kShThreads, 0, st, a,
+                                             P, L, tc != nullptr);
     return e == cudaSuccess ? BC_OK : BC_ERR_CUDA_BASE + (int)e;
 }
 

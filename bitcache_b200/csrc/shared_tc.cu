@@ -35,7 +35,7 @@
 // What bounds it is none of these but the chain from one tile to the next (scores,
 // softmax, P, values) with two tiles under way: about 3300 clocks a tile, and the
 // start and end of an item besides.  128 sequences with 8192 keys before them, 32 / 8
-// heads of 128: 83 us with the batch's own keys, of which the products at the tensor
+// heads of 128: 82 us with the batch's own keys, of which the products at the tensor
 // cores' rate would take 15.
 //
 // Scores are scaled so that P = 2^(s - U) lies below 2^15, U rising when it would
