@@ -76,9 +76,9 @@ struct TcCfg {
     static constexpr int RAWK_OFF = V_OFF + VST * VOP_B;
     static constexpr int RAWV_OFF = RAWK_OFF + kTcRaw * RAW_B;
     static constexpr int SCAN_OFF = (RAWV_OFF + kTcRaw * RAW_B + 15) / 16 * 16;
-    static constexpr int XCH_OFF = SCAN_OFF;  // [2][2][128] maxima of the row halves, once the sums are read
+    static constexpr int XCH_OFF = SCAN_OFF;  // [2][128] units of the rows, [128] sums, once the list's sums are read
     static constexpr int BAR_OFF = SCAN_OFF + 512 * 4;
-    static constexpr int FLAG_OFF = BAR_OFF + 36 * 8;
+    static constexpr int FLAG_OFF = BAR_OFF + 44 * 8;
     static constexpr int SMEM_B = FLAG_OFF + 20 * 4 + 1024;  // + alignment to the swizzle atom
     // tensor memory columns
     static constexpr int S_COL = 0, O_COL = 256, Q_COL = 256 + D;
@@ -87,7 +87,7 @@ struct TcCfg {
 
 enum TcBar {
     kRawKFull = 0, kRawKEmpty = 3, kRawVFull = 6, kRawVEmpty = 9, kKFull = 12, kKEmpty = 15, kVFull = 18, kVEmpty = 20,
-    kSFull = 22, kPFull = 24, kQFull = 26, kPvDone = 27, kDrain = 29, kPair = 30, kDone = 34, kTcBars = 35
+    kSFull = 22, kPFull = 24, kQFull = 26, kPvDone = 27, kDrain = 29, kPair = 30, kUnit = 34, kDone = 42, kTcBars = 43
 };
 
 // ---- tcgen05 ---------------------------------------------------------------
@@ -346,10 +346,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             mbar_init(&bar[kVFull + i], kTcUnpackWarps);
             mbar_init(&bar[kVEmpty + i], 1);
             mbar_init(&bar[kSFull + i], 1);
-            mbar_init(&bar[kPFull + i], 8);
+            mbar_init(&bar[kPFull + i], 4);
         }
         mbar_init(&bar[kQFull], 8);
-        for (int i = 0; i < 4; ++i) mbar_init(&bar[kPair + i], 2);
+        for (int i = 0; i < 4; ++i) mbar_init(&bar[kPair + i], 1);
+        for (int i = 0; i < 8; ++i) mbar_init(&bar[kUnit + i], 1);
         mbar_init(&bar[kPvDone], 1);
         mbar_init(&bar[kPvDone + 1], 1);
         mbar_init(&bar[kDrain], 1);
@@ -370,20 +371,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
     // registers: 256 x 112 + 512 x 56 + 128 x 48 of the 896 x 72 launched
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
-        // ---------------- softmax: row `rl` of the item's block, keys 64 half .. 64 half + 63 ----------------
+        // ---------------- softmax: row `rl` of the item's block, tiles i with i % 2 == half ----------------
         const int half = warp >> 2, quad = warp & 3;
-        const uint32_t lane_at = tmem + ((uint32_t)(32 * quad) << 16);
+        const uint32_t lane_at = tmem + ((uint32_t)(32 * quad) << 16), s_at = lane_at + C::S_COL + 128 * half;
         // few rows: copies of them fill the 128 lanes, and each copy takes its share of a tile's keys
-        const int copies = L.copies, copy = quad * copies >> 2, rl = 32 * quad + lane - copy * (128 / copies);
-        const int width = 64 / copies, key0 = (128 / copies) * copy + width * half;  // this warp's keys of a tile
-        float* xch = reinterpret_cast<float*>(smem + C::XCH_OFF) + 32 * quad + lane;  // [2][2][128]: parity, half, row
-        uint64_t* pair = &bar[kPair + quad];
-        uint32_t met = 0;  // exchanges with the row's other warp
+        const int copies = L.copies, copy = copies > 1 ? quad : 0, rl = 32 * quad + lane - copy * (128 / copies);
+        const int key0 = (128 / copies) * copy;  // this copy's first key of a tile
+        float* xch = reinterpret_cast<float*>(smem + C::XCH_OFF) + 32 * quad + lane;  // [2][128] units, [128] sums
         float sc = 0.0f, U = kShNone, l = 0.0f;
         sh_wait_before();
         bool ok = true;
-        for (int i = 0; ok && cur.left > 0; sh_next_piece(a, L, cur)) {
-            const int end = i + sh_piece_tiles(cur);
+        // the other warp's unit behind tile j (of this piece; its unit behind tile j - 2 has been seen)
+        auto follow = [&](int j) {
+            ok = __all_sync(0xffffffffu, tc_wait(&bar[kUnit + 2 * quad + (j & 1)], (uint32_t)(j >> 1) & 1u, dead));
+            const float U1 = xch[128 * (j & 1)];
+            l *= exp2f(U - U1);
+            U = U1;
+        };
+        for (int i = 0, piece = 0; ok && cur.left > 0; sh_next_piece(a, L, cur), ++piece) {
+            const int begin = i, end = i + sh_piece_tiles(cur);
             const int rows = a.per * a.group, r = cur.blk * L.rows + rl;
             const int64_t item = (int64_t)cur.e * a.n_kv + cur.h;
             const bool valid = rl < L.rows && r < rows, busy = __any_sync(0xffffffffu, valid);
@@ -412,149 +418,154 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             if (lane == 0) tc_arrive(&bar[kQFull]);
             U = kShNone;
             l = 0.0f;
-            int first = (cur.x.tile0 + cur.tile) * kTcTile + key0;
-            bool begin = true;
 #pragma unroll 1
-            for (; i < end; ++i, first += kTcTile, begin = false) {
-                const int b = i & 1;
-                ok = __all_sync(0xffffffffu, tc_wait(&bar[kSFull + b], (uint32_t)(i >> 1) & 1u, dead));
+            for (i += (i ^ half) & 1; i < end; i += 2) {
+                ok = __all_sync(0xffffffffu, tc_wait(&bar[kSFull + half], (uint32_t)(i >> 1) & 1u, dead));
                 if (!ok) break;
                 tc_fence_after();
                 if (busy) {
-                    const uint32_t s_at = lane_at + C::S_COL + 128 * b;
-                    const int lo = kbad[i & 7] ? 64 : cur.x.lo - first, hi = cur.x.hi - first;
+                    const int first = (cur.x.tile0 + cur.tile + i - begin) * kTcTile;
+                    const int lo = kbad[i & 7] ? kTcTile : cur.x.lo - first, hi = cur.x.hi - first;
+                    const bool cut = lo > 0 || hi < kTcTile;  // keys outside the prefix
+                    // 64 keys' scores (with copies 32), those outside the prefix -inf
                     uint32_t v[64];
-    #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (16 * c < width) tc_ld16(s_at + key0 + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(v + 16 * c));
-                    tc_wait_ld();
-                    if (lo > 0 || hi < width) {  // keys outside the prefix
-    #pragma unroll
-                        for (int k = 0; k < 64; ++k)
-                            if (k < lo || k >= hi) v[k] = 0xFF800000u;
-                    }
+                    auto scores = [&](int at) {
+                        tc_ld32(s_at + at, *reinterpret_cast<uint32_t(*)[32]>(v));
+                        if (copies == 1) tc_ld32(s_at + at + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
+                        tc_wait_ld();
+                        if (cut) {
+#pragma unroll
+                            for (int k = 0; k < 64; ++k)
+                                if (at + k < lo || at + k >= hi) v[k] = 0xFF800000u;
+                        }
+                    };
                     float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (16 * c < width) {
-    #pragma unroll
-                            for (int k = 16 * c; k < 16 * c + 16; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
+                    auto maxima = [&]() {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
+                        if (copies == 1) {
+#pragma unroll
+                            for (int k = 32; k < 64; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
                         }
-                    float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-                    xch[256 * (met & 1) + 128 * half] = top;
-                    __syncwarp();
-                    if (lane == 0) tc_arrive(pair);
-                    // P with the U of the tiles so far; the maxima, the other half's too, are looked at
-                    // afterwards, and in the rare case that U has to rise P is made once more
-                    // (with copies, the row's other warp may still read scores where this one's P and zeros go: wait)
-                    bool again = begin || copies > 1, seen = false;
-                    float tile_sum;
-    #pragma unroll 1
-                    for (;;) {
-                        float2 sum = make_float2(0.0f, 0.0f);
-                        if (!again) {
-                            const float2 sc2 = make_float2(sc, sc), U2 = make_float2(-U, -U);
-    #pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                if (16 * c >= width) continue;
-                                uint32_t p[8];
-    #pragma unroll
-                                for (int k = 0; k < 16; k += 2) {
-                                    float2 e = tc_fma2(make_float2(__uint_as_float(v[16 * c + k]), __uint_as_float(v[16 * c + k + 1])),
-                                                       sc2, U2);
-                                    e.x = exp2f(e.x);
-                                    e.y = exp2f(e.y);
-                                    sum = tc_add2(sum, e);
-                                    p[k / 2] = h2_bits(__floats2half2_rn(e.x, e.y));
-                                }
-                                // P of key k: column k / 2 of the half tile that it is in, 64 columns apart
-                                tc_st8(s_at + 64 * (key0 >> 6) + ((key0 & 63) >> 1) + 8 * c, p);
-                            }
-                            if (copies > 1) {  // the other copies' keys: P is 0
-                                uint32_t z[16] = {};
-                                tc_st16(s_at + 64 * ((key0 >> 6) ^ 1) + 16 * half, z);
-                                tc_st8(s_at + 64 * (key0 >> 6) + 16 * ((copy & 1) ^ 1) + 8 * half,
-                                       *reinterpret_cast<uint32_t(*)[8]>(z));
-                            }
-                        }
-                        tile_sum = sum.x + sum.y;
-                        if (seen) break;
-                        ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead));
-                        if (!ok) break;
-                        top = fmaxf(top, xch[256 * (met & 1) + 128 * (half ^ 1)]) * sc;
-                        const bool rise = __any_sync(0xffffffffu, top - U > 15.0f);
-                        if (!rise && !again) break;
-                        if (rise) {
-                            const float U1 = top - U > 15.0f ? top - 8.0f : U, f = exp2f(U - U1);
-                            U = U1;
-                            l *= f;
-                            if (!begin) {  // O holds the piece's tiles so far, once their products are through
-                                ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone + ((i - 1) & 1)], (uint32_t)((i - 1) >> 1) & 1u, dead));
-                                if (!ok) break;
-                                tc_fence_after();
-    #pragma unroll 1
-                                for (int c = 0; c < D / 32; ++c) {
-                                    const uint32_t at = lane_at + C::O_COL + D / 2 * half + 16 * c;
-                                    uint32_t o[16];
-                                    tc_ld16(at, o);
-                                    tc_wait_ld();
-    #pragma unroll
-                                    for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
-                                    tc_st16(at, o);
-                                }
-                            }
-                        }
-                        if (!again) tc_wait_st();  // the first P is down before the second goes over it
-                        seen = true;
-                        again = false;
+                    };
+                    scores(key0);
+                    maxima();
+                    if (copies == 1) {
+                        scores(64);
+                        maxima();
                     }
-                    if (!ok) break;
-                    ++met;
-                    l += tile_sum;
+                    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * sc;
+                    if (i > begin) {
+                        follow(i - 1);
+                        if (!ok) break;
+                    }
+                    if (__any_sync(0xffffffffu, top - U > 15.0f)) {
+                        const float U1 = top - U > 15.0f ? top - 8.0f : U, f = exp2f(U - U1);
+                        U = U1;
+                        l *= f;
+                        if (i > begin) {  // O holds the piece's tiles so far, once their products are through
+                            ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone + ((i - 1) & 1)], (uint32_t)((i - 1) >> 1) & 1u, dead));
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D / 16; ++c) {
+                                const uint32_t at = lane_at + C::O_COL + 16 * c;
+                                uint32_t o[16];
+                                tc_ld16(at, o);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * f);
+                                tc_st16(at, o);
+                            }
+                        }
+                    }
+                    xch[128 * half] = U;
+                    __syncwarp();
+                    if (lane == 0) tc_arrive(&bar[kUnit + 2 * quad + half]);
+                    float2 sum = make_float2(0.0f, 0.0f);
+                    // P of the keys in v: column k / 2 of the half tile that key k is in, 64 columns apart,
+                    // over scores that this warp has read
+                    auto weights = [&](int at, int width) {
+                        const float2 sc2 = make_float2(sc, sc), U2 = make_float2(-U, -U);
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            if (16 * c >= width) continue;
+                            uint32_t p[8];
+#pragma unroll
+                            for (int k = 0; k < 16; k += 2) {
+                                float2 e = tc_fma2(make_float2(__uint_as_float(v[16 * c + k]), __uint_as_float(v[16 * c + k + 1])),
+                                                   sc2, U2);
+                                e.x = exp2f(e.x);
+                                e.y = exp2f(e.y);
+                                sum = tc_add2(sum, e);
+                                p[k / 2] = h2_bits(__floats2half2_rn(e.x, e.y));
+                            }
+                            tc_st8(s_at + 64 * (at >> 6) + ((at & 63) >> 1) + 8 * c, p);
+                        }
+                    };
+                    if (copies == 1) {
+                        weights(64, 64);
+                        scores(0);
+                        weights(0, 64);
+                    } else {
+                        weights(key0, 32);
+                        const uint32_t z[16] = {};  // the other copies' keys: P is 0
+#pragma unroll 1
+                        for (int c = 0; c < 4; ++c)
+                            if (c != copy) tc_st16(s_at + 64 * (c >> 1) + 16 * (c & 1), z);
+                    }
+                    l += sum.x + sum.y;
                     tc_wait_st();
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc_arrive(&bar[kPFull + b]);
+                if (lane == 0) tc_arrive(&bar[kPFull + half]);
             }
-            if (ok) {
-                if (busy) {  // the row's sum: both halves'
-                    xch[256 * (met & 1) + 128 * half] = l;
-                    __syncwarp();
-                    if (lane == 0) tc_arrive(pair);
-                    ok = __all_sync(0xffffffffu, tc_wait(pair, met & 1u, dead));
+            if (!ok) break;
+            i = end;
+            const bool last = ((end - 1) & 1) == half;  // this warp had the piece's last tile
+            if (busy) {  // the row's sum: both warps'
+                if (!last) {
+                    follow(end - 1);
                     if (!ok) break;
-                    l += xch[256 * (met & 1) + 128 * (half ^ 1)];
-                    ++met;
+                    xch[256] = l;
+                    __syncwarp();
+                    if (lane == 0) tc_arrive(&bar[kPair + quad]);
+                } else {
+                    ok = __all_sync(0xffffffffu, tc_wait(&bar[kPair + quad], (uint32_t)piece & 1u, dead));
+                    if (!ok) break;
+                    l += xch[256];
                 }
-                ok = __all_sync(0xffffffffu, !busy || tc_wait(&bar[kPvDone + ((i - 1) & 1)], (uint32_t)((i - 1) >> 1) & 1u, dead));
-                if (!ok) break;
-                tc_fence_after();
-                if (busy) {
-                    float* row = sh_record(a, L, cur, blockIdx.x, D) + (copy * L.rows + rl) * (D + 4);
-                    const unsigned live = __ballot_sync(0xffffffffu, valid);
-                    // 64 columns at a time (all of them at head_dim 64: one warp each half of the rows)
+            }
+            // (the last tile but one first: its end tells that the phase before the last tile's is over)
+            for (int j = max(0, end - 2); ok && j < end; ++j)
+                ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone + (j & 1)], (uint32_t)(j >> 1) & 1u, dead));
+            if (!ok) break;
+            tc_fence_after();
+            if (busy) {
+                float* row = sh_record(a, L, cur, blockIdx.x, D) + (copy * L.rows + rl) * (D + 4);
+                const unsigned live = __ballot_sync(0xffffffffu, valid);
+                // 64 columns at a time (all of them at head_dim 64: one warp each half of the rows)
 #pragma unroll 1
-                    for (int s16 = D == 64 ? half : 0; s16 < (D == 64 ? half + 1 : 2); ++s16) {
-                        uint32_t v[32];
-                        const int col = D == 64 ? 0 : 64 * half;
-                        tc_ld_rows(lane_at + ((uint32_t)(16 * s16) << 16) + C::O_COL + col, v);
-                        tc_wait_ld();
+                for (int s16 = D == 64 ? half : 0; s16 < (D == 64 ? half + 1 : 2); ++s16) {
+                    uint32_t v[32];
+                    const int col = D == 64 ? 0 : 64 * half;
+                    tc_ld_rows(lane_at + ((uint32_t)(16 * s16) << 16) + C::O_COL + col, v);
+                    tc_wait_ld();
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const int at = 16 * s16 + 8 * y + (lane >> 2);  // the row's lane
-                            float* to = row + (at - lane) * (D + 4) + col + 2 * (lane & 3);
-                            if (live >> at & 1) {
+                    for (int y = 0; y < 2; ++y) {
+                        const int at = 16 * s16 + 8 * y + (lane >> 2);  // the row's lane
+                        float* to = row + (at - lane) * (D + 4) + col + 2 * (lane & 3);
+                        if (live >> at & 1) {
 #pragma unroll
-                                for (int j = 0; j < 8; ++j)
-                                    *reinterpret_cast<uint2*>(to + 8 * j) = make_uint2(v[4 * j + 2 * y], v[4 * j + 2 * y + 1]);
-                            }
+                            for (int j = 0; j < 8; ++j)
+                                *reinterpret_cast<uint2*>(to + 8 * j) = make_uint2(v[4 * j + 2 * y], v[4 * j + 2 * y + 1]);
                         }
                     }
-                    if (valid && half == 0) *reinterpret_cast<float2*>(row + D) = make_float2(U, l);
                 }
-                tc_fence_before();
+                if (valid && last) *reinterpret_cast<float2*>(row + D) = make_float2(U, l);
             }
+            tc_fence_before();
         }
         tc_leave(&bar[kDone]);
         return;
