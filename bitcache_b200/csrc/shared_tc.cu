@@ -10,42 +10,47 @@
 // (f carries what the rounding of the row's mean would lose).  V = bs sgn v + rs/7 n.
 //
 // Roles of the 28 warps of a CTA, one CTA per SM:
-//   0-7    softmax: a thread owns a query row and half of a tile's keys (warps 0-3
-//          keys 0-63, 4-7 the others; the two warps of a row exchange maxima).
-//          Writes the row's Q (made by k_shared_queries) into tensor memory, then per
-//          tile reads its scores, keeps U and l, writes P (fp16, over the scores) and,
-//          when U moves, rescales O.  Up to 32 rows stand four times in the 128 lanes,
-//          each copy with a quarter of the tile's keys; the copies are joined with the
-//          pieces.
-//   8-23   unpack: packed bytes -> fp16 operand rows in shared memory, two threads
-//          to a key.  K on the first two schedulers, K-major (128-byte swizzle,
-//          blocks of 64 elements); V on the other two, MN-major (dims contiguous).
-//          Each scheduler so has two instruction streams, not three; with fully
-//          unrolled bodies and all three on each, waiting for instructions took
-//          more than everything else (13600 clocks a tile, 4200 with rolled loops).
+//   0-7    softmax: a thread owns a query row and half of every tile's keys (warps 0-3
+//          keys 0-63, 4-7 the others).  Writes the row's Q (made by k_shared_queries)
+//          into tensor memory, then per tile reads its scores, keeps U and l, writes P
+//          (fp16, over the scores) and, when U moves, rescales O.  The two warps of a
+//          row hand U on from one half tile to the next, so a half's maximum is known
+//          before its weights are made and its values can go before the other's are
+//          there (with maxima exchanged at every tile, one warp's waits were both's:
+//          81.8 us instead of 78.2 in the case below).  Up to 32 rows stand four times
+//          in the 128 lanes, each copy with a quarter of a half's keys; the copies are
+//          joined with the pieces.
+//   8-23   unpack: packed bytes -> fp16 operand rows in shared memory, two threads to a
+//          key, 8-11 and 16-19 K, the others V.  K is K-major (128-byte swizzle, blocks
+//          of 64 elements), V MN-major (dims contiguous).  The loops are rolled: fully
+//          unrolled, waiting for instructions took more than everything else (13600
+//          clocks a tile).
 //   24     issues the products: Q (tensor memory) x K, P (tensor memory) x V.
 //   25, 26 bring K's / V's packed tiles with 1-D bulk copies, three ahead.
 //   27     fills the last warpgroup.
 // K's operand ring holds three half tiles (the sign part, the code part), V's two
 // tiles.
+//
 // Keeping Q in tensor memory spares half of the score product's shared-memory
 // reads.  Per tile 96 KB are written, 96 KB read by the tensor cores and 43 KB of
 // packed bytes go in and out, 1900 clocks at 128 B each; the products take 1536, the
-// exponentials of 128 rows 1024, the unpacking about 800 issue slots a scheduler.
-// What bounds it is none of these but the chain from one tile to the next (scores,
-// softmax, P, values) with two tiles under way: about 3300 clocks a tile, and the
-// start and end of an item besides.  128 sequences with 8192 keys before them, 32 / 8
-// heads of 128: 82 us with the batch's own keys, of which the products at the tensor
-// cores' rate would take 15.
+// exponentials of 128 rows 1024.  What bounds it is the instructions of all roles,
+// about 2500 issue slots of a scheduler and tile (half of them unpacking), and the
+// chain from a tile's scores to the ones two tiles later in the same buffer: some
+// 3300 clocks a tile, and the start and end of an item besides.  128 sequences with
+// 8192 keys before them, 32 / 8 heads of 128: 78 us with the batch's own keys, of
+// which the products at the tensor cores' rate would take 15.  (Score products of 64
+// keys, with four buffers, take as long each as those of 128: 229 us where these
+// take 195, 32 rows before 200000 keys.)
 //
 // Scores are scaled so that P = 2^(s - U) lies below 2^15, U rising when it would
 // not, to 2^8 above the largest; the elements of K, V, Q and P are rounded to fp16
 // once each, sums are fp32.
 //
 // A barrier tells odd phases from even ones, no more: whoever waits on one has to
-// know that the phase before is over.  The value products have two in turn, because
-// the scores of tile i tell (the tensor cores work in order) that the values of
-// tile i - 2 are through, which is the phase before that of tile i.
+// know that the phase before is over.  The value products have four in turn, one
+// for each half tile, because the scores of tile i tell (the tensor cores work in
+// order) that the values of tile i - 2 are through.
 #include "shared.cuh"
 #include "shared_tc.h"
 
@@ -78,7 +83,7 @@ struct TcCfg {
     static constexpr int SCAN_OFF = (RAWV_OFF + kTcRaw * RAW_B + 15) / 16 * 16;
     static constexpr int XCH_OFF = SCAN_OFF;  // [2][128] units of the rows, [128] sums, once the list's sums are read
     static constexpr int BAR_OFF = SCAN_OFF + 512 * 4;
-    static constexpr int FLAG_OFF = BAR_OFF + 44 * 8;
+    static constexpr int FLAG_OFF = BAR_OFF + 50 * 8;
     static constexpr int SMEM_B = FLAG_OFF + 20 * 4 + 1024;  // + alignment to the swizzle atom
     // tensor memory columns
     static constexpr int S_COL = 0, O_COL = 256, Q_COL = 256 + D;
@@ -87,7 +92,7 @@ struct TcCfg {
 
 enum TcBar {
     kRawKFull = 0, kRawKEmpty = 3, kRawVFull = 6, kRawVEmpty = 9, kKFull = 12, kKEmpty = 15, kVFull = 18, kVEmpty = 20,
-    kSFull = 22, kPFull = 24, kQFull = 26, kPvDone = 27, kDrain = 29, kPair = 30, kUnit = 34, kDone = 42, kTcBars = 43
+    kSFull = 22, kPFull = 26, kPvDone = 30, kQFull = 34, kDrain = 35, kPair = 36, kUnit = 40, kDone = 48, kTcBars = 49
 };
 
 // ---- tcgen05 ---------------------------------------------------------------
@@ -345,14 +350,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar[kVFull + i], kTcUnpackWarps);
             mbar_init(&bar[kVEmpty + i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&bar[kSFull + i], 1);
             mbar_init(&bar[kPFull + i], 4);
+            mbar_init(&bar[kPvDone + i], 1);
+            mbar_init(&bar[kPair + i], 1);
         }
         mbar_init(&bar[kQFull], 8);
-        for (int i = 0; i < 4; ++i) mbar_init(&bar[kPair + i], 1);
         for (int i = 0; i < 8; ++i) mbar_init(&bar[kUnit + i], 1);
-        mbar_init(&bar[kPvDone], 1);
-        mbar_init(&bar[kPvDone + 1], 1);
         mbar_init(&bar[kDrain], 1);
         mbar_init(&bar[kDone], kTcThreads / 32 - 1);
         fence_mbar_init();
@@ -371,17 +377,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
     // registers: 256 x 112 + 512 x 56 + 128 x 48 of the 896 x 72 launched
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
-        // ---------------- softmax: row `rl` of the item's block, tiles i with i % 2 == half ----------------
+        // ---------------- softmax: row `rl` of the item's block, keys 64 half .. of every tile ----------------
         const int half = warp >> 2, quad = warp & 3;
-        const uint32_t lane_at = tmem + ((uint32_t)(32 * quad) << 16), s_at = lane_at + C::S_COL + 128 * half;
-        // few rows: copies of them fill the 128 lanes, and each copy takes its share of a tile's keys
+        const uint32_t lane_at = tmem + ((uint32_t)(32 * quad) << 16);
+        // few rows: copies of them fill the 128 lanes, and each copy takes its share of a half tile's keys
         const int copies = L.copies, copy = copies > 1 ? quad : 0, rl = 32 * quad + lane - copy * (128 / copies);
-        const int key0 = (128 / copies) * copy;  // this copy's first key of a tile
+        const int key0 = 64 / copies * copy;  // this copy's first key of a half tile
         float* xch = reinterpret_cast<float*>(smem + C::XCH_OFF) + 32 * quad + lane;  // [2][128] units, [128] sums
         float sc = 0.0f, U = kShNone, l = 0.0f;
         sh_wait_before();
         bool ok = true;
-        // the other warp's unit behind tile j (of this piece; its unit behind tile j - 2 has been seen)
+        // the row's other warp's unit behind half tile j (of this piece; that behind j - 2 has been seen)
         auto follow = [&](int j) {
             ok = __all_sync(0xffffffffu, tc_wait(&bar[kUnit + 2 * quad + (j & 1)], (uint32_t)(j >> 1) & 1u, dead));
             const float U1 = xch[128 * (j & 1)];
@@ -419,52 +425,45 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             U = kShNone;
             l = 0.0f;
 #pragma unroll 1
-            for (i += (i ^ half) & 1; i < end; i += 2) {
-                ok = __all_sync(0xffffffffu, tc_wait(&bar[kSFull + half], (uint32_t)(i >> 1) & 1u, dead));
+            for (; i < end; ++i) {
+                const int t = 2 * i + half;
+                ok = __all_sync(0xffffffffu, tc_wait(&bar[kSFull + (i & 1)], (uint32_t)(i >> 1) & 1u, dead));
                 if (!ok) break;
                 tc_fence_after();
                 if (busy) {
-                    const int first = (cur.x.tile0 + cur.tile + i - begin) * kTcTile;
-                    const int lo = kbad[i & 7] ? kTcTile : cur.x.lo - first, hi = cur.x.hi - first;
-                    const bool cut = lo > 0 || hi < kTcTile;  // keys outside the prefix
-                    // 64 keys' scores (with copies 32), those outside the prefix -inf
-                    uint32_t v[64];
-                    auto scores = [&](int at) {
-                        tc_ld32(s_at + at, *reinterpret_cast<uint32_t(*)[32]>(v));
-                        if (copies == 1) tc_ld32(s_at + at + 32, *reinterpret_cast<uint32_t(*)[32]>(v + 32));
-                        tc_wait_ld();
-                        if (cut) {
-#pragma unroll
-                            for (int k = 0; k < 64; ++k)
-                                if (at + k < lo || at + k >= hi) v[k] = 0xFF800000u;
-                        }
-                    };
-                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    auto maxima = [&]() {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
-                        if (copies == 1) {
-#pragma unroll
-                            for (int k = 32; k < 64; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
-                        }
-                    };
-                    scores(key0);
-                    maxima();
+                    const uint32_t s_at = lane_at + C::S_COL + 64 * (t & 3);
+                    const int first = (cur.x.tile0 + cur.tile + i - begin) * kTcTile + 64 * half + key0;
+                    const int lo = kbad[i & 7] ? 64 : cur.x.lo - first, hi = cur.x.hi - first;
+                    uint32_t v[64];  // (with copies, 16 of them)
+                    tc_ld16(s_at + key0, *reinterpret_cast<uint32_t(*)[16]>(v));
                     if (copies == 1) {
-                        scores(64);
-                        maxima();
+#pragma unroll
+                        for (int c = 1; c < 4; ++c) tc_ld16(s_at + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(v + 16 * c));
+                    }
+                    tc_wait_ld();
+                    if (lo > 0 || hi < 64) {  // keys outside the prefix
+#pragma unroll
+                        for (int k = 0; k < 64; ++k)
+                            if (k < lo || k >= hi) v[k] = 0xFF800000u;
+                    }
+                    float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
+                    if (copies == 1) {
+#pragma unroll
+                        for (int k = 16; k < 64; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
                     }
                     const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * sc;
-                    if (i > begin) {
-                        follow(i - 1);
+                    if (t > 2 * begin) {
+                        follow(t - 1);
                         if (!ok) break;
                     }
                     if (__any_sync(0xffffffffu, top - U > 15.0f)) {
                         const float U1 = top - U > 15.0f ? top - 8.0f : U, f = exp2f(U - U1);
                         U = U1;
                         l *= f;
-                        if (i > begin) {  // O holds the piece's tiles so far, once their products are through
-                            ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone + ((i - 1) & 1)], (uint32_t)((i - 1) >> 1) & 1u, dead));
+                        if (t > 2 * begin) {  // O holds the piece's keys so far, once their products are through
+                            ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone + ((t - 1) & 3)], (uint32_t)((t - 1) >> 2) & 1u, dead));
                             if (!ok) break;
                             tc_fence_after();
 #pragma unroll 1
@@ -482,51 +481,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     xch[128 * half] = U;
                     __syncwarp();
                     if (lane == 0) tc_arrive(&bar[kUnit + 2 * quad + half]);
+                    // P of key k: column k / 2 of the half tile's, over scores that this warp has read
                     float2 sum = make_float2(0.0f, 0.0f);
-                    // P of the keys in v: column k / 2 of the half tile that key k is in, 64 columns apart,
-                    // over scores that this warp has read
-                    auto weights = [&](int at, int width) {
-                        const float2 sc2 = make_float2(sc, sc), U2 = make_float2(-U, -U);
+                    const float2 sc2 = make_float2(sc, sc), U2 = make_float2(-U, -U);
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            if (16 * c >= width) continue;
-                            uint32_t p[8];
+                    for (int c = 0; c < 4; ++c) {
+                        if (c > 0 && copies > 1) continue;
+                        uint32_t p[8];
 #pragma unroll
-                            for (int k = 0; k < 16; k += 2) {
-                                float2 e = tc_fma2(make_float2(__uint_as_float(v[16 * c + k]), __uint_as_float(v[16 * c + k + 1])),
-                                                   sc2, U2);
-                                e.x = exp2f(e.x);
-                                e.y = exp2f(e.y);
-                                sum = tc_add2(sum, e);
-                                p[k / 2] = h2_bits(__floats2half2_rn(e.x, e.y));
-                            }
-                            tc_st8(s_at + 64 * (at >> 6) + ((at & 63) >> 1) + 8 * c, p);
+                        for (int k = 0; k < 16; k += 2) {
+                            float2 e = tc_fma2(make_float2(__uint_as_float(v[16 * c + k]), __uint_as_float(v[16 * c + k + 1])),
+                                               sc2, U2);
+                            e.x = exp2f(e.x);
+                            e.y = exp2f(e.y);
+                            sum = tc_add2(sum, e);
+                            p[k / 2] = h2_bits(__floats2half2_rn(e.x, e.y));
                         }
-                    };
-                    if (copies == 1) {
-                        weights(64, 64);
-                        scores(0);
-                        weights(0, 64);
-                    } else {
-                        weights(key0, 32);
-                        const uint32_t z[16] = {};  // the other copies' keys: P is 0
+                        tc_st8(s_at + (key0 >> 1) + 8 * c, p);
+                    }
+                    if (copies > 1) {  // the other copies' keys: P is 0
+                        const uint32_t z[8] = {};
 #pragma unroll 1
                         for (int c = 0; c < 4; ++c)
-                            if (c != copy) tc_st16(s_at + 64 * (c >> 1) + 16 * (c & 1), z);
+                            if (c != copy) tc_st8(s_at + 8 * c, z);
                     }
                     l += sum.x + sum.y;
                     tc_wait_st();
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc_arrive(&bar[kPFull + half]);
+                if (lane == 0) tc_arrive(&bar[kPFull + (t & 3)]);
             }
             if (!ok) break;
-            i = end;
-            const bool last = ((end - 1) & 1) == half;  // this warp had the piece's last tile
-            if (busy) {  // the row's sum: both warps'
-                if (!last) {
-                    follow(end - 1);
+            if (busy) {  // the row's sum: both warps', in the unit of the piece's last keys, half 1's
+                if (half == 0) {
+                    follow(2 * end - 1);
                     if (!ok) break;
                     xch[256] = l;
                     __syncwarp();
@@ -537,9 +526,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     l += xch[256];
                 }
             }
-            // (the last tile but one first: its end tells that the phase before the last tile's is over)
-            for (int j = max(0, end - 2); ok && j < end; ++j)
-                ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone + (j & 1)], (uint32_t)(j >> 1) & 1u, dead));
+            // (the last half tile but one first: its end tells that the phase before the last one's is over)
+            for (int j = 2 * end - 2; ok && j < 2 * end; ++j)
+                ok = __all_sync(0xffffffffu, tc_wait(&bar[kPvDone + (j & 3)], (uint32_t)(j >> 2) & 1u, dead));
             if (!ok) break;
             tc_fence_after();
             if (busy) {
@@ -563,7 +552,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                         }
                     }
                 }
-                if (valid && last) *reinterpret_cast<float2*>(row + D) = make_float2(U, l);
+                if (valid && half == 1) *reinterpret_cast<float2*>(row + D) = make_float2(U, l);
             }
             tc_fence_before();
         }
@@ -712,19 +701,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             const uint32_t one = tc_elect();
             const uint64_t kd = tc_desc(smem_u32(smem), 16), vd = tc_desc(smem_u32(smem + C::V_OFF), kTcTile * 128);
             bool ok = true;
-            auto values = [&](int j, bool first) {  // O (+)= P(j) V(j)
-                ok = __all_sync(0xffffffffu, ok && tc_wait(&bar[kPFull + (j & 1)], (uint32_t)(j >> 1) & 1u, dead) &&
-                                                 tc_wait(&bar[kVFull + j % C::VST], (uint32_t)(j / C::VST) & 1u, dead));
+            auto values = [&](int t, bool first) {  // O (+)= P V of half tile t
+                const int j = t >> 1, h = t & 1;
+                ok = __all_sync(0xffffffffu, ok && tc_wait(&bar[kPFull + (t & 3)], (uint32_t)(t >> 2) & 1u, dead) &&
+                                                 (h || tc_wait(&bar[kVFull + j % C::VST], (uint32_t)(j / C::VST) & 1u, dead)));
                 if (!ok) return;
                 tc_fence_after();
-                const uint64_t at = vd + (j % C::VST) * (C::VOP_B >> 4);
-                const uint32_t p = tmem + C::S_COL + 128 * (j & 1);
+                const uint64_t at = vd + (j % C::VST) * (C::VOP_B >> 4) + (2048 >> 4) * 4 * h;
+                const uint32_t p = tmem + C::S_COL + 64 * (t & 3);
 #pragma unroll
-                for (int k = 0; k < kTcTile / 16; ++k)
-                    tc_mma(tmem + C::O_COL, p + 8 * k + 32 * (k >> 2), at + (2048 >> 4) * k, tc_idesc(D, true), !first || k > 0,
-                           one);
-                tc_commit(&bar[kVEmpty + j % C::VST], one);
-                tc_commit(&bar[kPvDone + (j & 1)], one);
+                for (int k = 0; k < 4; ++k)
+                    tc_mma(tmem + C::O_COL, p + 8 * k, at + (2048 >> 4) * k, tc_idesc(D, true), !first || k > 0, one);
+                if (h) tc_commit(&bar[kVEmpty + j % C::VST], one);
+                tc_commit(&bar[kPvDone + (t & 3)], one);
             };
             int i = 0, slot = 0;
             uint32_t round = 0;
@@ -757,7 +746,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                         if (!ok) break;
                         tc_commit(&bar[kSFull + b], one);
                     }
-                    if (i > from) values(i - 1, i - 1 == from);
+                    if (i > from) {
+                        values(2 * i - 2, i - 1 == from);
+                        values(2 * i - 1, false);
+                    }
                 }
                 i = end;
             }
@@ -859,9 +851,9 @@ ShList sh_tc_list(int n_seqs, int n_groups, int group) {
     L.pre_blocks = (int)((rows + 127) / 128);
     L.rows = (int)((rows + L.pre_blocks - 1) / L.pre_blocks);
     L.rows = (L.rows + 7) / 8 * 8;
-    // Up to 32 rows: four copies of the rows, each with a quarter of a tile's keys, so that all softmax lanes
-    // work (32 rows and 200000 keys: 212 us, 227 with one copy).  Two copies of 33 to 64 rows cost more than
-    // they spare (64 rows, 32768 keys: 70.4 us, 68.8 with one): the tile's chain of waits is then the longer.
+    // Up to 32 rows: four copies of the rows, each with a quarter of the keys, so that all softmax lanes work
+    // (32 rows: 195 us at 200000 keys, 203 with one copy; 59.8 and 58.4 at 32768).  Two copies of 33 to 64 rows
+    // cost more than they spare.
     L.copies = L.rows <= 32 ? 4 : 1;
     L.own_blocks = 1;
     L.shift = 7;
