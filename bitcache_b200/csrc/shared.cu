@@ -32,6 +32,11 @@
 // rounded to fp16.  They keep at least 11 significant bits down to 2^-22 of a
 // row's largest one: e is 2^(s - U) with U such that the largest P lies between
 // 2^8 and 2^15.
+//
+// What bounds it is a tile's chain (copies, scores, weights, values) in each warp
+// and the instructions of building A, not HBM: 128 sequences of 16 prompts up to 4000
+// keys, 16 heads of 64, take 45 us (77 MB: 1.7 TB/s), 48 ragged sequences up to 6000
+// keys, sign bits only, 8 heads of 256, 55 us (75 MB: 1.4 TB/s).
 #include "shared.cuh"
 #include "shared_tc.h"
 

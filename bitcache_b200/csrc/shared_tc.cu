@@ -5,9 +5,9 @@
 // tensor-memory lane) against a prefix, in tiles of 128 keys (N of the scores, K
 // of the values).  A score needs two dots, sgn q . sgn k and q . n, with scales of
 // the key's own, so K holds both parts side by side, scaled, and Q likewise:
-//   K = [ bs sgn k | rs / 8 n ],  Q = [ h sgn q | 8 / 7 q / f ],  h = fp16(mean|q|),
-//   f = mean|q| / h:  s = f Q . K
-// (f carries what the rounding of the row's mean would lose).  V = bs sgn v + rs/7 n.
+//   K = [ bs sgn k | rs / 8 n ],  Q = [ h sgn q | q ] / 2^e,  h = fp16(7 / 8 mean|q|):
+//   s = 8 / 7 2^e Q . K,  2^e <= mean|q| < 2^(e + 1), so that Q is exact but for h.
+// (Without codes Q is sgn q, and s = mean|q| Q . K.)  V = bs sgn v + rs/7 n.
 //
 // Roles of the 28 warps of a CTA, one CTA per SM:
 //   0-7    softmax: a thread owns a query row and half of every tile's keys (warps 0-3
@@ -44,8 +44,12 @@
 // take 195, 32 rows before 200000 keys.)
 //
 // Scores are scaled so that P = 2^(s - U) lies below 2^15, U rising when it would
-// not, to 2^8 above the largest; the elements of K, V, Q and P are rounded to fp16
-// once each, sums are fp32.
+// not, to 2^8 above the largest.  Sums are fp32.  The elements of K, V and P, h and
+// V's rs / 7 are rounded to fp16, the widest type that the tensor cores take at this
+// rate: with some channels four times the others, outputs are 5.0e-4 off the exact
+// ones, relative, of which their own fp16 rounding is 2.1e-4 and the five others 1.5e-4
+// to 2.8e-4 each, none of them by itself worth the instructions that would spare it.
+// The rows kernel, which scales products in fp32 and rounds P alone, has 2.9e-4.
 //
 // A barrier tells odd phases from even ones, no more: whoever waits on one has to
 // know that the phase before is over.  The value products have four in turn, one
@@ -296,10 +300,12 @@ __global__ void __launch_bounds__(32 * kTcQueryWarps) k_shared_queries(const Sha
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mag += __shfl_xor_sync(0xffffffffu, mag, o);
     const float mean = mag * (1.0f / D);
-    const __half h = __float2half_rn(mean);
-    const float hf = __half2float(h), f = hf == 0.0f ? 1.0f : mean / hf, g = (8.0f / 7.0f) / f;
-    if (lane == 0) scales[item * rows + r] = f * kShLog2e * rsqrtf((float)D);
-    const uint32_t hb = __half_as_ushort(h);
+    const int e = mean != 0.0f ? (__float_as_int(mean) >> 23 & 255) - 127 : 0;
+    const float down = mean < INFINITY ? __int_as_float((127 - e) << 23) : NAN;
+    if (lane == 0)
+        scales[item * rows + r] =
+            (COMP ? 8.0f / 7.0f * __int_as_float((127 + e) << 23) : mean) * kShLog2e * rsqrtf((float)D);
+    const uint32_t hb = __half_as_ushort(__float2half_rn(COMP ? mean * down * 0.875f : mean < INFINITY ? 1.0f : NAN));
 #pragma unroll
     for (int k = 0; k < D / 64; ++k) {
         const int c = 32 * k + lane, d0 = 32 * (c / 16) + c % 16;
@@ -307,7 +313,7 @@ __global__ void __launch_bounds__(32 * kTcQueryWarps) k_shared_queries(const Sha
                                                   ((hb | (__half2float(x[d0 + 16]) >= 0.0f ? 0u : 0x8000u)) << 16);
         if constexpr (COMP)
             op[(int64_t)(D / 8 + c / 4) * rows * 4 + c % 4] =
-                h2_bits(__floats2half2_rn(__half2float(x[sh_code_dim(D, 2 * c)]) * g, __half2float(x[sh_code_dim(D, 2 * c + 1)]) * g));
+                h2_bits(__floats2half2_rn(__half2float(x[sh_code_dim(D, 2 * c)]) * down, __half2float(x[sh_code_dim(D, 2 * c + 1)]) * down));
     }
 }
 
