@@ -17,7 +17,7 @@
 //          row hand U on from one half tile to the next, so a half's maximum is known
 //          before its weights are made and its values can go before the other's are
 //          there (with maxima exchanged at every tile, one warp's waits were both's:
-//          81.8 us instead of 78.2 in the case below).  Up to 32 rows stand four times
+//          82 us instead of 78 in the case below).  Up to 32 rows stand four times
 //          in the 128 lanes, each copy with a quarter of a half's keys; the copies are
 //          joined with the pieces.
 //   8-23   unpack: packed bytes -> fp16 operand rows in shared memory, two threads to a
@@ -38,7 +38,7 @@
 // about 2500 issue slots of a scheduler and tile (half of them unpacking), and the
 // chain from a tile's scores to the ones two tiles later in the same buffer: some
 // 3300 clocks a tile, and the start and end of an item besides.  128 sequences with
-// 8192 keys before them, 32 / 8 heads of 128: 78 us with the batch's own keys, of
+// 8192 keys before them, 32 / 8 heads of 128: 74 us with the batch's own keys, of
 // which the products at the tensor cores' rate would take 15.  (Score products of 64
 // keys, with four buffers, take as long each as those of 128: 229 us where these
 // take 195, 32 rows before 200000 keys.)
@@ -130,18 +130,6 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 columns of the warp's 32 lanes: lane's row, one register per column.
-__device__ __forceinline__ void tc_ld32(uint32_t addr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(addr)
-        : "memory");
-}
 // 64 columns of 16 lanes: lane t gets columns 8 j + 2 (t % 4), + 1 of rows t / 4 (r[4 j], r[4 j + 1]) and
 // t / 4 + 8, so that four lanes hold 32 consecutive bytes of a row.
 __device__ __forceinline__ void tc_ld_rows(uint32_t addr, uint32_t (&r)[32]) {
@@ -273,11 +261,11 @@ __device__ __forceinline__ float2 tc_add2(float2 x, float2 y) {
     return *reinterpret_cast<float2*>(&r);
 }
 
-// The query rows as A operands, one warp a row: [h sgn q | 8/7 q / f] in the order
-// of K's elements, and the scale of the row's scores in log2 units.  Ordered as the
+// The query rows as A operands, one warp a row: [h sgn q | q] / 2^e in the order of
+// K's elements, and the scale of the row's scores in log2 units.  Ordered as the
 // prefix kernel's lanes read them: by group and kv head, then 16-byte unit, then
-// row.  A kernel of its own: a softmax thread that made its row itself ran some 800 instructions
-// once, at the pace of their fetch (12000 clocks a piece).
+// row.  A kernel of its own: a softmax thread that made its row itself ran some 800
+// instructions once, at the pace of their fetch (12000 clocks a piece).
 constexpr int kTcQueryWarps = 8;
 template <int D, bool COMP>
 __global__ void __launch_bounds__(32 * kTcQueryWarps) k_shared_queries(const SharedArgs a, uint32_t* __restrict__ ops,
@@ -285,15 +273,16 @@ __global__ void __launch_bounds__(32 * kTcQueryWarps) k_shared_queries(const Sha
     constexpr int WORDS = (COMP ? 2 : 1) * D / 2;
     sh_wait_before();
     sh_let_next();
-    const int64_t head = (int64_t)blockIdx.x * kTcQueryWarps + (threadIdx.x >> 5), slot = head / a.group;
-    const int lane = threadIdx.x & 31, b = (int)(slot / a.n_kv);
+    // (unsigned: the heads of all sequences are below 2^31)
+    const unsigned head = blockIdx.x * kTcQueryWarps + (threadIdx.x >> 5), slot = head / (unsigned)a.group;
+    const int lane = threadIdx.x & 31, b = (int)(slot / (unsigned)a.n_kv);
     if (b >= a.n_seqs) return;
     // query row r of (group of sequences, kv head) `item`, of `rows`
     const int rows = a.per * a.group, seq = b % a.per;
-    const int64_t item = (int64_t)(b / a.per) * a.n_kv + (slot - (int64_t)b * a.n_kv);
+    const int64_t item = (int64_t)(b / a.per) * a.n_kv + (slot - (unsigned)b * a.n_kv);
     const int r = seq * a.group + (int)(head - slot * a.group);
     uint32_t* op = ops + item * rows * WORDS + 4 * r;
-    const __half* x = a.q + head * D;
+    const __half* x = a.q + (int64_t)head * D;
     float mag = 0.0f;
 #pragma unroll
     for (int k = 0; k < D / 32; ++k) mag += fabsf(__half2float(x[32 * k + lane]));
