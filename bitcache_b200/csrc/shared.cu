@@ -745,8 +745,8 @@ int sh_workers_on_device(int* n_workers) {
 }
 
 // Up to this many query rows the merge gives each a CTA's four warps, which share its records, else a warp.
-// One warp / four: 128 rows 14.8 / 12.2 us (the whole call), 256 rows 209 / 199, 512 rows 68.1 / 60.9; 768 rows
-// 54.7 / 58.8, 4096 rows 82 / 110, where the CTAs' sums over the list cost more than the records.
+// One warp / four: 128 rows 16.1 / 12.2 us (the whole call), 256 rows 213 / 194, 512 rows 65.2 / 58.4; 768 rows
+// 54.9 / 58.9, 4096 rows 74.2 / 105.8, where the CTAs' sums over the list cost more than the records.
 constexpr int64_t kShSplitRows = 4 * 148;
 
 // The prefix kernel takes the prefixes when `tc` is given, else the rows kernel has both.
@@ -769,8 +769,8 @@ int sh_run(const SharedArgs& a, ShList& L, const ShList* tc, void* scratch, cuda
 bool sh_head_dim(int d) { return d == 32 || d == 64 || d == 128 || d == 256; }
 
 // More query rows than this behind one prefix: the prefix kernel, else the rows kernel, which reads the
-// prefix once per 8 rows.  At 65536 keys, rows kernel against prefix kernel: 16 rows 71.6 / 87.3 us, 20 rows
-// 89.6 / 87.2, 32 rows 111.5 / 88.3.  (Up to 8192 keys 32 rows too are still 5 us faster there, but lengths
+// prefix once per 8 rows.  At 65536 keys, rows kernel against prefix kernel: 16 rows 58.3 / 77.8 us, 20 rows
+// 81.0 / 78.7, 32 rows 103.8 / 80.4.  (Up to 8192 keys 32 rows too are still 7 us faster there, but lengths
 // are on the device.)
 constexpr int kShTcRows = 16;
 bool sh_takes_tc(int n_seqs, int n_groups, int group, int head_dim) {
