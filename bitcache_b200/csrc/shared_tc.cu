@@ -54,7 +54,11 @@
 // A barrier tells odd phases from even ones, no more: whoever waits on one has to
 // know that the phase before is over.  The value products have four in turn, one
 // for each half tile, because the scores of tile i tell (the tensor cores work in
-// order) that the values of tile i - 2 are through.
+// order) that the values of tile i - 2 are through.  And since a row's two warps count
+// tiles and pieces alike, whether they have rows in them or not (the last block of a kv
+// head may fill fewer warps than the others), they arrive on each other's barriers for
+// every one.  Those without rows do not wait there: that the phases before are over
+// is known from the end of the values of a piece, which both warps have given their P.
 #include "shared.cuh"
 #include "shared_tc.h"
 
@@ -502,6 +506,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     }
                     l += sum.x + sum.y;
                     tc_wait_st();
+                } else if (lane == 0) {
+                    tc_arrive(&bar[kUnit + 2 * quad + half]);  // (kUnit and kPair count every tile and piece)
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -520,6 +526,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     if (!ok) break;
                     l += xch[256];
                 }
+            } else if (half == 0 && lane == 0) {
+                tc_arrive(&bar[kPair + quad]);
             }
             // (the last half tile but one first: its end tells that the phase before the last one's is over)
             for (int j = 2 * end - 2; ok && j < 2 * end; ++j)

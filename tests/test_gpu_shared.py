@@ -394,3 +394,16 @@ def test_refusals(cuda):
     assert call(b.q[:0], b.K, b.V, planes.PageTable(b.pt.pages[:0], 128, b.pt.n_pages), lens[:0]).shape == (0, 4, 128)
     b.check()
     assert _lib.device_error() == 0
+
+
+# Row counts whose last block of a kv head fills fewer of the prefix kernel's warps than the ones before it, and
+# prefixes and heads at which its CTAs go on from such a block to a whole one (odd and even numbers of tiles).
+@pytest.mark.parametrize("d,comp", [(128, True), (128, False), (64, True), (64, False)])
+@pytest.mark.parametrize("n,group,hkv,groups,prefix", [
+    (33, 4, 32, 1, 780), (34, 4, 32, 1, 1700), (80, 4, 32, 1, 650), (99, 4, 32, 1, 1040), (100, 4, 32, 1, 1290),
+    (17, 8, 32, 1, 2300), (33, 4, 8, 1, 8192), (66, 4, 16, 2, 1700),
+])
+def test_blocks_that_fill_fewer_warps(cuda, n, group, hkv, groups, prefix, d, comp):
+    lens = [prefix + 1 + (7 * i) % 30 for i in range(n)]
+    Batch(cuda, lens, [prefix - 40 * i for i in range(groups)], hkv, group, d, comp, 128, seed=n + d).check()
+    assert _lib.device_error() == 0
