@@ -8,6 +8,7 @@
 //   K = [ bs sgn k | rs / 8 n ],  Q = [ h sgn q | q ] / 2^e,  h = fp16(7 / 8 mean|q|):
 //   s = 8 / 7 2^e Q . K,  2^e <= mean|q| < 2^(e + 1), so that Q is exact but for h.
 // (Without codes Q is sgn q, and s = mean|q| Q . K.)  V = bs sgn v + rs/7 n.
+// A row of zeros has Q = 0 and a factor above 0, so that hidden keys' -inf stays -inf.
 //
 // Roles of the 28 warps of a CTA, one CTA per SM:
 //   0-7    softmax: a thread owns a query row and half of every tile's keys (warps 0-3
@@ -297,8 +298,8 @@ __global__ void __launch_bounds__(32 * kTcQueryWarps) k_shared_queries(const Sha
     const float down = mean < INFINITY ? __int_as_float((127 - e) << 23) : NAN;
     if (lane == 0)
         scales[item * rows + r] =
-            (COMP ? 8.0f / 7.0f * __int_as_float((127 + e) << 23) : mean) * kShLog2e * rsqrtf((float)D);
-    const uint32_t hb = __half_as_ushort(__float2half_rn(COMP ? mean * down * 0.875f : mean < INFINITY ? 1.0f : NAN));
+            (COMP ? 8.0f / 7.0f * __int_as_float((127 + e) << 23) : mean != 0.0f ? mean : 1.0f) * kShLog2e * rsqrtf((float)D);
+    const uint32_t hb = __half_as_ushort(__float2half_rn(COMP ? mean * down * 0.875f : mean < INFINITY ? (float)(mean != 0.0f) : NAN));
 #pragma unroll
     for (int k = 0; k < D / 64; ++k) {
         const int c = 32 * k + lane, d0 = 32 * (c / 16) + c % 16;

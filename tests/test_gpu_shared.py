@@ -407,3 +407,19 @@ def test_blocks_that_fill_fewer_warps(cuda, n, group, hkv, groups, prefix, d, co
     lens = [prefix + 1 + (7 * i) % 30 for i in range(n)]
     Batch(cuda, lens, [prefix - 40 * i for i in range(groups)], hkv, group, d, comp, 128, seed=n + d).check()
     assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("n,d,comp", [(3, 128, False), (40, 128, False), (40, 64, False), (40, 128, True), (24, 64, True)])
+def test_query_rows_of_zeros(cuda, n, d, comp):
+    """Padding tokens' queries: every score is 0, the output the mean of the values (in a prefix that ends inside a tile,
+    and with a page outside the pool)."""
+    b = Batch(cuda, [400] * n, [300], 2, 4, d, comp, 128, seed=19)
+    b.q[::2] = 0
+    b.q[1, 3] = -0.0
+    b.check()
+    assert _lib.device_error() == 0
+    hide = torch.zeros(b.pt.n_pages, 128, dtype=torch.bool, device=cuda)
+    hide[b.ids[0, 1, 1]] = True
+    b.pt.pages[1, 1] = -1
+    b.check(hide=hide)
+    assert _lib.device_error() == _lib.BC_DEVERR_PAGE
