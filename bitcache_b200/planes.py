@@ -523,10 +523,13 @@ def decode_attention_shared(q: torch.Tensor, K: Planes, V: Planes, pt: PageTable
     lib = _lib.load()
     st = _stream(q)
     group = heads // hkv
-    ws = _lib.workspace(q.device, st, lib.bc_decode_shared_workspace_bytes(n, groups, hkv, group, d), ("shared",))
+    # A workspace of the call's own, from torch's allocator: a captured call's belongs to its graph, and the
+    # launches of two threads on one stream may mix.  (Nothing has to be cleared.)
+    ws_bytes = lib.bc_decode_shared_workspace_bytes(n, groups, hkv, group, d)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
     _lib.check(lib.bc_decode_attention_shared(q.data_ptr(), K.c(), V.c(), pt.c(), lens, pre, out.data_ptr(), n, groups,
-                                              hkv, group, d, mode, _lib.ptr(ws), ws.numel() if ws is not None else 0,
-                                              st), "decode_attention_shared")
+                                              hkv, group, d, mode, ws.data_ptr(), ws_bytes, st),
+               "decode_attention_shared")
     return out
 
 

@@ -298,10 +298,11 @@ int bc_append_qkv_paged(bc_heads q, bc_heads k, bc_heads v, const int32_t* seq_i
  * A length of 0 gives zeros; a sequence shorter than its group's prefix attends its own
  * length of it.  Lengths outside [0, max_pages * page_size] are cut to it and raise
  * BC_DEVERR_INDEX; a page id outside the pool raises BC_DEVERR_PAGE and its keys are left
- * out.  head_dim 32, 64, 128 or 256, any group.  The workspace needs no clearing; calls
- * that overlap on the GPU must not share one; its size does not grow with every argument
- * (a larger batch may take another kernel), so it is asked for each shape.  No counterpart
- * in the reference. */
+ * out.  head_dim 32, 64, 128 or 256, any group.  The workspace needs no clearing.  A call
+ * is two to four launches: calls that overlap on the GPU must not share one, nor calls that
+ * several threads make on one stream, whose launches may mix; a captured call's has to live
+ * as long as its graph.  Its size does not grow with every argument (a larger batch may
+ * take another kernel), so it is asked for each shape.  No counterpart in the reference. */
 size_t bc_decode_shared_workspace_bytes(int n_seqs, int n_groups, int n_kv_heads, int group, int head_dim);
 int bc_decode_attention_shared(const void* q, bc_kv_planes K, bc_kv_planes V, bc_page_table pt,
                                const int32_t* seq_lens, const int32_t* prefix_lens, void* out, int n_seqs,

@@ -14,6 +14,8 @@ Doubled for the first three: (2^-9 + S 2^-14) E + 2^-11 |out| + 2^-24.
 Over a whole output the fp16 roundings are independent: their 2-norm is within
 2^-11 of |out| for each of the two, and 3 * 2^-11 is asked.
 """
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -423,3 +425,53 @@ def test_query_rows_of_zeros(cuda, n, d, comp):
     b.pt.pages[1, 1] = -1
     b.check(hide=hide)
     assert _lib.device_error() == _lib.BC_DEVERR_PAGE
+
+
+def test_threads_that_share_a_stream(cuda):
+    """A call is several launches: another thread's may come between them."""
+    batches = [Batch(cuda, [700 + 3 * i for i in range(24)], [640], 2, 4, 128, True, 128, seed=s) for s in (20, 21)]
+    for b in batches:
+        b.check()
+    first = [b.run() for b in batches]
+    wrong = [0, 0]
+
+    def work(i):
+        for _ in range(20):
+            outs = [batches[i].run() for _ in range(50)]
+            wrong[i] += sum(not torch.equal(o, first[i]) for o in outs)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == [0, 0] and _lib.device_error() == 0
+
+
+def test_a_captured_call_keeps_its_workspace(cuda):
+    """A graph of a small call, replayed after a larger call on the stream it was captured on, and on another one."""
+    small = Batch(cuda, [500, 520, 400, 410], [384], 2, 4, 128, True, 128, seed=22)
+    large = Batch(cuda, [900 + i for i in range(64)], [800], 2, 4, 128, True, 128, seed=23)
+    want, want_large = small.run(), large.run()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    out = torch.empty_like(small.q)
+    with torch.cuda.stream(s):
+        small.run(out=out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            small.run(out=out)
+        large.run()
+        filled = [torch.full((n,), 7, dtype=torch.uint8, device=cuda) for n in (1 << 16, 1 << 20, 1 << 22, 1 << 24) for _ in range(8)]
+        out.zero_()
+        graph.replay()
+    s.synchronize()
+    assert torch.equal(out, want)
+    assert all(bool((t == 7).all()) for t in filled)
+    for _ in range(20):  # the graph and calls on its stream may overlap
+        with torch.cuda.stream(s):
+            got = large.run()
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(got, want_large)
