@@ -331,10 +331,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
     sh_let_next();
     const int64_t total = sh_scan(a, L, scan);
     const int n_workers = sh_workers(L, total);
-    if ((int)blockIdx.x >= n_workers) return;
+    // A CTA without tiles waits too: with all prefixes empty nobody else would, and the end of this grid has to
+    // tell that of the queries' kernel.
+    if ((int)blockIdx.x >= n_workers) {
+        sh_wait_before();
+        return;
+    }
     ShCursor cur;
     sh_seek(a, L, scan, n_workers, blockIdx.x, cur);
-    if (cur.left <= 0) return;
+    if (cur.left <= 0) {
+        sh_wait_before();
+        return;
+    }
     if (tid == 0) {
         *dead = 0;
         for (int i = 0; i < kTcRaw; ++i) {

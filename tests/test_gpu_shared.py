@@ -475,3 +475,21 @@ def test_a_captured_call_keeps_its_workspace(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(got, want_large)
+
+
+def test_prefixes_of_no_keys(cuda):
+    """All prefixes empty, which only the device knows: the prefix kernel has nothing to do, and calls follow at once."""
+    b = Batch(cuda, [60 + i for i in range(40)], [0], 2, 4, 128, True, 128, seed=24)
+    b.check()
+    q = [b.q.clone(), b.q.flip(0).contiguous()]
+    want = []
+    for x in q:
+        b.q = x
+        want.append(b.check())
+    for _ in range(100):
+        got = []
+        for x in q:
+            b.q = x
+            got.append(b.run())
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+    assert _lib.device_error() == 0
