@@ -8,6 +8,12 @@
 //   K = [ bs sgn k | rs / 8 n ],  Q = [ h sgn q | q ] / 2^e,  h = fp16(7 / 8 mean|q|):
 //   s = 8 / 7 2^e Q . K,  2^e <= mean|q| < 2^(e + 1), so that Q is exact but for h.
 // (Without codes Q is sgn q, and s = mean|q| Q . K.)  V = bs sgn v + rs/7 n.
+// The rows of K and V of each half tile (64 keys) are held in a unit of their own, 2^(E - 28)
+// with E the exponent field of the half's largest scale, so that their largest elements
+// lie at 2^13 .. 2^16: small scales become no fp16 subnormals (in which rs / 7 of 2e-5
+// is 1% off), and bs + rs may pass the largest fp16.  K's unit goes back into the half's
+// scores, V's into its P.  (One warp finds the units as tiles arrive; when each role found
+// them for itself, 200000 keys before 32 rows took 219 us; 207 now, 199 without units.)
 // A row of zeros has Q = 0 and a factor above 0, so that hidden keys' -inf stays -inf.
 //
 // Roles of the 28 warps of a CTA, one CTA per SM:
@@ -28,7 +34,7 @@
 //          clocks a tile).
 //   24     issues the products: Q (tensor memory) x K, P (tensor memory) x V.
 //   25, 26 bring K's / V's packed tiles with 1-D bulk copies, three ahead.
-//   27     fills the last warpgroup.
+//   27     finds the units of K's and V's half tiles.
 // K's operand ring holds three half tiles (the sign part, the code part), V's two
 // tiles.
 //
@@ -44,12 +50,13 @@
 // keys, with four buffers, take as long each as those of 128: 229 us where these
 // take 195, 32 rows before 200000 keys.)
 //
-// Scores are scaled so that P = 2^(s - U) lies below 2^15, U rising when it would
-// not, to 2^8 above the largest.  Sums are fp32.  The elements of K, V and P, h and
+// Scores are scaled so that P = 2^(s - U) times V's unit lies below 2^15, U rising when
+// it would not, to 2^8 above the largest.  Sums are fp32.  The elements of K, V and P, h and
 // V's rs / 7 are rounded to fp16, the widest type that the tensor cores take at this
 // rate: with some channels four times the others, outputs are 5.0e-4 off the exact
 // ones, relative, of which their own fp16 rounding is 2.1e-4 and the five others 1.5e-4
 // to 2.8e-4 each, none of them by itself worth the instructions that would spare it.
+// Keys whose scales are below 2^-28 of their half tile's largest keep fewer bits.
 // The rows kernel, which scales products in fp32 and rounds P alone, has 2.9e-4.
 //
 // A barrier tells odd phases from even ones, no more: whoever waits on one has to
@@ -92,8 +99,9 @@ struct TcCfg {
     static constexpr int SCAN_OFF = (RAWV_OFF + kTcRaw * RAW_B + 15) / 16 * 16;
     static constexpr int XCH_OFF = SCAN_OFF;  // [2][128] units of the rows, [128] sums, once the list's sums are read
     static constexpr int BAR_OFF = SCAN_OFF + 512 * 4;
-    static constexpr int FLAG_OFF = BAR_OFF + 50 * 8;
-    static constexpr int SMEM_B = FLAG_OFF + 20 * 4 + 1024;  // + alignment to the swizzle atom
+    static constexpr int FLAG_OFF = BAR_OFF + 52 * 8;
+    static constexpr int UNIT_OFF = FLAG_OFF + 20 * 4;
+    static constexpr int SMEM_B = UNIT_OFF + 4 * 8 * 8 + 1024;  // + alignment to the swizzle atom
     // tensor memory columns
     static constexpr int S_COL = 0, O_COL = 256, Q_COL = 256 + D;
     static_assert(Q_COL + KE / 2 <= 512, "tensor memory");
@@ -101,7 +109,7 @@ struct TcCfg {
 
 enum TcBar {
     kRawKFull = 0, kRawKEmpty = 3, kRawVFull = 6, kRawVEmpty = 9, kKFull = 12, kKEmpty = 15, kVFull = 18, kVEmpty = 20,
-    kSFull = 22, kPFull = 26, kPvDone = 30, kQFull = 34, kDrain = 35, kPair = 36, kUnit = 40, kDone = 48, kTcBars = 49
+    kSFull = 22, kPFull = 26, kPvDone = 30, kQFull = 34, kDrain = 35, kPair = 36, kUnit = 40, kDone = 48, kScale = 49, kTcBars = 52
 };
 
 // ---- tcgen05 ---------------------------------------------------------------
@@ -266,6 +274,19 @@ __device__ __forceinline__ float2 tc_add2(float2 x, float2 y) {
     return *reinterpret_cast<float2*>(&r);
 }
 
+// Exponent field (0 .. 30) of the largest scale of a half tile's keys [lo, hi); bs: its packed scales.  A warp's call.
+// (An infinite or NaN scale counts as 2^15.)
+template <bool COMP>
+__device__ __forceinline__ int tc_half_exp(const uint8_t* bs, int lo, int hi) {
+    const int lane = threadIdx.x & 31, k = 2 * lane;
+    uint32_t w = reinterpret_cast<const uint32_t*>(bs)[lane] & 0x7FFF7FFFu;
+    if constexpr (COMP) w = __vmaxu2(w, reinterpret_cast<const uint32_t*>(bs + 2 * kTcTile)[lane] & 0x7FFF7FFFu);
+    const uint32_t a = k >= lo && k < hi ? w & 0xFFFFu : 0, b = k + 1 >= lo && k + 1 < hi ? w >> 16 : 0;
+    return min(30, (int)(__reduce_max_sync(0xffffffffu, max(a, b)) >> 10));
+}
+__device__ __forceinline__ float tc_pow2(int e) { return __int_as_float((127 + e) << 23); }
+__device__ __forceinline__ float half_at(const uint8_t* p) { return __half2float(*reinterpret_cast<const __half*>(p)); }
+
 // The query rows as A operands, one warp a row: [h sgn q | q] / 2^e in the order of
 // K's elements, and the scale of the row's scores in log2 units.  Ordered as the
 // prefix kernel's lanes read them: by group and kv head, then 16-byte unit, then
@@ -325,6 +346,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
     volatile int* vbad = flags + 8;    // [8]
     volatile int* dead = flags + 16;
     volatile uint32_t* tmem_at = reinterpret_cast<volatile uint32_t*>(flags + 17);
+    // unit of K's half tiles [2][8] (2^(28 - e), its inverse), and of V's (2^(28 - e), e - 28), tile i % 8
+    volatile float2* kunit = reinterpret_cast<volatile float2*>(smem + C::UNIT_OFF);
+    volatile float2* vunit = kunit + 16;
     const int tid = threadIdx.x, warp = (int)tc_uniform(tid >> 5), lane = tid & 31;
 
     // the queries' kernel has waited for all that came before; only its own results are waited for below
@@ -348,6 +372,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
         for (int i = 0; i < kTcRaw; ++i) {
             mbar_init(&bar[kRawKFull + i], 1);
             mbar_init(&bar[kRawVFull + i], 1);
+            mbar_init(&bar[kScale + i], 1);
             mbar_init(&bar[kRawKEmpty + i], kTcUnpackWarps);
             mbar_init(&bar[kRawVEmpty + i], kTcUnpackWarps);
         }
@@ -442,6 +467,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     const uint32_t s_at = lane_at + C::S_COL + 64 * (t & 3);
                     const int first = (cur.x.tile0 + cur.tile + i - begin) * kTcTile + 64 * half + key0;
                     const int lo = kbad[i & 7] ? 64 : cur.x.lo - first, hi = cur.x.hi - first;
+                    const float sk = sc * kunit[8 * half + (i & 7)].y, vup = vunit[8 * half + (i & 7)].x, ev = vunit[8 * half + (i & 7)].y;
                     uint32_t v[64];  // (with copies, 16 of them)
                     tc_ld16(s_at + key0, *reinterpret_cast<uint32_t(*)[16]>(v));
                     if (copies == 1) {
@@ -461,7 +487,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
 #pragma unroll
                         for (int k = 16; k < 64; ++k) m[k & 3] = fmaxf(m[k & 3], __uint_as_float(v[k]));
                     }
-                    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * sc;
+                    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * sk + ev;
                     if (t > 2 * begin) {
                         follow(t - 1);
                         if (!ok) break;
@@ -491,7 +517,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                     if (lane == 0) tc_arrive(&bar[kUnit + 2 * quad + half]);
                     // P of key k: column k / 2 of the half tile's, over scores that this warp has read
                     float2 sum = make_float2(0.0f, 0.0f);
-                    const float2 sc2 = make_float2(sc, sc), U2 = make_float2(-U, -U);
+                    const float2 sc2 = make_float2(sk, sk), U2 = make_float2(ev - U, ev - U);
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         if (c > 0 && copies > 1) continue;
@@ -513,7 +539,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                         for (int c = 0; c < 4; ++c)
                             if (c != copy) tc_st8(s_at + 8 * c, z);
                     }
-                    l += sum.x + sum.y;
+                    l += (sum.x + sum.y) * vup;
                     tc_wait_st();
                 } else if (lane == 0) {
                     tc_arrive(&bar[kUnit + 2 * quad + half]);  // (kUnit and kPair count every tile and piece)
@@ -591,13 +617,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                 for (const int end = i + sh_piece_tiles(cur); i < end; ++i) {
                     const int rs_ = i % kTcRaw;
                     const uint8_t* raw = smem + C::RAWK_OFF + rs_ * C::RAW_B;
-                    ok = tc_wait(&bar[kRawKFull + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
+                    ok = tc_wait(&bar[kScale + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
                     if (round) ok = ok && tc_wait(&bar[kKEmpty + slot], (round - 1) & 1u, dead);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
                     uint8_t* op = smem + slot * C::KOP_B + key * 128;
-                    const uint32_t bs = *reinterpret_cast<const uint16_t*>(raw + C::BS_OFF + 2 * key);
-                    const uint32_t flip = (bs | (bs << 16)) ^ 0x80008000u;
+                    const float up = kunit[8 * (key >> 6) + (i & 7)].x;
+                    const uint32_t flip = h2_bits(__float2half2_rn(half_at(raw + C::BS_OFF + 2 * key) * up)) ^ 0x80008000u;
 #pragma unroll 1
                     for (int w = part * (NW / 2); w < (part + 1) * (NW / 2); ++w) {
                         const uint32_t sg = reinterpret_cast<const uint32_t*>(raw)[key * NW + w];
@@ -616,8 +642,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         op = smem + slot * C::KOP_B + key * 128;
-                        const uint32_t rs = *reinterpret_cast<const uint16_t*>(raw + C::RS_OFF + 2 * key);
-                        const __half2 r8 = __hmul2(bits_h2(rs | (rs << 16)), bits_h2(0x30003000u));  // rs / 8
+                        const __half2 r8 = __float2half2_rn(half_at(raw + C::RS_OFF + 2 * key) * (up * 0.125f));
 #pragma unroll 1
                         for (int c = part * (NW / 2); c < (part + 1) * (NW / 2); ++c) {
                             const uint4 nb = *reinterpret_cast<const uint4*>(raw + C::SIGN_B + (key >> 3) * 4 * D + c * 128 + (key & 7) * 16);
@@ -646,17 +671,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
                 for (const int end = i + sh_piece_tiles(cur); i < end; ++i, pos += kTcTile) {
                     const int rs_ = i % kTcRaw, b = i % C::VST;
                     const uint8_t* raw = smem + C::RAWV_OFF + rs_ * C::RAW_B;
-                    ok = tc_wait(&bar[kRawVFull + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
+                    ok = tc_wait(&bar[kScale + rs_], (uint32_t)(i / kTcRaw) & 1u, dead);
                     if (i >= C::VST) ok = ok && tc_wait(&bar[kVEmpty + b], (uint32_t)(i / C::VST - 1) & 1u, dead);
                     ok = __all_sync(0xffffffffu, ok);
                     if (!ok) break;
-                    uint32_t bs = *reinterpret_cast<const uint16_t*>(raw + C::BS_OFF + 2 * key);
-                    uint32_t rs = COMP ? *reinterpret_cast<const uint16_t*>(raw + C::RS_OFF + 2 * key) : 0;
+                    const float up = vunit[8 * (key >> 6) + (i & 7)].x;
+                    float bs = half_at(raw + C::BS_OFF + 2 * key) * up, rs = COMP ? half_at(raw + C::RS_OFF + 2 * key) * (up * (1.0f / 7.0f)) : 0.0f;
                     // keys outside the prefix: P is 0 there, V has to be finite
-                    if (vbad[i & 7] || pos < cur.x.lo || pos >= cur.x.hi) bs = rs = 0;
+                    if (vbad[i & 7] || pos < cur.x.lo || pos >= cur.x.hi) bs = rs = 0.0f;
                     uint8_t* op = smem + C::V_OFF + b * C::VOP_B + key * 128;
-                    const uint32_t flip = (bs | (bs << 16)) ^ 0x80008000u;
-                    const __half2 r7 = __float2half2_rn(__half2float(__ushort_as_half((uint16_t)rs)) * (1.0f / 7.0f));
+                    const uint32_t flip = h2_bits(__float2half2_rn(bs)) ^ 0x80008000u;
+                    const __half2 r7 = __float2half2_rn(rs);
                     // chunk c: units 4c .. 4c + 3.  Nibble n of its word w is bit 4n + first of a sign
                     // word: word w, first c (head_dim 128); word w % 2, first 2c + w / 2 (64)
                     uint32_t sgw[NW];
@@ -824,6 +849,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) k_shared_prefix(const SharedArg
             // copies in flight land before the block's memory is given back (bounded)
             for (int t = max(0, i - kTcRaw); t < i; ++t)
                 tc_settle(&full[t % kTcRaw], (uint32_t)(t / kTcRaw) & 1u, dead);
+        }
+    }
+    if (warp == 27) {
+        // ---------------- units of the half tiles ----------------
+        bool ok = true;
+        int i = 0;
+        for (; ok && cur.left > 0; sh_next_piece(a, L, cur)) {
+            int at0 = (cur.x.tile0 + cur.tile) * kTcTile;
+#pragma unroll 1
+            for (const int end = i + sh_piece_tiles(cur); i < end; ++i, at0 += kTcTile) {
+                const int s = i % kTcRaw;
+                ok = tc_wait(&bar[kRawKFull + s], (uint32_t)(i / kTcRaw) & 1u, dead) &&
+                     tc_wait(&bar[kRawVFull + s], (uint32_t)(i / kTcRaw) & 1u, dead);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const uint8_t *k = smem + C::RAWK_OFF + s * C::RAW_B + C::BS_OFF, *v = smem + C::RAWV_OFF + s * C::RAW_B + C::BS_OFF;
+                const int lo = cur.x.lo - at0, khi = kbad[i & 7] ? 0 : cur.x.hi - at0, vhi = vbad[i & 7] ? 0 : cur.x.hi - at0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int ke = tc_half_exp<COMP>(k + 128 * h, lo - 64 * h, khi - 64 * h);
+                    const int ve = tc_half_exp<COMP>(v + 128 * h, lo - 64 * h, vhi - 64 * h);
+                    if (lane == 0) {
+                        volatile float2 &ku = kunit[8 * h + (i & 7)], &vu = vunit[8 * h + (i & 7)];
+                        ku.x = tc_pow2(28 - ke);
+                        ku.y = tc_pow2(ke - 28);
+                        vu.x = tc_pow2(28 - ve);
+                        vu.y = (float)(ve - 28);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) tc_arrive(&bar[kScale + s]);
+            }
         }
     }
     tc_leave(&bar[kDone]);

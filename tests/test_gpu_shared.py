@@ -493,3 +493,73 @@ def test_prefixes_of_no_keys(cuda):
             got.append(b.run())
         assert all(torch.equal(g, w) for g, w in zip(got, want))
     assert _lib.device_error() == 0
+
+
+def small_outputs(b):
+    """As check(); the whole output's bound allows for the fp16 rounding of subnormal elements, 2^-25 each."""
+    got = b.run()
+    out, tol = b.want()
+    err = (got.double() - out).abs()
+    assert torch.isfinite(got).all()
+    assert (err <= tol).all(), f"max error {err.max():.3g}, {(err / tol).max():.3g} of the tolerance"
+    assert err.norm() <= 3 * 2.0 ** -11 * out.norm() + 2.0 ** -25 * out.numel() ** 0.5
+
+
+@pytest.mark.parametrize("n", [3, 24, 40])
+@pytest.mark.parametrize("d,comp", [(128, True), (64, True), (128, False)])
+def test_small_value_scales(cuda, n, d, comp):
+    """Values whose scales are all about 2^-13 and less: fp16's subnormals, which the cache holds exactly; few keys, one of
+    them with most of the weight."""
+    b = Batch(cuda, [7] * n, [6], 2, 4, d, comp, 128, seed=25)
+    b.q *= 4
+    for factor in (2.0 ** -13, 2.0 ** -3, 2.0 ** -2):
+        b.V.bscale *= factor
+        if comp:
+            b.V.rscale *= factor
+        small_outputs(b)
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("n", [3, 24, 40])
+@pytest.mark.parametrize("d", [64, 128])
+def test_small_key_scales_and_large_queries(cuda, n, d):
+    """Key scales of about 2^-14; each query row lies along the code parts of two keys, so that their scores are large."""
+    b = Batch(cuda, [330] * n, [300], 2, 4, d, True, 128, seed=26)
+    for x in (b.K.bscale, b.K.rscale):
+        x *= 2.0 ** -14
+    code = values(b.K)[1][b.ids[0, :, 0].to(cuda)]  # [kv heads, keys, d]
+    code = (code / code.norm(dim=-1, keepdim=True)).repeat_interleave(4, 0)
+    r = torch.arange(n, device=cuda)
+    rows = code[:, (5 * r) % 64] + code[:, 64 + (7 * r) % 64]  # [heads, n, d]
+    b.q = (rows * (1.2e5 * (d / 128) ** 0.5)).clamp(-60000, 60000).transpose(0, 1).half().contiguous()
+    b.check()
+
+
+@pytest.mark.parametrize("n", [3, 24, 40])
+@pytest.mark.parametrize("d", [64, 128])
+def test_values_past_the_largest_fp16(cuda, n, d):
+    """Sign part and code part are finite in fp16, their sum is not; the outputs are means of many."""
+    b = Batch(cuda, [330] * n, [300], 2, 4, d, True, 128, seed=27)
+    for x in (b.V.bscale, b.V.rscale):
+        x[x == x] = 40000.0
+    b.check()
+
+
+@pytest.mark.parametrize("n", [3, 24, 40])
+@pytest.mark.parametrize("run", [1, 64, 128])
+def test_scales_of_many_sizes_in_a_tile(cuda, n, run):
+    """Runs of `run` keys whose value scales lie anywhere from 2^-14 to 2^6 of the others', keys' from 2^-8 on; large
+    scores favour some key of any size."""
+    b = Batch(cuda, [1000] * n, [1000], 2, 4, 128, True, 128, seed=28)
+    g = torch.Generator().manual_seed(run)
+    for h in range(2):
+        at = b.ids[0, h].to(cuda)
+        for P, low, high in ((b.V, -14, 6), (b.K, -8, 1)):
+            f = (2.0 ** torch.randint(low, high, (len(at) * 128 // run,), generator=g).repeat_interleave(run)).view(len(at), 128)
+            for x in (P.bscale, P.rscale):
+                x[at] = (x[at].float() * f.to(cuda)).half()
+                for i in range(1, n):  # the begun page's copies
+                    x[b.ids[i, h, 7], :104] = x[b.ids[0, h, 7], :104]
+    b.q *= 2
+    b.check()
+    assert _lib.device_error() == 0
