@@ -534,7 +534,14 @@ __global__ void __launch_bounds__(kRopeWarps * 32, APPEND ? 2 : 3) k_rope_lanes(
                     }
 #pragma unroll
                 for (int o = LPR / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const float inv = most > 0.0f ? __fdiv_rn(7.0f, most) : 0.0f;
+                float inv = most > 0.0f ? __fdiv_rn(7.0f, most) : 0.0f;
+                if (inv == INFINITY) {  // most below 2^-125: the clamped products are +-7 and 0 (and both scales 0)
+                    inv = 1.0f;
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x[y][j] = x[y][j] != 0.0f ? copysignf(7.0f, x[y][j]) : 0.0f;
+                }
                 any = inv > 0.0f;  // else (rows of zeros, rows that are not finite) all codes are 0
                 const uint16_t rb = f2h_bits(most);
                 rs = __half2float(__ushort_as_half(rb));

@@ -347,3 +347,35 @@ def test_refusals(cuda):
         with pytest.raises(RuntimeError):
             call()
     assert _lib.device_error() == 0
+
+
+def both_kernels(cuda, rows, dtype):
+    """Planes and hats of keys `rows` [T, d] by the aligned kernel and the any-alignment one."""
+    T, d = rows.shape
+    got = []
+    for offset in (0, 1):
+        store = torch.zeros(T * 3 * d + offset, dtype=dtype, device=cuda)
+        x = store[offset:].view(T, 3, d)
+        x[:, 1] = x[:, 2] = rows.to(cuda)
+        K, V, pt = cache(cuda, 1, 1, d, True, 128, 1, 4)
+        pos = torch.arange(T, dtype=torch.int32, device=cuda)
+        out = planes.append_qkv_paged(x[:, :1], x[:, 1:2], x[:, 2:], K, V, pt, torch.zeros_like(pos), pos,
+                                      planes.Rope(None, None), want_hat=True)
+        got.append([t for P in (K, V) for t in (P.sign, P.bscale, P.nib, P.rscale)] + list(out))
+    assert _lib.device_error() == 0
+    return got
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_append_of_rows_whose_residual_has_no_finite_inverse(cuda, d, dtype):
+    """Elements next to fp32's smallest: 7 / largest residual overflows, and all scales round to 0.  Codes are what the
+    clamped product gives (+-7, 0 for a residual of 0), the rows stand for zeros."""
+    g = torch.Generator().manual_seed(d)
+    rows = torch.randn(6, d, generator=g) * torch.tensor([1e-38, 1e-39, 3e-38, 1e-44, 0.0, 1.0])[:, None]
+    rows = rows.to(dtype)
+    lanes, plain = both_kernels(cuda, rows, dtype)
+    for a, b in zip(lanes, plain):
+        assert torch.equal(a, b)
+    for hat in lanes[-2:]:
+        assert torch.isfinite(hat).all() and not hat[:5].any() and hat[5].any()
