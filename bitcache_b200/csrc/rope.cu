@@ -574,14 +574,16 @@ __global__ void __launch_bounds__(kRopeWarps * 32, APPEND ? 2 : 3) k_rope_lanes(
                 }
             }
             if (encode && out) {  // the rows as the planes hold them
+                // codes of 0 times an infinite scale are NaN here too
+                const uint32_t base = __float_as_uint(any || rs == 0.0f ? held : NAN);
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                     float v[8];
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        v[j] = __uint_as_float(__float_as_uint(held) ^ (~pos_mask[y][j] & 0x80000000u));
+                        v[j] = __uint_as_float(base ^ (~pos_mask[y][j] & 0x80000000u));
                         if (any) {
-                            // code / 7 rounded to nearest: one correction of the product with 1 / 7
+                            // code / 7 rounded to nearest: one correction of the product with 1 / 7 (Markstein's)
                             constexpr float k7 = 1.0f / 7.0f;
                             const float code = __fsub_rn(x[y][j], kRound), q0 = __fmul_rn(code, k7);
                             const float q = __fmaf_rn(__fmaf_rn(q0, -7.0f, code), k7, q0);

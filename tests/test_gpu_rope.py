@@ -379,3 +379,18 @@ def test_append_of_rows_whose_residual_has_no_finite_inverse(cuda, d, dtype):
         assert torch.equal(a, b)
     for hat in lanes[-2:]:
         assert torch.isfinite(hat).all() and not hat[:5].any() and hat[5].any()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_hats_of_rows_that_are_not_finite(cuda, d, dtype):
+    """What the cache holds of a row with an infinity or NaN: sign * bscale + code / 7 * rscale, whichever kernel writes it."""
+    rows = torch.randn(4, d, generator=torch.Generator().manual_seed(d)).to(dtype)
+    rows[1, 3], rows[2, 5] = float("inf"), float("nan")
+    lanes, plain = both_kernels(cuda, rows, dtype)
+    for a, b in zip(lanes, plain):
+        if a.dtype.is_floating_point:
+            a, b = (torch.nan_to_num(t, nan=123.0) for t in (a, b))
+        assert torch.equal(a, b)
+    for hat in lanes[-2:]:
+        assert hat[1:3].isnan().all() and torch.isfinite(hat[[0, 3]]).all()
