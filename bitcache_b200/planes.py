@@ -534,6 +534,11 @@ def decode_attention_shared(q: torch.Tensor, K: Planes, V: Planes, pt: PageTable
 
 
 def _check_pool(K: Planes, V: Planes, pt: PageTable) -> None:
+    t = pt.pages
+    if not (t.is_cuda and t.dtype is torch.int32 and t.dim() == 2 and t.is_contiguous()):
+        raise RuntimeError("the block table must be a contiguous int32 CUDA tensor [rows, max_pages]")
+    if not (K.sign.is_cuda and V.sign.is_cuda):
+        raise RuntimeError("the page pools must be in GPU memory")
     for P in (K, V):
         if P.n_slots != pt.n_pages or P.kv_stride != pt.page_size:
             raise RuntimeError(f"the pool holds {P.n_slots} pages of {P.kv_stride} positions, "

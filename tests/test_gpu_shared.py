@@ -563,3 +563,19 @@ def test_scales_of_many_sizes_in_a_tile(cuda, n, run):
     b.q *= 2
     b.check()
     assert _lib.device_error() == 0
+
+
+def test_refusals_of_block_tables_and_pools(cuda):
+    b = Batch(cuda, [100, 200], [64], 2, 2, 128, True, 128, seed=29)
+    pool = planes.Planes.empty(b.pt.n_pages, 128, 128, True, torch.device("cpu"))
+    wide = torch.cat([b.pt.pages, b.pt.pages], 1)[:, :b.pt.pages.shape[1]]
+    tables = [b.pt.pages.long(), wide, b.pt.pages.cpu(), b.pt.pages.view(-1)]
+    q, k, v = (torch.zeros(2, h, 128, dtype=torch.float16, device=cuda) for h in (4, 2, 2))
+    ids = torch.zeros(2, dtype=torch.int32, device=cuda)
+    for K, V, t in [(b.K, b.V, t) for t in tables] + [(pool, b.V, b.pt.pages), (b.K, pool, b.pt.pages)]:
+        pt = planes.PageTable(t, 128, b.pt.n_pages)
+        with pytest.raises(RuntimeError):
+            planes.decode_attention_shared(b.q, K, V, pt, b.lens, b.prefixes)
+        with pytest.raises(RuntimeError):
+            planes.append_qkv_paged(q, k, v, K, V, pt, ids, ids, planes.Rope(None, None))
+    b.check()
