@@ -384,6 +384,8 @@ class Rope:
                     raise RuntimeError(f"{name} must be a contiguous float32 CUDA tensor [n_positions, rotary_dim / 2]")
             if cos.shape != sin.shape:
                 raise RuntimeError("cos and sin must have the same shape")
+            if cos.shape[0] == 0:
+                raise RuntimeError("cos and sin must have a row for each position")
         self.cos, self.sin, self.interleaved, self.eps = cos, sin, bool(interleaved), float(eps)
         self.q_weight, self.k_weight = (None if w is None else w.float().contiguous() for w in (q_weight, k_weight))
         n, half = (0, 0) if cos is None else cos.shape

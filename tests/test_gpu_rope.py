@@ -394,3 +394,9 @@ def test_hats_of_rows_that_are_not_finite(cuda, d, dtype):
         assert torch.equal(a, b)
     for hat in lanes[-2:]:
         assert hat[1:3].isnan().all() and torch.isfinite(hat[[0, 3]]).all()
+
+
+def test_refusal_of_tables_without_positions(cuda):
+    none = torch.zeros(0, 64, device=cuda)
+    with pytest.raises(RuntimeError):
+        planes.Rope(none, none)
