@@ -34,8 +34,7 @@ def nvcc() -> str:
 
 
 def _deps() -> list[str]:
-    return (glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(INCLUDE, "*.h"))
-            + glob.glob(os.path.join(INCLUDE, "*.cuh")) + [__file__])
+    return [f for d in (CSRC, INCLUDE) for end in ("*.h", "*.cuh") for f in glob.glob(os.path.join(d, end))] + [__file__]
 
 
 def _stale(target: str, deps: list[str]) -> bool:
