@@ -769,10 +769,11 @@ int sh_run(const SharedArgs& a, ShList& L, const ShList* tc, void* scratch, cuda
 bool sh_head_dim(int d) { return d == 32 || d == 64 || d == 128 || d == 256; }
 
 // More query rows than this behind one prefix: the prefix kernel, else the rows kernel, which reads the
-// prefix once per 8 rows.  At 65536 keys, rows kernel against prefix kernel: 16 rows 58.3 / 77.8 us, 20 rows
-// 81.0 / 78.7, 32 rows 103.8 / 80.4.  (Up to 8192 keys 32 rows too are still 7 us faster there, but lengths
-// are on the device.)
-constexpr int kShTcRows = 16;
+// prefix once per 8 rows.  Rows kernel against prefix kernel, 32 / 8 heads of 128: at 65536 keys 16 rows 59.3 /
+// 83.8 us, 24 rows 82.9 / 86.0, 32 rows 105.1 / 85.8; 24 rows at 8192 keys 23.0 / 31.4, at 200000 221.8 / 192.3;
+// at 65536 24 rows of heads of 64 60.2 / 74.9, without codes 50.7 / 67.8.  (Lengths are on the device: 32 rows
+// behind 1000 keys, 14.2 / 20.0, pay for those behind long prefixes.)
+constexpr int kShTcRows = 24;
 bool sh_takes_tc(int n_seqs, int n_groups, int group, int head_dim) {
     return (head_dim == 64 || head_dim == 128) && (int64_t)(n_seqs / n_groups) * group > kShTcRows && n_seqs > n_groups;
 }

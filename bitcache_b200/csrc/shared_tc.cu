@@ -921,7 +921,7 @@ ShList sh_tc_list(int n_seqs, int n_groups, int group) {
     L.rows = (int)((rows + L.pre_blocks - 1) / L.pre_blocks);
     L.rows = (L.rows + 7) / 8 * 8;
     // Up to 32 rows: four copies of the rows, each with a quarter of the keys, so that all softmax lanes work
-    // (32 rows: 195 us at 200000 keys, 203 with one copy; 59.8 and 58.4 at 32768).  Two copies of 33 to 64 rows
+    // (32 rows: 206 us at 200000 keys, 215 with one copy; 60.7 and 58.0 at 32768).  Two copies of 33 to 64 rows
     // cost more than they spare.
     L.copies = L.rows <= 32 ? 4 : 1;
     L.own_blocks = 1;
