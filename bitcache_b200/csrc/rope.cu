@@ -182,9 +182,10 @@ __global__ void __launch_bounds__(kRopeWarps * 32) k_rope_rows(const RopeArgs a)
 // registers.  The tree sums cost 10 shuffles for 4 rows here, 20 in the kernel above,
 // whose 2-byte loads also keep too little in flight.  Norm and rotation alone are
 // bound by HBM: 16384 tokens of 32 + 8 heads of 128, bf16, 72 us, 4.8 TB/s (the
-// same rows through registers instead of the lanes' rings of copies: 117 us).  The
-// append is bound by the instructions that encode 16 of a token's 48 rows: 24 prompts
-// of 512 to 1024 tokens, same heads, with k_hat and v_hat, 153 us, 3.2 TB/s.
+// same rows through registers instead of the lanes' rings of copies: 117 us; in the
+// kernel above 257).  The append is bound by the instructions that encode 16 of a
+// token's 48 rows and, with two CTAs an SM, by their latency: 24 prompts of
+// 512 to 1024 tokens, same heads, with k_hat and v_hat, 154 us, 3.2 TB/s (528 above).
 // ---------------------------------------------------------------------------
 template <int D>
 struct Lanes {
@@ -269,9 +270,9 @@ __device__ __forceinline__ void load8(const uint8_t* at, int y, float, float (&x
     x[4] = __uint_as_float(w.x), x[5] = __uint_as_float(w.y), x[6] = __uint_as_float(w.z), x[7] = __uint_as_float(w.w);
 }
 
-// Two products at once, each rounded as alone.  Only for products of products: the
-// assembler contracts a packed product with a packed sum behind it, whatever
-// rounding both name.
+// Two products at once, each rounded as alone.  Only for products of products: with a
+// packed sum behind a packed product, results were seen to differ from those of
+// operations rounded one by one.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     unsigned long long r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));

@@ -41,11 +41,11 @@
 // Keeping Q in tensor memory spares half of the score product's shared-memory
 // reads.  Per tile 96 KB are written, 96 KB read by the tensor cores and 43 KB of
 // packed bytes go in and out, 1900 clocks at 128 B each; the products take 1536, the
-// exponentials of 128 rows 1024.  What bounds it is the instructions of all roles,
-// about 2500 issue slots of a scheduler and tile (half of them unpacking), and the
-// chain from a tile's scores to the ones two tiles later in the same buffer: some
-// 3300 clocks a tile, and the start and end of an item besides.  128 sequences with
-// 8192 keys before them, 32 / 8 heads of 128: 74 us with the batch's own keys, of
+// exponentials of 128 rows 1024.  What bounds it: the chain from a tile's scores to the ones
+// two tiles later in the same buffer, and the instructions of all roles, about 2500
+// issue slots of a scheduler and tile (half of them unpacking; 55% of those there are),
+// some 3300 clocks a tile; with few tiles, an item's start and end besides, about half
+// of the time at 14 tiles a CTA.  128 sequences with 8192 keys before them, 32 / 8 heads of 128: 77 us with the batch's own keys, of
 // which the products at the tensor cores' rate would take 15.  (Score products of 64
 // keys, with four buffers, take as long each as those of 128: 229 us where these
 // take 195, 32 rows before 200000 keys.)
@@ -53,7 +53,7 @@
 // Scores are scaled so that P = 2^(s - U) times V's unit lies below 2^15, U rising when
 // it would not, to 2^8 above the largest.  Sums are fp32.  The elements of K, V and P, h and
 // V's rs / 7 are rounded to fp16, the widest type that the tensor cores take at this
-// rate: with some channels four times the others, outputs are 5.0e-4 off the exact
+// rate: with some channels four times the others, outputs are 5.0e-4 to 5.4e-4 off the exact
 // ones, relative, of which their own fp16 rounding is 2.1e-4 and the five others 1.5e-4
 // to 2.8e-4 each, none of them by itself worth the instructions that would spare it.
 // Keys whose scales are below 2^-28 of their half tile's largest keep fewer bits.

@@ -294,7 +294,8 @@ int bc_append_qkv_paged(bc_heads q, bc_heads k, bc_heads v, const int32_t* seq_i
  * them.  The sequences form n_groups equal runs; positions below prefix_lens[g] hold the
  * same rows in every sequence of group g (a common prompt: the same pages, or copies; not
  * checked) and are read once for the whole group, through the block table of its first
- * sequence.  prefix_lens NULL: nothing is shared.  A prefix may end anywhere in a page.
+ * sequence: the rows of that one have to name the prefix's pages as long as the group
+ * lives, even when its own length is 0.  prefix_lens NULL: nothing is shared.  A prefix may end anywhere in a page.
  * A length of 0 gives zeros; a sequence shorter than its group's prefix attends its own
  * length of it.  Lengths outside [0, max_pages * page_size] are cut to it and raise
  * BC_DEVERR_INDEX; a page id outside the pool raises BC_DEVERR_PAGE and its keys are left
